@@ -6,6 +6,7 @@ current device is not a gfx950, every entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -26,6 +27,8 @@ METHODS = {
     "crb_symdamp_norefine": 5,
 }
 METRICS = {"magnitude": 0, "hessian": 1}
+# enum crbq_reduction
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 c_i64 = ctypes.c_int64
 c_i32 = ctypes.c_int32
@@ -54,6 +57,7 @@ class CrbqBlockTrace(ctypes.Structure):
 TRACE_BYTES = ctypes.sizeof(CrbqBlockTrace)
 NOALLOC_SCRATCH_BYTES = 80 << 20      # CRBQ_NOALLOC_SCRATCH_BYTES (include/crbq.h)
 LINEAR_MAX_EX = 256                   # CRBQ_LINEAR_MAX_EX
+HEAD_MAX_K = 256                      # CRBQ_HEAD_MAX_K
 ERR_TOO_LARGE = -5                    # CRBQ_ERR_TOO_LARGE
 ERR_CAPTURE = -6                      # CRBQ_ERR_CAPTURE
 
@@ -118,6 +122,21 @@ _SIGS = {
     "crbq_linear_packed": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i64,
                                    c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_vp, c_size,
                                    c_vp]),
+    "crbq_head_state_floats": (c_size, [c_i64, c_i64]),
+    "crbq_head_workspace_size": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i32]),
+    "crbq_head_xent": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64,
+                               ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "crbq_head_xent_grad": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp,
+                                    c_i64, ctypes.c_float, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp,
+                                    c_i64, c_vp, c_size, c_vp]),
+    "crbq_head_distill": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp,
+                                  c_i32, c_i64, c_vp, c_i64, c_i32, c_vp, ctypes.c_float,
+                                  ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "crbq_head_distill_grad": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64,
+                                       c_i32, ctypes.c_float, ctypes.c_float, c_vp, c_vp, c_i32,
+                                       c_vp, c_i64, c_vp, c_i64, c_vp, c_size, c_vp]),
+    "crbq_top_logits": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, ctypes.c_float, c_vp,
+                                c_vp, c_vp, c_vp]),
 }
 
 _lock = threading.Lock()
@@ -180,6 +199,16 @@ def ready(device: torch.device | None = None) -> ctypes.CDLL:
 def stream_of(t: torch.Tensor) -> int:
     """torch.cuda.current_stream(t.device).cuda_stream, without the Stream object (1 us)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (kernels are launched
+    on the current device)."""
+    return (_same_device if device.index == torch.cuda.current_device()
+            else torch.cuda.device(device))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -1,0 +1,279 @@
+// 16-bit matrix-product tiles of the output-head kernels (head.hip).
+//
+// A workgroup of 8 wavefronts sums D[m][n] = sum_k A[m][k] B[n][k] over a
+// BM x BN tile on v_mfma_f32_16x16x32_{f16,bf16} (fp32 accumulate).  Each
+// operand comes in one of two layouts:
+//   K-contiguous (KC): element (row, k) at P[row * ld + k];
+//   K-strided:         element (row, k) at P[k * ld + row],
+// and is staged through LDS 64 k at a time by direct-to-LDS buffer loads
+// (16 bytes per lane, no register round trip).  A K-contiguous stage keeps
+// its rows as 128 bytes with the 16-byte chunks XOR-permuted by the row, a
+// K-strided stage keeps its 64 k rows as they are, chunks permuted by bits
+// 0, 1 and 3 of the row, and the lanes read their 8 consecutive k with LDS
+// transpose reads (ds_read_b64_tr_b16): either way half a wavefront's reads
+// fall on distinct banks.  What lies outside an operand (rows past its end, k past its
+// end) is turned into zeros by the buffer loads' range check, or, for the k
+// tail inside a K-contiguous row, by an offset beyond any range.
+//
+// The accumulators: element r of acc[i][j] of a lane is
+//   m = wm + 16 i + 4 (lane >> 4) + r,  n = wn + 16 j + (lane & 15),
+// so a lane holds 4 consecutive m of one n: the kernels take the output's
+// contiguous (or reduced) dimension as m.
+#pragma once
+#include "common.h"
+
+namespace crbq {
+
+typedef int i4_t __attribute__((ext_vector_type(4)));
+typedef __fp16 tr4_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef __attribute__((address_space(3))) tr4_t lds_tr4_t;
+
+constexpr int G_K = 64;                 // k per stage
+constexpr int G_THREADS = 512;
+constexpr int64_t G_MAX_LD = (int64_t)1 << 22;   // 256 rows * ld * 2 bytes < 2^31
+
+template <typename T8>
+__device__ __forceinline__ f4_t g_mfma(T8 a, T8 b, f4_t c);
+template <>
+__device__ __forceinline__ f4_t g_mfma<h8_t>(h8_t a, h8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f4_t g_mfma<b8_t>(b8_t a, b8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// LDS-only barrier: this wavefront's LDS operations, not its global loads.
+__device__ __forceinline__ void g_sync_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void g_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// One operand of a tile: `rows` x K elements from row0 on (`rows` = the rows
+// that exist from row0 to the operand's end; more than the tile's are fine).
+// The range check goes by whole 4-byte words: hence the even ends.
+struct GOperand {
+  const uint16_t* p;       // KC: &P[row0 * ld]; K-strided: &P[row0]
+  int64_t ld;
+  int64_t rows;            // rows (outputs) from row0 to the end; K-strided: even
+  int64_t K;               // k's that exist; KC: a multiple of 8
+  const uint64_t* live;    // K-strided only, may be null: bit k % 64 of word k / 64 clear =
+                           // row k reads as zeros, whatever it holds
+};
+
+__device__ __forceinline__ i4_t g_rsrc(const uint16_t* base, int64_t nrec) {
+  const uint64_t a = (uint64_t)base;
+  return i4_t{__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+              __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)),
+              __builtin_amdgcn_readfirstlane((int)nrec), 0x00020000};
+}
+
+// Row permutation of a K-strided stage (of 16-byte chunks, within 16).
+__device__ __forceinline__ int g_swz(int t) { return ((t & 3) | ((t >> 1) & 4)) << 1; }
+
+template <int R, bool KC>
+struct GStage {
+  static constexpr int BYTES = R * G_K * 2;
+  static constexpr int LOADS = BYTES / 1024;                     // 1 KB each
+  static constexpr int PER_WAVE = LOADS >= 8 ? LOADS / 8 : 1;    // fewer: some are issued twice
+  static constexpr int ROWS_PER_LOAD = KC ? 8 : 512 / R;
+  static_assert(KC ? R % 16 == 0 : (R == 128 || R == 256), "stage shape");
+
+  __device__ static int group(int wave, int kk) { return (wave * PER_WAVE + kk) % LOADS; }
+  // lane's row and 16-byte chunk (of the source) in load group g
+  __device__ static int row(int g, int lane) {
+    return KC ? 8 * g + (lane >> 3) : ROWS_PER_LOAD * g + lane / (R / 8);
+  }
+  __device__ static int chunk(int g, int lane) {
+    const int r = row(g, lane);
+    return KC ? (lane & 7) ^ (r & 7) : (lane % (R / 8)) ^ g_swz(r);
+  }
+  __device__ static unsigned voff(int g, int lane, int64_t ld) {
+    return (unsigned)((row(g, lane) * ld + chunk(g, lane) * 8) * 2);
+  }
+  // descriptor of the stage that starts at k0 of K
+  __device__ static i4_t rsrc(const GOperand& o, int64_t k0, int64_t K) {
+    const int64_t kl = K - k0;
+    int64_t n = 0;
+    if (KC) {
+      const int64_t rows = o.rows < R ? o.rows : R;
+      if (kl > 0) n = ((rows - 1) * o.ld + kl) * 2;
+      return g_rsrc(o.p + (kl > 0 ? k0 : 0), n);
+    }
+    const int64_t rows = kl < G_K ? kl : G_K;
+    if (kl > 0) n = ((rows - 1) * o.ld + o.rows) * 2;
+    return g_rsrc(o.p + (kl > 0 ? k0 * o.ld : 0), n);
+  }
+};
+
+__device__ __forceinline__ void g_load_lds(const void* dst, i4_t rs, unsigned voff) {
+  const unsigned d = __builtin_amdgcn_readfirstlane(
+      (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)dst);
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(d));
+}
+
+template <typename T8, int PITCH>
+__device__ __forceinline__ T8 g_tr_frag(const char* p) {
+  typedef __attribute__((address_space(3))) const char lchar;
+  lchar* q = (lchar*)(const void*)p;
+  const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4_t*)(q));
+  const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4_t*)(q + 4 * PITCH));
+  struct P { tr4_t a, b; } v{lo, hi};
+  return __builtin_bit_cast(T8, v);
+}
+
+// Tile geometry: WGM x WGN wavefronts, NS stages in LDS (NS - 1 in flight).
+template <int BM_, int BN_, int WGM_, int NS_, bool AKC_, bool BKC_>
+struct GTile {
+  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = 8 / WGM_, NS = NS_;
+  static constexpr bool AKC = AKC_, BKC = BKC_;
+  static constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 16, NJ = WN / 16;
+  using SA = GStage<BM, AKC>;
+  using SB = GStage<BN, BKC>;
+  static constexpr int STAGE = SA::BYTES + SB::BYTES;
+  static constexpr int LDS = NS * STAGE;
+  static constexpr int LW = SA::PER_WAVE + SB::PER_WAVE;         // loads of a wavefront, a stage
+  static_assert(LDS <= 160 * 1024 && MI >= 1 && NJ >= 1 && (NS - 2) * LW <= 63, "tile shape");
+};
+
+// acc = the tile's sums over k in [k_beg, k_end): both multiples of 64, or k_end
+// the operands' end (where theirs differ, the shorter one's; what the longer
+// one holds behind it meets zeros and has to be finite).  On return every
+// wavefront has left the stages.
+template <typename T8, typename G>
+__device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOperand& B,
+                                       int64_t k_beg, int64_t k_end,
+                                       f4_t (&acc)[G::MI][G::NJ]) {
+  using SA = typename G::SA;
+  using SB = typename G::SB;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = (wave / G::WGN) * G::WM, wn = (wave % G::WGN) * G::WN;
+  const int nch = k_end > k_beg ? (int)((k_end - k_beg + G_K - 1) / G_K) : 0;
+  constexpr unsigned OUT = 0x80000000u;
+  unsigned va[SA::PER_WAVE], vb[SB::PER_WAVE];
+#pragma unroll
+  for (int q = 0; q < SA::PER_WAVE; ++q) va[q] = SA::voff(SA::group(wave, q), lane, A.ld);
+#pragma unroll
+  for (int q = 0; q < SB::PER_WAVE; ++q) vb[q] = SB::voff(SB::group(wave, q), lane, B.ld);
+  const int kc8 = ((lane & 7) ^ ((lane >> 3) & 7)) * 8;          // a KC lane's first k
+  // fragment addresses within a stage (bytes)
+  const int r16 = lane & 15, gq = lane >> 4;
+  const int trow = 8 * gq + (r16 >> 2), fsw = g_swz(trow);
+  int fa[G::MI], fb[G::NJ];
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+    const int ch = wm + 16 * i + 4 * (r16 & 3);
+    fa[i] = G::AKC ? (wm + 16 * i + r16) * (G_K * 2)
+                   : trow * G::BM * 2 + (((ch >> 3) ^ fsw) << 4) + (ch & 7) * 2;
+  }
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int ch = wn + 16 * j + 4 * (r16 & 3);
+    fb[j] = SA::BYTES + (G::BKC ? (wn + 16 * j + r16) * (G_K * 2)
+                                : trow * G::BN * 2 + (((ch >> 3) ^ fsw) << 4) + (ch & 7) * 2);
+  }
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+  // load q of a stage's LW loads of this wavefront
+  struct Src {
+    i4_t ra, rb;
+    bool kin;              // KC lanes: this lane's chunk lies before K
+    uint64_t live;
+  };
+  auto source = [&](int c) {
+    const int64_t k0 = k_beg + (int64_t)c * G_K;
+    Src s;
+    s.ra = SA::rsrc(A, k0, c < nch ? A.K : 0);                  // past the end: all zeros
+    s.rb = SB::rsrc(B, k0, c < nch ? B.K : 0);
+    s.kin = k0 + kc8 < (G::BKC ? B.K : A.K);
+    s.live = ~0ull;
+    if (!G::AKC && A.live) s.live = c < nch ? A.live[k0 / G_K] : 0;
+    return s;
+  };
+  auto load = [&](int c, int q, const Src& s) {
+    char* buf = smem + (c % G::NS) * G::STAGE;
+    if (q < SA::PER_WAVE) {
+      const int g = SA::group(wave, q);
+      unsigned v = va[q < SA::PER_WAVE ? q : 0];
+      if (G::AKC) v = s.kin ? v : OUT;
+      else v = ((s.live >> SA::row(g, lane)) & 1) ? v : OUT;
+      g_load_lds(buf + g * 1024, s.ra, v);
+    } else {
+      const int qb = q - SA::PER_WAVE, g = SB::group(wave, qb);
+      unsigned v = vb[qb >= 0 && qb < SB::PER_WAVE ? qb : 0];
+      if (G::BKC) v = s.kin ? v : OUT;
+      g_load_lds(buf + SA::BYTES + g * 1024, s.rb, v);
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < G::NS - 1; ++c) {
+    const Src s = source(c);
+#pragma unroll
+    for (int q = 0; q < G::LW; ++q) load(c, q, s);
+  }
+  g_wait_vm<(G::NS - 2) * G::LW>();
+  g_sync_lds();
+  for (int c = 0; c < nch; ++c) {
+    const Src s = source(c + G::NS - 1);
+    const char* cur = smem + (c % G::NS) * G::STAGE;
+#pragma unroll
+    for (int h = 0; h < G_K / 32; ++h) {
+      // KC: the lane's chunk (gq + 4 h) of rows that share r16's low 3 bits
+      const int kc = ((gq + 4 * h) ^ (r16 & 7)) << 4;
+      auto fragA = [&](int i) -> T8 {
+        if constexpr (G::AKC) return *(const T8*)(cur + fa[i] + kc);
+        else return g_tr_frag<T8, G::BM * 2>(cur + fa[i] + h * 32 * G::BM * 2);
+      };
+      auto fragB = [&](int j) -> T8 {
+        if constexpr (G::BKC) return *(const T8*)(cur + fb[j] + kc);
+        else return g_tr_frag<T8, G::BN * 2>(cur + fb[j] + h * 32 * G::BN * 2);
+      };
+      T8 bb[G::NJ];
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) bb[j] = fragB(j);
+      T8 an = fragA(0);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) {
+        const T8 a = an;
+        if (i + 1 < G::MI) an = fragA(i + 1);
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a, bb[j], acc[i][j]);
+        if (h == 0) {
+          // the stage's loads between the MFMAs of its first half
+#pragma unroll
+          for (int q = 0; q < G::LW; ++q)
+            if (q * G::MI / G::LW == i) load(c + G::NS - 1, q, s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    g_wait_vm<(G::NS - 2) * G::LW>();
+    g_sync_lds();
+  }
+  g_wait_vm<0>();
+  g_sync_lds();
+}
+
+// Workgroup id -> linear index such that the workgroups one XCD receives
+// (every 8th id) take consecutive indices.
+__device__ __forceinline__ int g_xcd(int id, int nwg) {
+  const int q = nwg / 8, r = nwg % 8, x = id % 8, k = id / 8;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + k;
+}
+// Linear index -> (m tile, n tile) in bands of 8 n tiles: 32 consecutive
+// indices (an XCD's CUs) form a 4 x 8 block of tiles that shares 12 panels.
+__device__ __forceinline__ void g_band(int lin, int nm, int nn, int& tm, int& tn) {
+  const int per = nm * 8, band = lin / per, n0 = band * 8;
+  const int w = nn - n0 < 8 ? nn - n0 : 8, in = lin - band * per;
+  tm = in / w;
+  tn = n0 + in % w;
+}
+
+}  // namespace crbq

@@ -1,0 +1,880 @@
+// Losses of a causal LM's output head over a large vocabulary, on MFMA, with
+// their gradients and without keeping the logits.  (No counterpart in the
+// reference, whose perplexity computes all logits and calls a cross
+// entropy, eval_ppl_utils.py:626-636.)
+//
+// With z[t][v] = s sum_c h[t][c] W[v][c] and S_t the tokens listed for row t
+// (cross entropy: its label, with probability 1; distillation: the teacher's
+// k largest, with probabilities p and, optionally, a tail of probability
+// p_T that stands for all other tokens together):
+//   a_t    = log sum_{v not in S_t} exp z[t][v]
+//   lse_t  = log(exp a_t + sum_{S_t} exp z[t][v])
+//   loss_t = sum_{S_t} p_v (log p_v - z[t][v] + lse_t) + p_T (log p_T - a_t + lse_t)
+// (a token listed twice: both entries' terms in the loss, its p_v in the
+// gradient their sum),
+// and with q_v = exp(z_v - lse), q_T = exp(a - lse):
+//   dloss_t/dz_v = m q_v - p_v                   v in S_t (cross entropy: -q_T)
+//                = (m q_T - p_T) exp(z_v - a)    otherwise
+// where m = sum p + p_T: 1, unless the teacher's numbers do not add up.
+// The sum a_t leaves the listed tokens out from the start, so that neither
+// a confident row's loss nor its gradient is a difference of nearly equal
+// numbers.
+//
+// Forward: one product over tiles of vocabulary x tokens whose epilogue
+// keeps, per token, the running maximum and sum of exponentials of the tile
+// (fp32) and the listed tokens' own z; a second kernel joins the tiles.
+// Backward: per piece of the vocabulary, the product again with an epilogue
+// that writes the piece's dz (16 bits, the operand of the two products that
+// follow), then dh += dz W (fp32 sums) and dW = dz^T h.  dz is rounded to the inputs'
+// type as the gradients themselves are: its error (at most 2^-8 or 2^-11 of it, independent
+// from element to element) is that of the final rounding again.  It is scaled by a
+// power of two (fp16) and by the largest row coefficient so that it stays in range.
+#include "gemm16.h"
+
+namespace crbq {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int PAD_IDX = 0x7fffffff;     // an empty slot of a row's list
+
+__device__ __forceinline__ float g_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+template <typename T8> struct Half;
+template <> struct Half<h8_t> { typedef _Float16 t; };
+template <> struct Half<b8_t> { typedef __bf16 t; };
+template <typename T8>
+__device__ __forceinline__ uint16_t to16(float x) {
+  return __builtin_bit_cast(uint16_t, (typename Half<T8>::t)x);
+}
+// dz is kept times this: |dz| <= 1, below fp16's 65504 with room
+template <typename T8>
+constexpr float dz_scale() { return __is_same(T8, h8_t) ? 16384.f : 1.f; }
+
+// lanes that differ in bits 4 and 5 (the four 16-lane groups): max and sum
+__device__ __forceinline__ float gmax4(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float gsum4(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// (m, s): maximum and sum of exp(x - m); joins two such pairs
+__device__ __forceinline__ void ms_join(float& m, float& s, float m2, float s2) {
+  const float mm = fmaxf(m, m2);
+  const float x = m == mm ? s : s * g_exp(m - mm);        // m = -inf = mm: s is 0
+  const float y = m2 == mm ? s2 : s2 * g_exp(m2 - mm);
+  m = mm;
+  s = x + y;
+}
+// log(exp a + exp b)
+__device__ __forceinline__ float log_add(float a, float b) {
+  const float m = fmaxf(a, b), d = -fabsf(a - b);
+  return m == -INFINITY ? m : (d == d ? m + log1pf(expf(d)) : a + b);
+}
+
+// Where the listed tokens of the rows are (forward).
+struct Listed {
+  const int64_t* labels;   // cross entropy: one per row
+  const uint32_t* mask;    // distillation: a bit per (row, token), ldm words a row
+  const int32_t* sidx;     //   and each row's k tokens, ascending, PAD_IDX behind them
+  int64_t ldm;
+  int k;
+};
+
+// ---------------------------------------------------------------------------
+// forward product: partial (max, sum) of every (row, tile row of wavefronts)
+// and the listed tokens' z
+// ---------------------------------------------------------------------------
+template <typename T8, typename G, bool XENT>
+__global__ __launch_bounds__(G_THREADS) void k_head_fwd(
+    const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ W, int64_t ldw,
+    int64_t T, int64_t V, int64_t C, float scale, Listed ls, int nm, int nn, float2* part,
+    int64_t npart, float* zt) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  int tm, tn;
+  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
+  const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
+  const GOperand A{W + v0 * ldw, ldw, V - v0, C, nullptr};
+  const GOperand B{h + t0 * ldh, ldh, T - t0, C, nullptr};
+  f4_t acc[G::MI][G::NJ];
+  g_tile<T8, G>(smem, A, B, 0, C, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wr = wave / G::WGN;
+  const int64_t vw = v0 + wr * G::WM;                  // the wavefront's first token
+  const int g4 = (lane >> 4) * 4;
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
+    const bool ok = t < T;
+    int lab = -1;                                      // the label's place among the wavefront's
+    uint32_t words[G::WM / 32];
+    if (XENT) {
+      const int64_t y = ok ? ls.labels[t] : -1;
+      lab = y >= vw && y < vw + G::WM ? (int)(y - vw) : -1;
+    } else {
+#pragma unroll
+      for (int w = 0; w < G::WM / 32; ++w)
+        words[w] = ok ? ls.mask[t * ls.ldm + (vw >> 5) + w] : 0u;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int o = 16 * i + g4 + r;
+        float x = acc[i][j][r] * scale;
+        const bool hit = XENT ? o == lab : ((words[i / 2] >> (o & 31)) & 1) != 0;
+        if (hit) {
+          if (XENT) {
+            zt[t] = x;
+          } else {
+            // the token's slot in its row's ascending list
+            const int32_t* s = ls.sidx + t * ls.k;
+            const int v = (int)(vw + o);
+            int lo = 0, hi = ls.k - 1;
+            while (lo < hi) {
+              const int md = (lo + hi) >> 1;
+              if (s[md] < v) lo = md + 1;
+              else hi = md;
+            }
+            zt[t * ls.k + lo] = x;
+          }
+        }
+        x = hit || vw + o >= V ? -INFINITY : x;
+        acc[i][j][r] = x;
+        m = fmaxf(m, x);
+      }
+    m = gmax4(m);
+    float s = 0.f;
+    const float mb = m == -INFINITY ? 0.f : m;         // nothing left: exp(-inf) = 0
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += g_exp(acc[i][j][r] - mb);
+    s = gsum4(s);
+    if (ok && lane < 16) part[t * npart + (int64_t)tm * G::WGM + wr] = make_float2(m, s);
+  }
+}
+
+// The saved state of a forward, in floats: a [T], lse [T], one factor (1 or
+// 1 / the rows a mean is over), one unused; then cross entropy: z of the
+// label [T]; distillation: p_T [T], sum of p log p over the listed entries
+// [T], m [T], and of the lists' distinct tokens z [T][k], p [T][k] and, ascending,
+// the tokens themselves (int32) [T][k].
+struct State {
+  float *a, *lse, *inv, *pt, *ent, *mass, *zt, *p;
+  int32_t* sidx;
+  __host__ __device__ State(float* b, int64_t T, int64_t k) {
+    a = b;
+    lse = a + T;
+    inv = lse + T;
+    pt = inv + 2;
+    ent = pt + T;
+    mass = ent + T;
+    zt = k ? mass + T : pt;
+    p = zt + T * k;
+    sidx = (int32_t*)(p + T * k);
+  }
+};
+
+// Joins a row's partial sums and finishes its loss; a wavefront a row.  A
+// row that is left out (ignored label, empty list) has loss 0; rows[t] < 0
+// never holds otherwise, so its count flag goes beside it.
+template <bool XENT>
+__global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ part, int64_t npart,
+                                                   int64_t T, int64_t V, int k,
+                                                   const int64_t* __restrict__ labels,
+                                                   int64_t ignore, State st, float* rows,
+                                                   uint8_t* live, int reduction) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && reduction == 0) st.inv[0] = 1.f;
+  if (t >= T) return;
+  float m = -INFINITY, s = 0.f;
+  for (int64_t i = lane; i < npart; i += 64) {
+    const float2 p = part[t * npart + i];
+    ms_join(m, s, p.x, p.y);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) ms_join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  const float a = m + logf(s);                         // -inf where every token is listed
+  float loss, lse;
+  bool on;
+  if (XENT) {
+    const int64_t y = labels[t];
+    on = y != ignore;
+    const bool in = y >= 0 && y < V;
+    const float z = in ? st.zt[t] : NAN;               // a label outside: NaN, loss and gradient
+    const float d = a - z;
+    loss = d > 0.f ? d + log1pf(expf(-d)) : log1pf(expf(d));
+    lse = in ? z + loss : NAN;
+    if (d != d) loss = d;
+    if (!on) loss = 0.f;
+  } else {
+    float tm = -INFINITY, ts = 0.f, np = 0.f;
+    for (int i = lane; i < k; i += 64)
+      if (st.sidx[t * k + i] != PAD_IDX) {
+        ms_join(tm, ts, st.zt[t * k + i], 1.f);
+        np += 1.f;
+      }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) ms_join(tm, ts, __shfl_xor(tm, d), __shfl_xor(ts, d));
+    on = wave_sum_f(np) > 0.f;
+    lse = log_add(a, tm + logf(ts));
+    float l = 0.f;
+    for (int i = lane; i < k; i += 64) {
+      const float p = st.p[t * k + i];
+      if (st.sidx[t * k + i] != PAD_IDX && !(p == 0.f)) l += p * (lse - st.zt[t * k + i]);
+    }
+    loss = wave_sum_f(l) + st.ent[t];
+    float pt = st.pt[t];
+    if (a == -INFINITY) {                              // no token is left for the tail
+      if (lane == 0) {
+        st.mass[t] -= pt;
+        st.pt[t] = 0.f;
+      }
+      pt = 0.f;
+    }
+    if (!(pt == 0.f)) loss += pt * (logf(pt) - a + lse);
+    if (!on) loss = 0.f;
+  }
+  if (lane == 0) {
+    st.a[t] = a;
+    st.lse[t] = lse;
+    rows[t] = loss;
+    if (live) live[t] = on;
+  }
+}
+
+// Sum or mean of the rows' losses, in a fixed order, by one workgroup.
+__global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ rows,
+                                                      const uint8_t* __restrict__ live, int64_t T,
+                                                      int mean, float* loss, float* inv) {
+  __shared__ float ls[16], lc[16];
+  float s = 0.f, c = 0.f;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) {
+    s += rows[t];
+    c += live[t] ? 1.f : 0.f;
+  }
+  s = wave_sum_f(s);
+  c = wave_sum_f(c);
+  if ((threadIdx.x & 63) == 0) {
+    ls[threadIdx.x >> 6] = s;
+    lc[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = c = 0.f;
+    for (int w = 0; w < 16; ++w) {
+      s += ls[w];
+      c += lc[w];
+    }
+    loss[0] = mean ? s / c : s;                        // a mean over no row: NaN
+    inv[0] = mean ? (c > 0.f ? 1.f / c : 0.f) : 1.f;
+  }
+}
+
+__global__ void k_fill_u32(uint32_t* p, int64_t n, uint32_t v) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x)
+    p[i] = v;
+}
+
+// The teacher's list of each row: tokens ascending, probabilities, the
+// bits of the forward product.  One wavefront a row.  Tokens outside
+// [0, V) are empty slots; of one listed twice the list holds one entry with
+// the sum of its probabilities.
+constexpr int LIST_MAX = 256;
+template <typename TV>
+__global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t ldv,
+                                             const int32_t* __restrict__ idx, int64_t ldi,
+                                             const float* __restrict__ tlse, float itemp,
+                                             int64_t V, int k, State st, uint32_t* mask,
+                                             int64_t ldm) {
+  __shared__ int ix[LIST_MAX];
+  __shared__ float pr[LIST_MAX];
+  const int lane = threadIdx.x;
+  const int64_t t = blockIdx.x;
+  float m = -INFINITY;
+  for (int i = lane; i < k; i += 64) {
+    const int v = idx[t * ldi + i];
+    const float x = (float)val[t * ldv + i] * itemp;
+    ix[i] = v >= 0 && v < V ? v : -1;
+    pr[i] = x;
+    if (ix[i] >= 0) m = fmaxf(m, x);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = tlse ? tlse[t] : m;
+  float s = 0.f;
+  for (int i = lane; i < k; i += 64) {
+    pr[i] = ix[i] >= 0 ? expf(pr[i] - ref) : 0.f;
+    s += pr[i];
+  }
+  s = wave_sum_f(s);
+  __syncthreads();
+  const float norm = tlse ? 1.f : 1.f / s;
+  float ent = 0.f;
+  for (int i = lane; i < k; i += 64) {
+    const float p = pr[i] * norm;
+    if (ix[i] >= 0 && !(p == 0.f)) ent += p * logf(p);
+  }
+  ent = wave_sum_f(ent);
+  // first occurrences, and their probabilities with the repeats'
+  int mine[LIST_MAX / 64];
+  float prob[LIST_MAX / 64];
+#pragma unroll
+  for (int q = 0; q < LIST_MAX / 64; ++q) {
+    const int i = lane + 64 * q;
+    mine[q] = -1;
+    prob[q] = 0.f;
+    if (i < k && ix[i] >= 0) {
+      bool first = true;
+      for (int j = 0; j < k; ++j)
+        if (ix[j] == ix[i]) {
+          if (j < i) first = false;
+          prob[q] += pr[j];
+        }
+      mine[q] = first ? ix[i] : -1;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < LIST_MAX / 64; ++q)
+    if (lane + 64 * q < k) {
+      ix[lane + 64 * q] = mine[q];
+      st.sidx[t * k + lane + 64 * q] = PAD_IDX;
+      st.p[t * k + lane + 64 * q] = 0.f;
+      st.zt[t * k + lane + 64 * q] = 0.f;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < LIST_MAX / 64; ++q)
+    if (mine[q] >= 0) {
+      int rank = 0;
+      for (int j = 0; j < k; ++j) rank += ix[j] >= 0 && ix[j] < mine[q];
+      st.sidx[t * k + rank] = mine[q];
+      st.p[t * k + rank] = prob[q] * norm;
+      atomicOr(mask + t * ldm + (mine[q] >> 5), 1u << (mine[q] & 31));
+    }
+  if (lane == 0) {
+    st.ent[t] = ent;
+    st.pt[t] = tlse && s < 1.f ? 1.f - s : 0.f;
+    st.mass[t] = tlse && !(s < 1.f) ? s : 1.f;         // NaN stays NaN
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// max |g| over the rows, one workgroup (a gradient per row)
+__global__ __launch_bounds__(1024) void k_absmax(const float* __restrict__ g, int64_t T,
+                                                 float* out) {
+  __shared__ float l[16];
+  float m = 0.f;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) m = fmaxf(m, fabsf(g[t]));
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) l[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, l[w]);
+    out[0] = m;
+  }
+}
+
+// Row coefficients: dz of a row = coef (q - p) is stored relative to the
+// largest one, times dz_scale; *fac undoes both where the sums are rounded.
+// live: bit t set where the row's coefficient is not 0 (the other rows of h
+// are read as zeros: a masked row's NaN stays out of dW).
+// rowb[t] = the row's factor of exp(z - a); ratio[t] its share of the largest
+// coefficient, times dz_scale.
+template <bool XENT>
+__global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T, int k,
+                                                  const int64_t* __restrict__ labels,
+                                                  int64_t ignore, const float* __restrict__ g,
+                                                  int per_row, const float* __restrict__ gmax,
+                                                  float zscale, float scale, float* rowb,
+                                                  float* ratio, uint64_t* live, float* fac) {
+  const int64_t t = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  float r = 0.f;
+  const float big = per_row ? gmax[0] : 1.f;
+  if (t < T) {
+    bool on = true;
+    if (XENT) on = labels[t] != ignore;
+    else on = st.sidx[t * k] != PAD_IDX;               // sorted: an empty list starts empty
+    if (on) r = per_row ? (big == 0.f ? 0.f : g[t] / big) : 1.f;
+    r = r * zscale;
+    const float a = st.a[t], qt = expf(a - st.lse[t]);
+    ratio[t] = r;
+    rowb[t] = r == 0.f ? 0.f : r * (XENT ? qt : st.mass[t] * qt - st.pt[t]);
+  }
+  const uint64_t bits = __ballot(!(r == 0.f));
+  if (threadIdx.x == 0) live[blockIdx.x] = bits;
+  if (t == 0) fac[0] = (per_row ? big : g[0] * st.inv[0]) * (scale / zscale);
+}
+
+// dz of a piece of the vocabulary: dz[t][v - vbeg] = rowb exp(z - a), zeros
+// in the columns past the vocabulary; the listed tokens' own follow (k_dz_listed).
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dz(
+    const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ W, int64_t ldw,
+    int64_t T, int64_t nv, int64_t C, float scale, const float* __restrict__ a,
+    const float* __restrict__ rowb, int nm, int nn, uint16_t* dz, int64_t ldz) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  int tm, tn;
+  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
+  const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
+  const GOperand A{W + v0 * ldw, ldw, nv - v0, C, nullptr};
+  const GOperand B{h + t0 * ldh, ldh, T - t0, C, nullptr};
+  f4_t acc[G::MI][G::NJ];
+  g_tile<T8, G>(smem, A, B, 0, C, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t vw = v0 + (wave / G::WGN) * G::WM;
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
+    if (t >= T) continue;
+    const float b = rowb[t], at = a[t];
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i) {
+      const int64_t v = vw + 16 * i + 4 * (lane >> 4);
+      uint16_t o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = b * g_exp(acc[i][j][r] * scale - at);
+        o[r] = b == 0.f || v + r >= nv ? 0 : to16<T8>(x);
+      }
+      if (v < ldz)
+        *(uint2*)(dz + t * ldz + v) = make_uint2(o[0] | (uint32_t)o[1] << 16,
+                                                 o[2] | (uint32_t)o[3] << 16);
+    }
+  }
+}
+
+// the listed tokens' dz within [vbeg, vbeg + nv)
+template <typename T8, bool XENT>
+__global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
+                                                   const int64_t* __restrict__ labels,
+                                                   const float* __restrict__ ratio, int64_t vbeg,
+                                                   int64_t nv, uint16_t* dz, int64_t ldz) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = XENT ? e : e / k;
+  if (t >= T) return;
+  const int64_t v = XENT ? labels[t] : (int64_t)st.sidx[e];
+  if (v < vbeg || v >= vbeg + nv || (!XENT && v == PAD_IDX)) return;
+  const float r = ratio[t], lse = st.lse[t];
+  float d;
+  if (XENT) d = -expf(st.a[t] - lse);
+  else d = st.mass[t] * expf(st.zt[e] - lse) - st.p[e];
+  dz[t * ldz + v - vbeg] = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
+}
+
+// dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the split's v
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dh(
+    const uint16_t* __restrict__ W, int64_t ldw, const uint16_t* __restrict__ dz, int64_t ldz,
+    int64_t T, int64_t nv, int64_t C, int64_t span, int nm, int nn, float* P, int add) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  int tm, tn;
+  const int lin = g_xcd(blockIdx.x, gridDim.x), split = lin / (nm * nn);
+  g_band(lin - split * nm * nn, nm, nn, tm, tn);
+  const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
+  const int64_t kb = split * span, ke = kb + span < nv ? kb + span : nv;
+  const GOperand A{W + c0, ldw, C - c0, nv, nullptr};
+  const GOperand B{dz + t0 * ldz, ldz, T - t0, ldz, nullptr};
+  f4_t acc[G::MI][G::NJ];
+  g_tile<T8, G>(smem, A, B, kb, ke, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  P += (int64_t)split * T * C;
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
+    if (t >= T) continue;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i) {
+      const int64_t c = c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4);
+      if (c >= C) continue;
+      float4* q = (float4*)(P + t * C + c);
+      float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+      if (add) {
+        const float4 u = *q;
+        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+      }
+      *q = v;
+    }
+  }
+}
+
+// dh = fac * (P[0] + P[1] + ...), rounded once; 4 channels a thread
+template <typename T8>
+__global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int ns, int64_t T,
+                                                int64_t C, const float* __restrict__ fac,
+                                                uint16_t* dh, int64_t ldd) {
+  const int64_t n4 = T * (C / 4);
+  const float f = fac[0];
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n4; e += (int64_t)gridDim.x * 256) {
+    float4 v = *(const float4*)(P + e * 4);
+    for (int s = 1; s < ns; ++s) {
+      const float4 u = *(const float4*)(P + (int64_t)s * T * C + e * 4);
+      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
+    const int64_t t = e / (C / 4), c = (e - t * (C / 4)) * 4;
+    *(uint2*)(dh + t * ldd + c) =
+        make_uint2(to16<T8>(f * v.x) | (uint32_t)to16<T8>(f * v.y) << 16,
+                   to16<T8>(f * v.z) | (uint32_t)to16<T8>(f * v.w) << 16);
+  }
+}
+
+// dW[v][c] = fac * sum_t dz[t][v] h[t][c] of a piece's rows v
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dw(
+    const uint16_t* __restrict__ h, int64_t ldh, const uint64_t* __restrict__ live,
+    const uint16_t* __restrict__ dz, int64_t ldz, int64_t T, int64_t nv, int64_t C, int nm,
+    int nn, const float* __restrict__ fac, uint16_t* dW, int64_t ldo) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  int tm, tn;
+  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
+  const int64_t c0 = (int64_t)tm * G::BM, v0 = (int64_t)tn * G::BN;
+  const GOperand A{h + c0, ldh, C - c0, T, live};
+  const GOperand B{dz + v0, ldz, ldz - v0, T, nullptr};
+  f4_t acc[G::MI][G::NJ];
+  g_tile<T8, G>(smem, A, B, 0, T, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const float f = fac[0];
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    const int64_t v = v0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
+    if (v >= nv) continue;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i) {
+      const int64_t c = c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4);
+      if (c >= C) continue;
+      *(uint2*)(dW + v * ldo + c) = make_uint2(
+          to16<T8>(f * acc[i][j][0]) | (uint32_t)to16<T8>(f * acc[i][j][1]) << 16,
+          to16<T8>(f * acc[i][j][2]) | (uint32_t)to16<T8>(f * acc[i][j][3]) << 16);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// Tiles of the products (m x n): vocabulary x tokens for z, channels x tokens
+// for dh, channels x vocabulary for dW.
+using ZL = GTile<256, 256, 2, 2, true, true>;
+using ZM = GTile<256, 64, 4, 4, true, true>;
+using ZS = GTile<256, 16, 8, 4, true, true>;
+using HL = GTile<256, 256, 2, 2, false, true>;
+using HM = GTile<256, 64, 4, 4, false, true>;
+using HS = GTile<256, 16, 8, 4, false, true>;
+using WL = GTile<256, 256, 2, 2, false, false>;
+
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// tokens per tile: 0 = 16, 1 = 64, 2 = 256
+static int token_tile(int64_t T) { return T <= 16 ? 0 : T <= 64 ? 1 : 2; }
+static int64_t n_part(int64_t T, int64_t V) {
+  static const int wgm[3] = {ZS::WGM, ZM::WGM, ZL::WGM};
+  return cdiv(V, 256) * wgm[token_tile(T)];
+}
+static int64_t mask_words(int64_t V) { return cdiv(V, 256) * 8; }
+
+// Vocabulary of a backward piece: dz of a piece in about 128 MB (it is read
+// back by two products: within the 256 MB of the last-level cache), at
+// least 8192 tokens of the vocabulary.
+static int64_t piece_of(int64_t T, int64_t V) {
+  int64_t p = ((int64_t)64 << 20) / T / 256 * 256;
+  if (p < 8192) p = 8192;
+  const int64_t all = cdiv(V, 256) * 256;
+  return p < all ? p : all;
+}
+// Parts that dh's sum over a piece is split into, to fill 256 CUs.
+static int dh_splits(int64_t T, int64_t C, int64_t piece) {
+  static const int bn[3] = {16, 64, 256};
+  const int64_t tiles = cdiv(C, 256) * cdiv(T, bn[token_tile(T)]);
+  int64_t s = 512 / tiles;
+  const int64_t most = piece / 512;                    // 8 stages each at least
+  if (s > most) s = most;
+  if (s > 32) s = 32;
+  return (int)(s < 1 ? 1 : s);
+}
+
+struct FwdWs {
+  float2* part;
+  float* rows;
+  uint8_t* live;
+  uint32_t* mask;
+  size_t bytes;
+  FwdWs(void* ws, size_t cap, int64_t T, int64_t V, int64_t k, bool& ok) {
+    WsCarver w(ws, cap);
+    part = w.take<float2>((size_t)(T * n_part(T, V)));
+    rows = w.take<float>((size_t)T);
+    live = w.take<uint8_t>((size_t)T);
+    mask = k ? w.take<uint32_t>((size_t)(T * mask_words(V))) : nullptr;
+    bytes = w.off;
+    ok = w.ok();
+  }
+};
+
+struct GradWs {
+  int64_t piece;
+  int ns;
+  uint16_t* dz;
+  float *P, *rowb, *ratio, *fac, *gmax;
+  uint64_t* live;
+  size_t bytes;
+  GradWs(void* ws, size_t cap, int64_t T, int64_t V, int64_t C, bool& ok) {
+    WsCarver w(ws, cap);
+    piece = piece_of(T, V);
+    ns = dh_splits(T, C, piece);
+    dz = w.take<uint16_t>((size_t)(T * piece));
+    P = w.take<float>((size_t)(T * C) * ns);
+    rowb = w.take<float>((size_t)T);
+    ratio = w.take<float>((size_t)T);
+    fac = w.take<float>(1);
+    gmax = w.take<float>(1);
+    live = w.take<uint64_t>((size_t)cdiv(T, 64));
+    bytes = w.off;
+    ok = w.ok();
+  }
+};
+
+static bool bad_matrix(const void* p, int64_t ld, int64_t C) {
+  return !p || ld < C || ld >= G_MAX_LD || (ld & 7) || (((uintptr_t)p) & 15);
+}
+static int check_head(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
+                      int64_t T, int64_t V, int64_t C) {
+  if (dtype != CRBQ_F16 && dtype != CRBQ_BF16) return CRBQ_ERR_ARG;
+  if (T < 1 || V < 1 || C < 8 || (C & 7) || V >= ((int64_t)1 << 31) - 256 ||
+      T >= ((int64_t)1 << 31) - 256)
+    return CRBQ_ERR_ARG;
+  if (bad_matrix(h, ldh, C) || bad_matrix(W, ldw, C)) return CRBQ_ERR_ARG;
+  if (cdiv(V, 256) * cdiv(T, 16) >= ((int64_t)1 << 31)) return CRBQ_ERR_ARG;
+  return CRBQ_OK;
+}
+
+template <typename T8, typename G, bool XENT>
+static void launch_fwd(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw, int64_t T,
+                       int64_t V, int64_t C, float scale, const Listed& ls, const FwdWs& w,
+                       float* zt, hipStream_t s) {
+  const int nm = (int)cdiv(V, G::BM), nn = (int)cdiv(T, G::BN);
+  k_head_fwd<T8, G, XENT><<<(unsigned)((int64_t)nm * nn), G_THREADS, 0, s>>>(
+      h, ldh, W, ldw, T, V, C, scale, ls, nm, nn, w.part, n_part(T, V), zt);
+}
+
+template <typename T8, bool XENT>
+static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, int64_t V,
+                    int64_t C, float scale, const Listed& ls, int64_t ignore, int reduction,
+                    float* loss, const State& st, const FwdWs& w, hipStream_t s) {
+  const uint16_t *hh = (const uint16_t*)h, *ww = (const uint16_t*)W;
+  switch (token_tile(T)) {
+    case 0: launch_fwd<T8, ZS, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s); break;
+    case 1: launch_fwd<T8, ZM, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s); break;
+    default: launch_fwd<T8, ZL, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s);
+  }
+  CRBQ_LAUNCH_CHECK();
+  float* rows = reduction ? w.rows : loss;
+  k_head_join<XENT><<<(unsigned)cdiv(T, 4), 256, 0, s>>>(w.part, n_part(T, V), T, V, ls.k,
+                                                         ls.labels, ignore, st, rows,
+                                                         reduction ? w.live : nullptr, reduction);
+  CRBQ_LAUNCH_CHECK();
+  if (reduction) {
+    k_head_reduce<<<1, 1024, 0, s>>>(w.rows, w.live, T, reduction == CRBQ_MEAN, loss, st.inv);
+    CRBQ_LAUNCH_CHECK();
+  }
+  return CRBQ_OK;
+}
+
+template <typename T8, typename GZ, typename GH, bool XENT>
+static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw, int64_t T,
+                     int64_t V, int64_t C, const int64_t* labels, int64_t ignore, int k,
+                     float scale, const State& st, const float* g, int per_row, uint16_t* dh,
+                     int64_t ldd, uint16_t* dW, int64_t ldo, const GradWs& w, hipStream_t s) {
+  if (per_row) {
+    k_absmax<<<1, 1024, 0, s>>>(g, T, w.gmax);
+    CRBQ_LAUNCH_CHECK();
+  }
+  const float zs = dz_scale<T8>();
+  k_grad_rows<XENT><<<(unsigned)cdiv(T, 64), 64, 0, s>>>(st, T, k, labels, ignore, g, per_row,
+                                                         w.gmax, zs, scale, w.rowb, w.ratio,
+                                                         w.live, w.fac);
+  CRBQ_LAUNCH_CHECK();
+  const int nt = (int)cdiv(T, GZ::BN);
+  for (int64_t v = 0; v < V; v += w.piece) {
+    const int64_t nv = V - v < w.piece ? V - v : w.piece, ldz = cdiv(nv, 256) * 256;
+    const uint16_t* Wv = W + v * ldw;
+    const int nm = (int)cdiv(nv, GZ::BM);
+    k_head_dz<T8, GZ><<<(unsigned)(nm * nt), G_THREADS, 0, s>>>(
+        h, ldh, Wv, ldw, T, nv, C, scale, st.a, w.rowb, nm, nt, w.dz, ldz);
+    CRBQ_LAUNCH_CHECK();
+    k_dz_listed<T8, XENT><<<(unsigned)cdiv(XENT ? T : T * k, 256), 256, 0, s>>>(
+        st, T, k, labels, w.ratio, v, nv, w.dz, ldz);
+    CRBQ_LAUNCH_CHECK();
+    if (dh) {
+      const int mh = (int)cdiv(C, GH::BM);
+      const int64_t span = cdiv(cdiv(w.piece, w.ns), 64) * 64;
+      k_head_dh<T8, GH><<<(unsigned)(mh * nt * w.ns), G_THREADS, 0, s>>>(
+          Wv, ldw, w.dz, ldz, T, nv, C, span, mh, nt, w.P, v > 0);
+      CRBQ_LAUNCH_CHECK();
+    }
+    if (dW) {
+      const int mw = (int)cdiv(C, WL::BM), nw = (int)cdiv(nv, WL::BN);
+      k_head_dw<T8, WL><<<(unsigned)(mw * nw), G_THREADS, 0, s>>>(
+          h, ldh, w.live, w.dz, ldz, T, nv, C, mw, nw, w.fac, dW + v * ldo, ldo);
+      CRBQ_LAUNCH_CHECK();
+    }
+  }
+  if (dh) {
+    const int64_t nb = cdiv(T * (C / 4), 256);
+    k_dh_out<T8><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, s>>>(w.P, w.ns, T, C, w.fac, dh,
+                                                                   ldd);
+    CRBQ_LAUNCH_CHECK();
+  }
+  return CRBQ_OK;
+}
+
+template <typename T8, bool XENT>
+static int head_grad_t(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T,
+                       int64_t V, int64_t C, const int64_t* labels, int64_t ignore, int k,
+                       float scale, const State& st, const float* g, int per_row, void* dh,
+                       int64_t ldd, void* dW, int64_t ldo, const GradWs& w, hipStream_t s) {
+  const uint16_t *hh = (const uint16_t*)h, *ww = (const uint16_t*)W;
+  uint16_t *oh = (uint16_t*)dh, *ow = (uint16_t*)dW;
+  switch (token_tile(T)) {
+    case 0:
+      return head_grad<T8, ZS, HS, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
+                                         g, per_row, oh, ldd, ow, ldo, w, s);
+    case 1:
+      return head_grad<T8, ZM, HM, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
+                                         g, per_row, oh, ldd, ow, ldo, w, s);
+    default:
+      return head_grad<T8, ZL, HL, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
+                                         g, per_row, oh, ldd, ow, ldo, w, s);
+  }
+}
+
+static bool bad_reduction(int r) { return r != CRBQ_NONE && r != CRBQ_MEAN && r != CRBQ_SUM; }
+
+}  // namespace crbq
+
+using namespace crbq;
+
+extern "C" size_t crbq_head_state_floats(int64_t T, int64_t k) {
+  if (T < 1 || k < 0 || k > CRBQ_HEAD_MAX_K) return 0;
+  return (size_t)(k ? (3 * k + 5) * T + 2 : 3 * T + 2);
+}
+
+extern "C" size_t crbq_head_workspace_size(int64_t T, int64_t V, int64_t C, int64_t k, int grad) {
+  if (T < 1 || V < 1 || C < 1 || k < 0 || k > CRBQ_HEAD_MAX_K) return 0;
+  bool ok;
+  return grad ? GradWs(nullptr, 0, T, V, C, ok).bytes : FwdWs(nullptr, 0, T, V, k, ok).bytes;
+}
+
+extern "C" int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
+                              int64_t T, int64_t V, int64_t C, const int64_t* labels,
+                              int64_t ignore_index, float scale, int reduction, float* loss,
+                              float* state, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
+  if (!labels || !loss || !state || bad_reduction(reduction)) return CRBQ_ERR_ARG;
+  bool ok;
+  const FwdWs w(ws, ws_bytes, T, V, 0, ok);
+  if (!ok) return CRBQ_ERR_WORKSPACE;
+  const Listed ls{labels, nullptr, nullptr, 0, 0};
+  const State st(state, T, 0);
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == CRBQ_F16
+             ? head_fwd<h8_t, true>(h, ldh, W, ldw, T, V, C, scale, ls, ignore_index, reduction,
+                                    loss, st, w, s)
+             : head_fwd<b8_t, true>(h, ldh, W, ldw, T, V, C, scale, ls, ignore_index, reduction,
+                                    loss, st, w, s);
+}
+
+extern "C" int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
+                                   int dtype, int64_t T, int64_t V, int64_t C,
+                                   const int64_t* labels, int64_t ignore_index, float scale,
+                                   const float* state, const float* g, int g_per_row, void* dh,
+                                   int64_t ldd, void* dW, int64_t ldo, void* ws, size_t ws_bytes,
+                                   void* stream) {
+  if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
+  if (!labels || !state || !g || (!dh && !dW)) return CRBQ_ERR_ARG;
+  if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
+  bool ok;
+  const GradWs w(ws, ws_bytes, T, V, C, ok);
+  if (!ok) return CRBQ_ERR_WORKSPACE;
+  const State st((float*)state, T, 0);
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == CRBQ_F16
+             ? head_grad_t<h8_t, true>(h, ldh, W, ldw, T, V, C, labels, ignore_index, 1, scale, st,
+                                       g, g_per_row, dh, ldd, dW, ldo, w, s)
+             : head_grad_t<b8_t, true>(h, ldh, W, ldw, T, V, C, labels, ignore_index, 1, scale, st,
+                                       g, g_per_row, dh, ldd, dW, ldo, w, s);
+}
+
+extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int64_t ldw,
+                                 int dtype, int64_t T, int64_t V, int64_t C, const void* top_val,
+                                 int val_dtype, int64_t ldv, const int32_t* top_idx, int64_t ldi,
+                                 int k, const float* top_lse, float scale, float temperature,
+                                 int reduction, float* loss, float* state, void* ws,
+                                 size_t ws_bytes, void* stream) {
+  if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
+  if (!top_val || !top_idx || !loss || !state || bad_reduction(reduction) || k < 1 ||
+      k > CRBQ_HEAD_MAX_K || ldv < k || ldi < k || !(temperature > 0.f))
+    return CRBQ_ERR_ARG;
+  if (val_dtype != CRBQ_F32 && val_dtype != CRBQ_F16 && val_dtype != CRBQ_BF16)
+    return CRBQ_ERR_ARG;
+  bool ok;
+  const FwdWs w(ws, ws_bytes, T, V, k, ok);
+  if (!ok) return CRBQ_ERR_WORKSPACE;
+  const State st(state, T, k);
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t ldm = mask_words(V), nw = T * ldm;
+  k_fill_u32<<<(unsigned)(cdiv(nw, 1024) < 2048 ? cdiv(nw, 1024) : 2048), 256, 0, s>>>(w.mask, nw,
+                                                                                       0u);
+  CRBQ_LAUNCH_CHECK();
+  const float it = 1.f / temperature;
+  if (val_dtype == CRBQ_F32)
+    k_list<float><<<(unsigned)T, 64, 0, s>>>((const float*)top_val, ldv, top_idx, ldi, top_lse, it,
+                                             V, k, st, w.mask, ldm);
+  else if (val_dtype == CRBQ_F16)
+    k_list<_Float16><<<(unsigned)T, 64, 0, s>>>((const _Float16*)top_val, ldv, top_idx, ldi,
+                                                top_lse, it, V, k, st, w.mask, ldm);
+  else
+    k_list<__bf16><<<(unsigned)T, 64, 0, s>>>((const __bf16*)top_val, ldv, top_idx, ldi, top_lse,
+                                              it, V, k, st, w.mask, ldm);
+  CRBQ_LAUNCH_CHECK();
+  const Listed ls{nullptr, w.mask, st.sidx, ldm, k};
+  return dtype == CRBQ_F16 ? head_fwd<h8_t, false>(h, ldh, W, ldw, T, V, C, scale * it, ls, 0,
+                                                   reduction, loss, st, w, s)
+                           : head_fwd<b8_t, false>(h, ldh, W, ldw, T, V, C, scale * it, ls, 0,
+                                                   reduction, loss, st, w, s);
+}
+
+extern "C" int crbq_head_distill_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
+                                      int dtype, int64_t T, int64_t V, int64_t C, int k,
+                                      float scale, float temperature, const float* state,
+                                      const float* g, int g_per_row, void* dh, int64_t ldd,
+                                      void* dW, int64_t ldo, void* ws, size_t ws_bytes,
+                                      void* stream) {
+  if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
+  if (!state || !g || (!dh && !dW) || k < 1 || k > CRBQ_HEAD_MAX_K || !(temperature > 0.f))
+    return CRBQ_ERR_ARG;
+  if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
+  bool ok;
+  const GradWs w(ws, ws_bytes, T, V, C, ok);
+  if (!ok) return CRBQ_ERR_WORKSPACE;
+  const State st((float*)state, T, k);
+  hipStream_t s = (hipStream_t)stream;
+  const float sc = scale * (1.f / temperature);
+  return dtype == CRBQ_F16
+             ? head_grad_t<h8_t, false>(h, ldh, W, ldw, T, V, C, nullptr, 0, k, sc, st, g,
+                                        g_per_row, dh, ldd, dW, ldo, w, s)
+             : head_grad_t<b8_t, false>(h, ldh, W, ldw, T, V, C, nullptr, 0, k, sc, st, g,
+                                        g_per_row, dh, ldd, dW, ldo, w, s);
+}

@@ -533,3 +533,197 @@ def linear_packed(codes: torch.Tensor, lut: torch.Tensor, sal: torch.Tensor, C: 
                                  y.stride(0), ptr(ws), nws, stream_of(y)),
           "crbq_linear_packed")
     return y
+
+
+# -- losses of the output head -------------------------------------------------
+def _one_gpu(what, *ts):
+    dev = ts[0].get_device()                     # -1 on the CPU
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in ts):
+        raise _lib.CrbqError(f"{what}: its tensors must live on the GPU, on one device")
+
+
+def _head_matrix(x: torch.Tensor) -> torch.Tensor:
+    """x [n, C] as the head kernels read it: rows of a multiple of 8 elements
+    (zeros behind the last channel) that start at multiples of 16 bytes."""
+    C = x.shape[1]
+    if C % 8:
+        y = torch.zeros((x.shape[0], (C + 7) // 8 * 8), dtype=x.dtype, device=x.device)
+        y[:, :C] = x
+        return y
+    if x.shape[0] == 1 and x.stride(1) == 1 and x.data_ptr() % 16 == 0:
+        return x.as_strided((1, C), (C, 1))      # the stride of a single row says nothing
+    if x.stride(1) != 1 or x.stride(0) < C or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _head_pair(what, h, W):
+    _one_gpu(what, h, W)
+    if h.dtype not in (torch.float16, torch.bfloat16) or W.dtype != h.dtype:
+        raise _lib.CrbqError(f"{what} takes hidden states and a weight that are both fp16 or both "
+                             f"bf16, not {h.dtype} and {W.dtype}")
+    if h.dim() != 2 or W.dim() != 2 or h.shape[1] != W.shape[1] or 0 in h.shape or 0 in W.shape:
+        raise _lib.CrbqError(f"{what} takes hidden states [T, C] and a weight [V, C], not "
+                             f"{tuple(h.shape)} and {tuple(W.shape)}")
+    return _head_matrix(h), _head_matrix(W)
+
+
+def _reduction(what, reduction):
+    if reduction not in _lib.REDUCTIONS:
+        raise _lib.CrbqError(f"{what}: reduction {reduction!r} is none of "
+                             f"{sorted(_lib.REDUCTIONS)}")
+    return _lib.REDUCTIONS[reduction]
+
+
+def _head_buffers(lib, h, W, k, red, dev):
+    T, C = h.shape
+    nws = int(lib.crbq_head_workspace_size(T, W.shape[0], C, k, 0))
+    state = torch.empty(int(lib.crbq_head_state_floats(T, k)), dtype=torch.float32, device=dev)
+    loss = torch.empty((T,) if red == 0 else (), dtype=torch.float32, device=dev)
+    return loss, state, _ws(nws, dev), nws
+
+
+def head_xent(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, scale: float = 1.0,
+              ignore_index: int = -100, reduction: str = "mean"):
+    """Cross entropy of the logits scale * h W^T (never kept) against labels
+    [T] int64.  Returns (loss fp32 [T] or scalar, state for head_xent_grad)."""
+    hp, Wp = _head_pair("head_xent", h, W)
+    _one_gpu("head_xent", h, labels)
+    if labels.dtype != torch.int64 or labels.shape != h.shape[:1]:
+        raise _lib.CrbqError("head_xent takes int64 labels [T]")
+    labels = labels.contiguous()
+    red = _reduction("head_xent", reduction)
+    lib = _lib.ready(h.device)
+    with _lib.on_device(h.device):
+        loss, state, ws, nws = _head_buffers(lib, hp, Wp, 0, red, h.device)
+        check(lib.crbq_head_xent(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
+                                 _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0], hp.shape[1],
+                                 labels.data_ptr(), int(ignore_index), float(scale), red,
+                                 loss.data_ptr(), state.data_ptr(), ws.data_ptr(), nws,
+                                 stream_of(h)), "crbq_head_xent")
+    return loss, state
+
+
+def _grad_args(what, hp, Wp, state, g, need_h, need_w, lib):
+    """Output buffers (padded like their inputs), workspace and g of a gradient call."""
+    _one_gpu(what, hp, state, g)
+    if not (need_h or need_w):
+        raise _lib.CrbqError(f"{what}: no gradient asked for")
+    if g.dtype != torch.float32 or g.dim() > 1 or (g.dim() == 1 and g.shape != hp.shape[:1]):
+        raise _lib.CrbqError(f"{what} takes an fp32 loss gradient, one number or [T]")
+    dh = torch.empty_like(hp, memory_format=torch.contiguous_format) if need_h else None
+    dW = torch.empty_like(Wp, memory_format=torch.contiguous_format) if need_w else None
+    T, C = hp.shape
+    nws = int(lib.crbq_head_workspace_size(T, Wp.shape[0], C, 0, 1))
+    return dh, dW, _ws(nws, hp.device), nws, g.contiguous()
+
+
+def _out_args(dh, dW):
+    return (ptr(dh), dh.stride(0) if dh is not None else 0, ptr(dW),
+            dW.stride(0) if dW is not None else 0)
+
+
+def _cut(x, C):
+    return x if x is None or x.shape[1] == C else x[:, :C].contiguous()
+
+
+def head_xent_grad(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, state: torch.Tensor,
+                   g: torch.Tensor, scale: float = 1.0, ignore_index: int = -100,
+                   need_h: bool = True, need_w: bool = True):
+    """(dh, dW) (None where not asked for) of head_xent's loss times g: one
+    fp32 number, or [T] for reduction "none"."""
+    hp, Wp = _head_pair("head_xent_grad", h, W)
+    lib = _lib.ready(h.device)
+    labels = labels.contiguous()
+    with _lib.on_device(h.device):
+        dh, dW, ws, nws, g = _grad_args("head_xent_grad", hp, Wp, state, g, need_h, need_w, lib)
+        check(lib.crbq_head_xent_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
+                                      _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0], hp.shape[1],
+                                      labels.data_ptr(), int(ignore_index), float(scale),
+                                      state.data_ptr(), g.data_ptr(), int(g.dim() == 1),
+                                      *_out_args(dh, dW), ws.data_ptr(), nws, stream_of(h)),
+              "crbq_head_xent_grad")
+    return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])
+
+
+def head_distill(h: torch.Tensor, W: torch.Tensor, top_val: torch.Tensor, top_idx: torch.Tensor,
+                 top_lse: torch.Tensor | None = None, scale: float = 1.0,
+                 temperature: float = 1.0, reduction: str = "mean"):
+    """KL from a teacher's listed logits (top_val, top_idx int32 [T, k],
+    top_lse fp32 [T] or None) to softmax(scale / temperature * h W^T).
+    Returns (loss fp32 [T] or scalar, state for head_distill_grad)."""
+    hp, Wp = _head_pair("head_distill", h, W)
+    _one_gpu("head_distill", h, top_val, top_idx, top_lse)
+    T = h.shape[0]
+    if top_val.dtype not in _lib.DTYPES or top_idx.dtype != torch.int32:
+        raise _lib.CrbqError("head_distill takes floating teacher logits and int32 tokens")
+    if top_val.dim() != 2 or top_val.shape != top_idx.shape or top_val.shape[0] != T or not (
+            1 <= top_val.shape[1] <= _lib.HEAD_MAX_K):
+        raise _lib.CrbqError(f"head_distill takes teacher logits and tokens [T, k], k up to "
+                             f"{_lib.HEAD_MAX_K}, not {tuple(top_val.shape)} and "
+                             f"{tuple(top_idx.shape)}")
+    if top_lse is not None and (top_lse.dtype != torch.float32 or top_lse.shape != (T,)):
+        raise _lib.CrbqError("head_distill takes an fp32 teacher log-sum-exp [T]")
+    if not temperature > 0:
+        raise _lib.CrbqError("head_distill takes a temperature above 0")
+    k = top_val.shape[1]
+    val = top_val if top_val.stride(1) == 1 and top_val.stride(0) >= k else top_val.contiguous()
+    idx = top_idx if top_idx.stride(1) == 1 and top_idx.stride(0) >= k else top_idx.contiguous()
+    tlse = top_lse.contiguous() if top_lse is not None else None
+    red = _reduction("head_distill", reduction)
+    lib = _lib.ready(h.device)
+    with _lib.on_device(h.device):
+        loss, state, ws, nws = _head_buffers(lib, hp, Wp, k, red, h.device)
+        check(lib.crbq_head_distill(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
+                                    _lib.DTYPES[h.dtype], T, Wp.shape[0], hp.shape[1],
+                                    val.data_ptr(), _lib.DTYPES[val.dtype], max(val.stride(0), k),
+                                    idx.data_ptr(), max(idx.stride(0), k), k, ptr(tlse),
+                                    float(scale), float(temperature), red, loss.data_ptr(),
+                                    state.data_ptr(), ws.data_ptr(), nws, stream_of(h)),
+              "crbq_head_distill")
+    return loss, state
+
+
+def head_distill_grad(h: torch.Tensor, W: torch.Tensor, k: int, state: torch.Tensor,
+                      g: torch.Tensor, scale: float = 1.0, temperature: float = 1.0,
+                      need_h: bool = True, need_w: bool = True):
+    """(dh, dW) (None where not asked for) of head_distill's loss times g."""
+    hp, Wp = _head_pair("head_distill_grad", h, W)
+    lib = _lib.ready(h.device)
+    with _lib.on_device(h.device):
+        dh, dW, ws, nws, g = _grad_args("head_distill_grad", hp, Wp, state, g, need_h, need_w,
+                                        lib)
+        check(lib.crbq_head_distill_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
+                                         _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0],
+                                         hp.shape[1], int(k), float(scale), float(temperature),
+                                         state.data_ptr(), g.data_ptr(), int(g.dim() == 1),
+                                         *_out_args(dh, dW), ws.data_ptr(), nws, stream_of(h)),
+              "crbq_head_distill_grad")
+    return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
+    """The k largest of each row of logits [T, V], descending, ties to the
+    lowest index: (val [T, k], idx int32 [T, k], lse fp32 [T] of the row
+    divided by temperature)."""
+    _one_gpu("top_logits", logits)
+    if logits.dtype not in _lib.DTYPES:
+        raise _lib.CrbqError(f"top_logits takes fp32, fp16 or bf16 logits, not {logits.dtype}")
+    if logits.dim() != 2 or 0 in logits.shape:
+        raise _lib.CrbqError(f"top_logits takes logits [T, V], not {tuple(logits.shape)}")
+    T, V = logits.shape
+    k = int(k)
+    if not 1 <= k <= min(V, _lib.HEAD_MAX_K):
+        raise _lib.CrbqError(f"top_logits: k = {k} is not within 1..{min(V, _lib.HEAD_MAX_K)}")
+    if not temperature > 0:
+        raise _lib.CrbqError("top_logits takes a temperature above 0")
+    x = logits if logits.stride(1) == 1 and (T == 1 or logits.stride(0) >= V) else logits.contiguous()
+    lib = _lib.ready(x.device)
+    with _lib.on_device(x.device):
+        val = torch.empty((T, k), dtype=x.dtype, device=x.device)
+        idx = torch.empty((T, k), dtype=torch.int32, device=x.device)
+        lse = torch.empty(T, dtype=torch.float32, device=x.device)
+        check(lib.crbq_top_logits(x.data_ptr(), _lib.DTYPES[x.dtype], T, V, max(x.stride(0), V), k,
+                                  float(temperature), val.data_ptr(), idx.data_ptr(),
+                                  lse.data_ptr(), stream_of(x)), "crbq_top_logits")
+    return val, idx, lse

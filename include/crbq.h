@@ -353,6 +353,66 @@ int crbq_linear_packed(const uint8_t* codes, int64_t ldc, const void* lut, const
                        const void* bias, void* y, int64_t ldy, void* ws, size_t ws_bytes,
                        void* stream);
 
+/* ---- losses of the output head over a large vocabulary --------------------
+ * No counterpart in the reference, whose perplexity forms all logits and
+ * calls a cross entropy (eval_ppl_utils.py:626-636).  Hidden states h [T][C]
+ * and the head's weight W [V][C], both fp16 or both bf16 (16-byte aligned,
+ * row strides multiples of 8 below 2^22, C a multiple of 8); logits
+ * z = scale * h W^T are computed piece by piece in fp32 and never kept.
+ *
+ * crbq_head_xent: loss_t = log sum_v exp z[t][v] - z[t][labels[t]].
+ *   labels[t] == ignore_index: the row is left out (loss 0, no gradient,
+ *   not counted); a label outside [0, V) otherwise: NaN.
+ * crbq_head_distill: z is divided by temperature too; each row lists k
+ *   tokens of a teacher (top_idx [T][ldi]; outside [0, V): an empty slot;
+ *   a token listed twice: both entries count, each with its probability)
+ *   with its logits top_val [T][ldv] (val_dtype).  top_lse NULL: p = softmax of the
+ *   listed logits / temperature, loss_t = sum p (log p - log q), q the
+ *   student's softmax over all V.  top_lse[t] = the teacher's log sum exp
+ *   over its vocabulary of logits / temperature: p = exp(logit /
+ *   temperature - top_lse), and the tokens not listed are one more outcome,
+ *   with probability max(0, 1 - sum p) and the student's 1 - sum q.  No
+ *   factor temperature^2.  A row with no token listed is left out.
+ * reduction: CRBQ_NONE: loss [T]; CRBQ_SUM, CRBQ_MEAN: loss [1], the sum
+ *   over rows or the mean over the rows not left out (over none: NaN).
+ * state: crbq_head_state_floats(T, k) floats (k = 0: cross entropy), what
+ *   the gradients need of the forward; the caller keeps it.
+ * *_grad: gradients of the same call's loss times g (g_per_row 0: *g one
+ *   number; 1: g[t] per row, for CRBQ_NONE) to h (dh [T][ldd]) and W
+ *   (dW [V][ldo]) in the inputs' dtype; either may be NULL.  The logits are
+ *   computed again; sums are fp32, in a fixed order.  A left-out row of h
+ *   is not read into dW.
+ * crbq_head_workspace_size(T, V, C, k, grad): bytes of ws for either. */
+enum crbq_reduction { CRBQ_NONE = 0, CRBQ_MEAN = 1, CRBQ_SUM = 2 };
+#define CRBQ_HEAD_MAX_K 256
+size_t crbq_head_state_floats(int64_t T, int64_t k);
+size_t crbq_head_workspace_size(int64_t T, int64_t V, int64_t C, int64_t k, int grad);
+int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype, int64_t T,
+                   int64_t V, int64_t C, const int64_t* labels, int64_t ignore_index,
+                   float scale, int reduction, float* loss, float* state, void* ws,
+                   size_t ws_bytes, void* stream);
+int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
+                        int64_t T, int64_t V, int64_t C, const int64_t* labels,
+                        int64_t ignore_index, float scale, const float* state, const float* g,
+                        int g_per_row, void* dh, int64_t ldd, void* dW, int64_t ldo, void* ws,
+                        size_t ws_bytes, void* stream);
+int crbq_head_distill(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
+                      int64_t T, int64_t V, int64_t C, const void* top_val, int val_dtype,
+                      int64_t ldv, const int32_t* top_idx, int64_t ldi, int k,
+                      const float* top_lse, float scale, float temperature, int reduction,
+                      float* loss, float* state, void* ws, size_t ws_bytes, void* stream);
+int crbq_head_distill_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
+                           int64_t T, int64_t V, int64_t C, int k, float scale,
+                           float temperature, const float* state, const float* g, int g_per_row,
+                           void* dh, int64_t ldd, void* dW, int64_t ldo, void* ws,
+                           size_t ws_bytes, void* stream);
+/* The k largest of each row of logits [T][V] (row stride ld, any dtype),
+ * descending, ties to the lowest index, NaN above everything: val [T][k]
+ * (the logits' dtype), idx [T][k], and lse[t] = log sum exp of the row
+ * divided by temperature.  k <= min(V, CRBQ_HEAD_MAX_K). */
+int crbq_top_logits(const void* logits, int dtype, int64_t T, int64_t V, int64_t ld, int k,
+                    float temperature, void* val, int32_t* idx, float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
