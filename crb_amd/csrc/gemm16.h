@@ -212,50 +212,100 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
       g_load_lds(buf + SA::BYTES + g * 1024, s.rb, v);
     }
   };
+  // fragments of half h of the stage in `cur`
+  auto fragA = [&](const char* cur, int h, int i) -> T8 {
+    if constexpr (G::AKC) return *(const T8*)(cur + fa[i] + (((gq + 4 * h) ^ (r16 & 7)) << 4));
+    else return g_tr_frag<T8, G::BM * 2>(cur + fa[i] + h * 32 * G::BM * 2);
+  };
+  auto fragB = [&](const char* cur, int h, int j) -> T8 {
+    if constexpr (G::BKC) return *(const T8*)(cur + fb[j] + (((gq + 4 * h) ^ (r16 & 7)) << 4));
+    else return g_tr_frag<T8, G::BN * 2>(cur + fb[j] + h * 32 * G::BN * 2);
+  };
+  if constexpr (G::NS == 2) {
+    // Two stages in LDS.  While the MFMAs of one half stage run, the
+    // fragments of the next half are read into the other register set.
+    // One barrier a stage, between its halves: there every
+    // wavefront has read all of stage c (so stage c + 2 may be loaded over
+    // it) and its loads of stage c + 1, issued a whole stage before, have
+    // arrived (so its fragments may be read): no MFMA waits for an LDS read
+    // that could only start behind the barrier.
+    T8 a0[G::MI], b0[G::NJ], a1[G::MI], b1[G::NJ];
 #pragma unroll
-  for (int c = 0; c < G::NS - 1; ++c) {
-    const Src s = source(c);
+    for (int c = 0; c < 2; ++c) {
+      const Src s = source(c);
 #pragma unroll
-    for (int q = 0; q < G::LW; ++q) load(c, q, s);
-  }
-  g_wait_vm<(G::NS - 2) * G::LW>();
-  g_sync_lds();
-  for (int c = 0; c < nch; ++c) {
-    const Src s = source(c + G::NS - 1);
-    const char* cur = smem + (c % G::NS) * G::STAGE;
+      for (int q = 0; q < G::LW; ++q) load(c, q, s);
+    }
+    g_wait_vm<G::LW>();
+    g_sync_lds();
 #pragma unroll
-    for (int h = 0; h < G_K / 32; ++h) {
-      // KC: the lane's chunk (gq + 4 h) of rows that share r16's low 3 bits
-      const int kc = ((gq + 4 * h) ^ (r16 & 7)) << 4;
-      auto fragA = [&](int i) -> T8 {
-        if constexpr (G::AKC) return *(const T8*)(cur + fa[i] + kc);
-        else return g_tr_frag<T8, G::BM * 2>(cur + fa[i] + h * 32 * G::BM * 2);
-      };
-      auto fragB = [&](int j) -> T8 {
-        if constexpr (G::BKC) return *(const T8*)(cur + fb[j] + kc);
-        else return g_tr_frag<T8, G::BN * 2>(cur + fb[j] + h * 32 * G::BN * 2);
-      };
-      T8 bb[G::NJ];
+    for (int j = 0; j < G::NJ; ++j) b0[j] = fragB(smem, 0, j);
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j) bb[j] = fragB(j);
-      T8 an = fragA(0);
+    for (int i = 0; i < G::MI; ++i) a0[i] = fragA(smem, 0, i);
+    for (int c = 0; c < nch; ++c) {
+      const char* cur = smem + (c & 1) * G::STAGE;
+      const char* nxt = smem + ((c + 1) & 1) * G::STAGE;
+      const Src s = source(c + 2);
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b1[j] = fragB(cur, 1, j);
 #pragma unroll
       for (int i = 0; i < G::MI; ++i) {
-        const T8 a = an;
-        if (i + 1 < G::MI) an = fragA(i + 1);
+        a1[i] = fragA(cur, 1, i);
 #pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a, bb[j], acc[i][j]);
-        if (h == 0) {
-          // the stage's loads between the MFMAs of its first half
-#pragma unroll
-          for (int q = 0; q < G::LW; ++q)
-            if (q * G::MI / G::LW == i) load(c + G::NS - 1, q, s);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a0[i], b0[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      g_wait_vm<0>();
+      g_sync_lds();
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b0[j] = fragB(nxt, 0, j);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) {
+        a0[i] = fragA(nxt, 0, i);
+#pragma unroll
+        for (int q = 0; q < G::LW; ++q)
+          if (q * G::MI / G::LW == i) load(c + 2, q, s);
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a1[i], b1[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < G::NS - 1; ++c) {
+      const Src s = source(c);
+#pragma unroll
+      for (int q = 0; q < G::LW; ++q) load(c, q, s);
     }
     g_wait_vm<(G::NS - 2) * G::LW>();
     g_sync_lds();
+    for (int c = 0; c < nch; ++c) {
+      const Src s = source(c + G::NS - 1);
+      const char* cur = smem + (c % G::NS) * G::STAGE;
+#pragma unroll
+      for (int h = 0; h < G_K / 32; ++h) {
+        T8 bb[G::NJ];
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) bb[j] = fragB(cur, h, j);
+        T8 an = fragA(cur, h, 0);
+#pragma unroll
+        for (int i = 0; i < G::MI; ++i) {
+          const T8 a = an;
+          if (i + 1 < G::MI) an = fragA(cur, h, i + 1);
+#pragma unroll
+          for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a, bb[j], acc[i][j]);
+          if (h == 0) {
+            // the stage's loads between the MFMAs of its first half
+#pragma unroll
+            for (int q = 0; q < G::LW; ++q)
+              if (q * G::MI / G::LW == i) load(c + G::NS - 1, q, s);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      g_wait_vm<(G::NS - 2) * G::LW>();
+      g_sync_lds();
+    }
   }
   g_wait_vm<0>();
   g_sync_lds();
