@@ -20,6 +20,8 @@
 // so a lane holds 4 consecutive m of one n: the kernels take the output's
 // contiguous (or reduced) dimension as m.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace crbq {
@@ -139,178 +141,6 @@ struct GTile {
   static_assert(LDS <= 160 * 1024 && MI >= 1 && NJ >= 1 && (NS - 2) * LW <= 63, "tile shape");
 };
 
-// acc = the tile's sums over k in [k_beg, k_end): both multiples of 64, or k_end
-// the operands' end (where theirs differ, the shorter one's; what the longer
-// one holds behind it meets zeros and has to be finite).  On return every
-// wavefront has left the stages.
-template <typename T8, typename G>
-__device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOperand& B,
-                                       int64_t k_beg, int64_t k_end,
-                                       f4_t (&acc)[G::MI][G::NJ]) {
-  using SA = typename G::SA;
-  using SB = typename G::SB;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (wave / G::WGN) * G::WM, wn = (wave % G::WGN) * G::WN;
-  const int nch = k_end > k_beg ? (int)((k_end - k_beg + G_K - 1) / G_K) : 0;
-  constexpr unsigned OUT = 0x80000000u;
-  unsigned va[SA::PER_WAVE], vb[SB::PER_WAVE];
-#pragma unroll
-  for (int q = 0; q < SA::PER_WAVE; ++q) va[q] = SA::voff(SA::group(wave, q), lane, A.ld);
-#pragma unroll
-  for (int q = 0; q < SB::PER_WAVE; ++q) vb[q] = SB::voff(SB::group(wave, q), lane, B.ld);
-  const int kc8 = ((lane & 7) ^ ((lane >> 3) & 7)) * 8;          // a KC lane's first k
-  // fragment addresses within a stage (bytes)
-  const int r16 = lane & 15, gq = lane >> 4;
-  const int trow = 8 * gq + (r16 >> 2), fsw = g_swz(trow);
-  int fa[G::MI], fb[G::NJ];
-#pragma unroll
-  for (int i = 0; i < G::MI; ++i) {
-    const int ch = wm + 16 * i + 4 * (r16 & 3);
-    fa[i] = G::AKC ? (wm + 16 * i + r16) * (G_K * 2)
-                   : trow * G::BM * 2 + (((ch >> 3) ^ fsw) << 4) + (ch & 7) * 2;
-  }
-#pragma unroll
-  for (int j = 0; j < G::NJ; ++j) {
-    const int ch = wn + 16 * j + 4 * (r16 & 3);
-    fb[j] = SA::BYTES + (G::BKC ? (wn + 16 * j + r16) * (G_K * 2)
-                                : trow * G::BN * 2 + (((ch >> 3) ^ fsw) << 4) + (ch & 7) * 2);
-  }
-#pragma unroll
-  for (int i = 0; i < G::MI; ++i)
-#pragma unroll
-    for (int j = 0; j < G::NJ; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
-
-  // load q of a stage's LW loads of this wavefront
-  struct Src {
-    i4_t ra, rb;
-    bool kin;              // KC lanes: this lane's chunk lies before K
-    uint64_t live;
-  };
-  auto source = [&](int c) {
-    const int64_t k0 = k_beg + (int64_t)c * G_K;
-    Src s;
-    s.ra = SA::rsrc(A, k0, c < nch ? A.K : 0);                  // past the end: all zeros
-    s.rb = SB::rsrc(B, k0, c < nch ? B.K : 0);
-    s.kin = k0 + kc8 < (G::BKC ? B.K : A.K);
-    s.live = ~0ull;
-    if (!G::AKC && A.live) s.live = c < nch ? A.live[k0 / G_K] : 0;
-    return s;
-  };
-  auto load = [&](int c, int q, const Src& s) {
-    char* buf = smem + (c % G::NS) * G::STAGE;
-    if (q < SA::PER_WAVE) {
-      const int g = SA::group(wave, q);
-      unsigned v = va[q < SA::PER_WAVE ? q : 0];
-      if (G::AKC) v = s.kin ? v : OUT;
-      else v = ((s.live >> SA::row(g, lane)) & 1) ? v : OUT;
-      g_load_lds(buf + g * 1024, s.ra, v);
-    } else {
-      const int qb = q - SA::PER_WAVE, g = SB::group(wave, qb);
-      unsigned v = vb[qb >= 0 && qb < SB::PER_WAVE ? qb : 0];
-      if (G::BKC) v = s.kin ? v : OUT;
-      g_load_lds(buf + SA::BYTES + g * 1024, s.rb, v);
-    }
-  };
-  // fragments of half h of the stage in `cur`
-  auto fragA = [&](const char* cur, int h, int i) -> T8 {
-    if constexpr (G::AKC) return *(const T8*)(cur + fa[i] + (((gq + 4 * h) ^ (r16 & 7)) << 4));
-    else return g_tr_frag<T8, G::BM * 2>(cur + fa[i] + h * 32 * G::BM * 2);
-  };
-  auto fragB = [&](const char* cur, int h, int j) -> T8 {
-    if constexpr (G::BKC) return *(const T8*)(cur + fb[j] + (((gq + 4 * h) ^ (r16 & 7)) << 4));
-    else return g_tr_frag<T8, G::BN * 2>(cur + fb[j] + h * 32 * G::BN * 2);
-  };
-  if constexpr (G::NS == 2) {
-    // Two stages in LDS.  While the MFMAs of one half stage run, the
-    // fragments of the next half are read into the other register set.
-    // One barrier a stage, between its halves: there every
-    // wavefront has read all of stage c (so stage c + 2 may be loaded over
-    // it) and its loads of stage c + 1, issued a whole stage before, have
-    // arrived (so its fragments may be read): no MFMA waits for an LDS read
-    // that could only start behind the barrier.
-    T8 a0[G::MI], b0[G::NJ], a1[G::MI], b1[G::NJ];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const Src s = source(c);
-#pragma unroll
-      for (int q = 0; q < G::LW; ++q) load(c, q, s);
-    }
-    g_wait_vm<G::LW>();
-    g_sync_lds();
-#pragma unroll
-    for (int j = 0; j < G::NJ; ++j) b0[j] = fragB(smem, 0, j);
-#pragma unroll
-    for (int i = 0; i < G::MI; ++i) a0[i] = fragA(smem, 0, i);
-    for (int c = 0; c < nch; ++c) {
-      const char* cur = smem + (c & 1) * G::STAGE;
-      const char* nxt = smem + ((c + 1) & 1) * G::STAGE;
-      const Src s = source(c + 2);
-#pragma unroll
-      for (int j = 0; j < G::NJ; ++j) b1[j] = fragB(cur, 1, j);
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i) {
-        a1[i] = fragA(cur, 1, i);
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a0[i], b0[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      g_wait_vm<0>();
-      g_sync_lds();
-#pragma unroll
-      for (int j = 0; j < G::NJ; ++j) b0[j] = fragB(nxt, 0, j);
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i) {
-        a0[i] = fragA(nxt, 0, i);
-#pragma unroll
-        for (int q = 0; q < G::LW; ++q)
-          if (q * G::MI / G::LW == i) load(c + 2, q, s);
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a1[i], b1[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < G::NS - 1; ++c) {
-      const Src s = source(c);
-#pragma unroll
-      for (int q = 0; q < G::LW; ++q) load(c, q, s);
-    }
-    g_wait_vm<(G::NS - 2) * G::LW>();
-    g_sync_lds();
-    for (int c = 0; c < nch; ++c) {
-      const Src s = source(c + G::NS - 1);
-      const char* cur = smem + (c % G::NS) * G::STAGE;
-#pragma unroll
-      for (int h = 0; h < G_K / 32; ++h) {
-        T8 bb[G::NJ];
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) bb[j] = fragB(cur, h, j);
-        T8 an = fragA(cur, h, 0);
-#pragma unroll
-        for (int i = 0; i < G::MI; ++i) {
-          const T8 a = an;
-          if (i + 1 < G::MI) an = fragA(cur, h, i + 1);
-#pragma unroll
-          for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a, bb[j], acc[i][j]);
-          if (h == 0) {
-            // the stage's loads between the MFMAs of its first half
-#pragma unroll
-            for (int q = 0; q < G::LW; ++q)
-              if (q * G::MI / G::LW == i) load(c + G::NS - 1, q, s);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-      }
-      g_wait_vm<(G::NS - 2) * G::LW>();
-      g_sync_lds();
-    }
-  }
-  g_wait_vm<0>();
-  g_sync_lds();
-}
-
 // Workgroup id -> linear index such that the workgroups one XCD receives
 // (every 8th id) take consecutive indices.
 __device__ __forceinline__ int g_xcd(int id, int nwg) {
@@ -324,6 +154,290 @@ __device__ __forceinline__ void g_band(int lin, int nm, int nn, int& tm, int& tn
   const int w = nn - n0 < 8 ? nn - n0 : 8, in = lin - band * per;
   tm = in / w;
   tn = n0 + in % w;
+}
+
+// What a lane needs to load stages and to read fragments of them.
+template <typename T8, typename G>
+struct GLane {
+  using SA = typename G::SA;
+  using SB = typename G::SB;
+  static constexpr unsigned OUT = 0x80000000u;         // beyond any range
+  unsigned va[SA::PER_WAVE], vb[SB::PER_WAVE];         // offsets of its loads
+  int lane, wave, kc8, fa, fb, kx;
+
+  __device__ GLane(int64_t lda, int64_t ldb) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int q = 0; q < SA::PER_WAVE; ++q) va[q] = SA::voff(SA::group(wave, q), lane, lda);
+#pragma unroll
+    for (int q = 0; q < SB::PER_WAVE; ++q) vb[q] = SB::voff(SB::group(wave, q), lane, ldb);
+    kc8 = ((lane & 7) ^ ((lane >> 3) & 7)) * 8;        // a KC lane's first k of a stage
+    const int wm = (wave / G::WGN) * G::WM, wn = (wave % G::WGN) * G::WN;
+    fa = base<G::AKC, G::BM>(wm);
+    fb = base<G::BKC, G::BN>(wn);
+    kx = (lane >> 4) ^ (lane & 7);
+  }
+  // First fragment's address in a stage of R rows, at row w of it.  KC: rows
+  // are 128 bytes, the chunk comes with the half stage; K-strided: lane (group gq, s)
+  // addresses k row 8 gq + s / 4 at row w + 4 (s % 4).
+  template <bool KC, int R>
+  __device__ int base(int w) const {
+    const int r16 = lane & 15, trow = 8 * (lane >> 4) + (r16 >> 2), ch = w + 4 * (r16 & 3);
+    return KC ? (w + r16) * (G_K * 2)
+              : trow * R * 2 + (((ch >> 3) ^ g_swz(trow)) << 4) + (ch & 7) * 2;
+  }
+  // Fragment i (16 rows on) of half h of the operand whose stage starts at
+  // LDS address `at` (a multiple of 1024).  K-strided: 16 rows are two chunks,
+  // address bits 5 to 7, which the permutation exclusive-ors.
+  template <bool KC, int R>
+  __device__ T8 frag(const char* smem, int at, int f, int h, int i) const {
+    if constexpr (KC)
+      return *(const T8*)(smem + (at + f + ((kx ^ (4 * h)) << 4)) + i * 16 * G_K * 2);
+    else
+      return g_tr_frag<T8, R * 2>(smem + ((at + f) ^ (i << 5)) + h * 32 * R * 2);
+  }
+  __device__ T8 fragA(const char* smem, int at, int h, int i) const {
+    return frag<G::AKC, G::BM>(smem, at, fa, h, i);
+  }
+  __device__ T8 fragB(const char* smem, int at, int h, int j) const {
+    return frag<G::BKC, G::BN>(smem, at + SA::BYTES, fb, h, j);
+  }
+  // a stage's descriptors and masks
+  struct Src {
+    i4_t ra, rb;
+    bool kin;              // KC lanes: this lane's chunk lies before K
+    uint64_t live;
+  };
+  __device__ Src source(const GOperand& A, const GOperand& B, int64_t k0, bool any) const {
+    Src s;
+    s.ra = SA::rsrc(A, k0, any ? A.K : 0);
+    s.rb = SB::rsrc(B, k0, any ? B.K : 0);
+    s.kin = k0 + kc8 < (G::BKC ? B.K : A.K);
+    s.live = ~0ull;
+    if (!G::AKC && A.live) s.live = any ? A.live[k0 / G_K] : 0;
+    return s;
+  }
+  // load q (of G::LW) of a stage into the LDS at buf
+  __device__ void load(char* buf, int q, const Src& s) const {
+    if (q < SA::PER_WAVE) {
+      const int g = SA::group(wave, q);
+      unsigned v = va[q < SA::PER_WAVE ? q : 0];
+      if (G::AKC) v = s.kin ? v : OUT;
+      else v = ((s.live >> SA::row(g, lane)) & 1) ? v : OUT;
+      g_load_lds(buf + g * 1024, s.ra, v);
+    } else {
+      const int qb = q - SA::PER_WAVE, g = SB::group(wave, qb);
+      unsigned v = vb[qb >= 0 && qb < SB::PER_WAVE ? qb : 0];
+      if (G::BKC) v = s.kin ? v : OUT;
+      g_load_lds(buf + SA::BYTES + g * 1024, s.rb, v);
+    }
+  }
+};
+
+// f(integral constant 0), ..., f(N - 1): accumulators are indexed by constants only
+template <int N, typename F>
+__device__ __forceinline__ void g_each(const F& f) {
+  if constexpr (N > 0) {
+    g_each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
+// The lane, for an epilogue: opaque, so that what an epilogue computes from it
+// is computed there and not kept in registers over the products.
+__device__ __forceinline__ int g_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+template <typename G>
+__device__ __forceinline__ void g_zero(f4_t (&acc)[G::MI][G::NJ]) {
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+}
+
+// One tile, NS - 1 stages of loads in flight (few rows of B: the loads of A
+// are all that counts).  acc = its sums over k in [k_beg, k_end): both multiples
+// of 64, or k_end the operands' end (where theirs differ, the shorter
+// one's; what the longer one holds behind it meets zeros and has to be
+// finite).  On return every wavefront has left the stages.
+template <typename T8, typename G>
+__device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOperand& B,
+                                       int64_t k_beg, int64_t k_end,
+                                       f4_t (&acc)[G::MI][G::NJ]) {
+  const GLane<T8, G> L(A.ld, B.ld);
+  const int nch = k_end > k_beg ? (int)((k_end - k_beg + G_K - 1) / G_K) : 0;
+  g_zero<G>(acc);
+#pragma unroll
+  for (int c = 0; c < G::NS - 1; ++c) {
+    const auto s = L.source(A, B, k_beg + (int64_t)c * G_K, c < nch);
+#pragma unroll
+    for (int q = 0; q < G::LW; ++q) L.load(smem + c * G::STAGE, q, s);
+  }
+  g_wait_vm<(G::NS - 2) * G::LW>();
+  g_sync_lds();
+  for (int c = 0; c < nch; ++c) {
+    const int n = c + G::NS - 1;
+    const auto s = L.source(A, B, k_beg + (int64_t)n * G_K, n < nch);
+    char* nbuf = smem + (n % G::NS) * G::STAGE;
+    const int at = (c % G::NS) * G::STAGE;
+#pragma unroll
+    for (int h = 0; h < G_K / 32; ++h) {
+      T8 bb[G::NJ];
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) bb[j] = L.fragB(smem, at, h, j);
+      T8 an = L.fragA(smem, at, h, 0);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) {
+        const T8 a = an;
+        if (i + 1 < G::MI) an = L.fragA(smem, at, h, i + 1);
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a, bb[j], acc[i][j]);
+        if (h == 0) {
+          // the stage's loads between the MFMAs of its first half
+#pragma unroll
+          for (int q = 0; q < G::LW; ++q)
+            if (q * G::MI / G::LW == i) L.load(nbuf, q, s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    g_wait_vm<(G::NS - 2) * G::LW>();
+    g_sync_lds();
+  }
+  g_wait_vm<0>();
+  g_sync_lds();
+}
+
+// A workgroup's share of a launch's tiles, one after the other without a
+// gap: tiles lin, lin + gridDim, ... of job.tiles.
+//   job.tile(lin, A, B, k_beg, nch)  a tile's operands, first k and stages (>= 1)
+//   job.side(lin, priv)              loads what the tile's epilogue needs into the
+//                                    wavefront's own 4 KB of LDS (g_load_lds*)
+//   job.finish(lin, priv, acc)       the epilogue
+// Two stages in LDS.  While the MFMAs of one half stage run, the fragments of
+// the next half are read into the other register set.  One barrier a stage,
+// between its halves: there every wavefront has read all of the stage (so the
+// stage after the next may be loaded over it), and the loads of the next
+// stage, issued a whole stage before, have arrived (so its fragments may be
+// read): no MFMA waits for an LDS read that could only start behind a
+// barrier.  The next tile's first stages are loaded under this tile's last, so
+// its loads run under the epilogue too.
+constexpr int G_PRIV = 4096;
+template <typename T8, typename G, typename Job>
+__device__ __forceinline__ void g_run(char* smem, const Job& job) {
+  static_assert(G::NS == 2, "two stages");
+  const GLane<T8, G> L(job.lda, job.ldb);
+  char* priv = smem + G::LDS + L.wave * G_PRIV;
+  const int nwg = gridDim.x, first = g_xcd(blockIdx.x, nwg);
+  // the stage to be loaded next: c of tile ll
+  int ll = first, lc = 0, ln = 0;
+  int64_t lk = 0;
+  GOperand A, B;
+  auto open = [&]() {
+    if (ll < job.tiles) job.tile(ll, A, B, lk, ln);
+  };
+  auto source = [&]() {
+    const auto s = L.source(A, B, lk + (int64_t)lc * G_K, ll < job.tiles);
+    if (++lc == ln) {
+      lc = 0;
+      ll += nwg;
+      open();
+    }
+    return s;
+  };
+  open();
+  if (ll >= job.tiles) return;                         // no tile at all
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const auto s = source();
+#pragma unroll
+    for (int q = 0; q < G::LW; ++q) L.load(smem + c * G::STAGE, q, s);
+  }
+  g_wait_vm<G::LW>();
+  g_sync_lds();
+  int par = 0;                                         // the stage's buffer
+  for (int lin = first; lin < job.tiles; lin += nwg) {
+    // read again behind an epilogue, which needs the registers
+    T8 a0[G::MI], b0[G::NJ], a1[G::MI], b1[G::NJ];
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) b0[j] = L.fragB(smem, par * G::STAGE, 0, j);
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i) a0[i] = L.fragA(smem, par * G::STAGE, 0, i);
+    f4_t acc[G::MI][G::NJ];
+    g_zero<G>(acc);
+    int nch;
+    {
+      GOperand ta, tb;
+      int64_t tk;
+      job.tile(lin, ta, tb, tk, nch);
+    }
+    job.side(lin, priv);
+    for (int c = 0; c < nch; ++c) {
+      const int at = par * G::STAGE, nx = G::STAGE - at;
+      const auto s = source();
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b1[j] = L.fragB(smem, at, 1, j);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) {
+        a1[i] = L.fragA(smem, at, 1, i);
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a0[i], b0[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      g_wait_vm<0>();
+      g_sync_lds();
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) b0[j] = L.fragB(smem, nx, 0, j);
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i) {
+        a0[i] = L.fragA(smem, nx, 0, i);
+#pragma unroll
+        for (int q = 0; q < G::LW; ++q)
+          if (q * G::MI / G::LW == i) L.load(smem + at, q, s);
+#pragma unroll
+        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a1[i], b1[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      par ^= 1;
+    }
+    job.finish(lin, priv, acc);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // priv is free for the next side()
+  }
+  g_wait_vm<0>();
+}
+
+// 64 words (lane l: word l of p) and 64 rows of 16 bytes (lane l: p + l * ld) into
+// the wavefront's own LDS; what lies behind nbytes reads as zeros.
+__device__ __forceinline__ void g_load_lds_words(const void* dst, const void* p, int64_t nbytes,
+                                                 int lane) {
+  const unsigned d = __builtin_amdgcn_readfirstlane(
+      (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)dst);
+  const i4_t rs = g_rsrc((const uint16_t*)p, nbytes > 0 ? (nbytes < 256 ? nbytes : 256) : 0);
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(rs), "{m0}"(d));
+}
+
+// 16 rows (n) of a tile's 16-bit output, MI * 16 elements each, through the wavefront's
+// own LDS: in as each lane's 4 consecutive elements of one row, out as
+// 16-byte stores of whole rows.  put(row, m, 8 elements) stores.
+template <typename G, typename F>
+__device__ __forceinline__ void g_rows_out(char* priv, const uint2 (&v)[G::MI], F&& put) {
+  static_assert(G::MI == 8, "rows of 256 bytes");
+  const int lane = g_lane(), n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+    *(uint2*)(priv + n * 256 + (((2 * i + (g >> 1)) ^ n) << 4) + (g & 1) * 8) = v[i];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = 4 * q + g;
+    put(r, n * 8, *(const uint4*)(priv + r * 256 + ((n ^ r) << 4)));
+  }
+  asm volatile("" ::: "memory");
 }
 
 }  // namespace crbq

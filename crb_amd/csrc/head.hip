@@ -60,11 +60,11 @@ __device__ __forceinline__ float gsum4(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// (m, s): maximum and sum of exp(x - m); joins two such pairs
+// (m, s): maximum and sum of 2^(x - m); joins two such pairs
 __device__ __forceinline__ void ms_join(float& m, float& s, float m2, float s2) {
   const float mm = fmaxf(m, m2);
-  const float x = m == mm ? s : s * g_exp(m - mm);        // m = -inf = mm: s is 0
-  const float y = m2 == mm ? s2 : s2 * g_exp(m2 - mm);
+  const float x = m == mm ? s : s * __builtin_amdgcn_exp2f(m - mm);   // m = -inf = mm: s is 0
+  const float y = m2 == mm ? s2 : s2 * __builtin_amdgcn_exp2f(m2 - mm);
   m = mm;
   s = x + y;
 }
@@ -87,76 +87,208 @@ struct Listed {
 // forward product: partial (max, sum) of every (row, tile row of wavefronts)
 // and the listed tokens' z
 // ---------------------------------------------------------------------------
+struct FwdArgs {
+  const uint16_t *h, *W;
+  int64_t ldh, ldw, T, V, C;
+  float scale;
+  Listed ls;
+  int nm, nn;
+  float2* part;
+  int64_t npart;
+  float* zt;
+};
+
+// The slot of token v in row t's ascending list.
+__device__ __forceinline__ int64_t list_slot(const Listed& ls, int64_t t, int v) {
+  const int32_t* s = ls.sidx + t * ls.k;
+  int lo = 0, hi = ls.k - 1;
+  while (lo < hi) {
+    const int md = (lo + hi) >> 1;
+    if (s[md] < v) lo = md + 1;
+    else hi = md;
+  }
+  return t * ls.k + lo;
+}
+
+// Column t (n) of a wavefront's tile: listed tokens and what lies behind
+// the vocabulary become -inf (the listed ones' z is written), then the
+// maximum and the sum of exponentials over its MI * 16 tokens from vw on.
+// In units of log 2: exp z = 2^(acc * scale2), so an exponential is one
+// multiply-add and one v_exp; the listed tokens and the end are looked for
+// only where a wavefront has any.  Bound by the v_exp (16 cycles a wavefront)
+// and the 2 to 3 vector operations beside each.
+template <typename G, bool XENT, int j>
+__device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t vw, int lab,
+                                           const uint32_t (&words)[G::WM / 32],
+                                           f4_t (&acc)[G::MI][G::NJ], float2* out) {
+  const int lane = g_lane(), g4 = (lane >> 4) * 4;
+  const bool ok = t < p.T;
+  bool any;
+  if (XENT) {
+    any = lab >= 0;
+  } else {
+    uint32_t w = 0;
+#pragma unroll
+    for (int q = 0; q < G::WM / 32; ++q) w |= words[q];
+    any = w != 0;
+  }
+  const float fin = p.scale < 0.f ? INFINITY : -INFINITY;        // scale * fin = -inf
+  if (__any(any)) {
+    g_each<G::MI>([&](auto ii) __attribute__((always_inline)) {
+      constexpr int i = decltype(ii)::value;
+      const uint32_t nib = XENT ? (uint32_t)(lab >> 2 == 4 * i + (lane >> 4))
+                                : (words[i / 2] >> (16 * (i & 1) + g4)) & 15u;
+      if (nib)
+        g_each<4>([&](auto rr) __attribute__((always_inline)) {
+          constexpr int r = decltype(rr)::value;
+          const int o = 16 * i + g4 + r;
+          if (XENT ? o == lab : (nib >> r) & 1u) {
+            p.zt[XENT ? t : list_slot(p.ls, t, (int)(vw + o))] = acc[i][j][r] * p.scale;
+            acc[i][j][r] = fin;
+          }
+        });
+    });
+  }
+  if (vw + G::WM > p.V) {
+    const int end = p.V > vw ? (int)(p.V - vw) : 0;
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * i + g4 + r >= end) acc[i][j][r] = fin;
+  }
+  const float scale2 = p.scale * LOG2E;
+  float m = fin;
+  if (p.scale < 0.f) {
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fminf(m, acc[i][j][r]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+  }
+  m = gmax4(p.scale == 0.f && m != -INFINITY ? 0.f : m * scale2);
+  const float mb = m == -INFINITY ? 0.f : m;           // nothing left: 2^-inf = 0
+  float s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      s[r & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], scale2, -mb));
+  const float sum = gsum4(s[0] + s[1]);
+  if (ok && lane < 16) *out = make_float2(m, sum);
+}
+
+// few tokens: one tile a workgroup, the weight's loads deep in flight
 template <typename T8, typename G, bool XENT>
-__global__ __launch_bounds__(G_THREADS) void k_head_fwd(
-    const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ W, int64_t ldw,
-    int64_t T, int64_t V, int64_t C, float scale, Listed ls, int nm, int nn, float2* part,
-    int64_t npart, float* zt) {
+__global__ __launch_bounds__(G_THREADS) void k_head_fwd(const FwdArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   int tm, tn;
-  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
+  g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
   const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
-  const GOperand A{W + v0 * ldw, ldw, V - v0, C, nullptr};
-  const GOperand B{h + t0 * ldh, ldh, T - t0, C, nullptr};
+  const GOperand A{p.W + v0 * p.ldw, p.ldw, p.V - v0, p.C, nullptr};
+  const GOperand B{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
   f4_t acc[G::MI][G::NJ];
-  g_tile<T8, G>(smem, A, B, 0, C, acc);
+  g_tile<T8, G>(smem, A, B, 0, p.C, acc);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wr = wave / G::WGN;
   const int64_t vw = v0 + wr * G::WM;                  // the wavefront's first token
-  const int g4 = (lane >> 4) * 4;
-#pragma unroll
-  for (int j = 0; j < G::NJ; ++j) {
+  g_each<G::NJ>([&](auto jj) __attribute__((always_inline)) {
+    constexpr int j = decltype(jj)::value;
     const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
-    const bool ok = t < T;
+    const bool ok = t < p.T;
     int lab = -1;                                      // the label's place among the wavefront's
-    uint32_t words[G::WM / 32];
+    uint32_t words[G::WM / 32] = {};
     if (XENT) {
-      const int64_t y = ok ? ls.labels[t] : -1;
+      const int64_t y = ok ? p.ls.labels[t] : -1;
       lab = y >= vw && y < vw + G::WM ? (int)(y - vw) : -1;
-    } else {
+    } else if (ok) {
 #pragma unroll
-      for (int w = 0; w < G::WM / 32; ++w)
-        words[w] = ok ? ls.mask[t * ls.ldm + (vw >> 5) + w] : 0u;
+      for (int w = 0; w < G::WM / 32; ++w) words[w] = p.ls.mask[t * p.ls.ldm + (vw >> 5) + w];
     }
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < G::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int o = 16 * i + g4 + r;
-        float x = acc[i][j][r] * scale;
-        const bool hit = XENT ? o == lab : ((words[i / 2] >> (o & 31)) & 1) != 0;
-        if (hit) {
-          if (XENT) {
-            zt[t] = x;
-          } else {
-            // the token's slot in its row's ascending list
-            const int32_t* s = ls.sidx + t * ls.k;
-            const int v = (int)(vw + o);
-            int lo = 0, hi = ls.k - 1;
-            while (lo < hi) {
-              const int md = (lo + hi) >> 1;
-              if (s[md] < v) lo = md + 1;
-              else hi = md;
-            }
-            zt[t * ls.k + lo] = x;
-          }
-        }
-        x = hit || vw + o >= V ? -INFINITY : x;
-        acc[i][j][r] = x;
-        m = fmaxf(m, x);
-      }
-    m = gmax4(m);
-    float s = 0.f;
-    const float mb = m == -INFINITY ? 0.f : m;         // nothing left: exp(-inf) = 0
-#pragma unroll
-    for (int i = 0; i < G::MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s += g_exp(acc[i][j][r] - mb);
-    s = gsum4(s);
-    if (ok && lane < 16) part[t * npart + (int64_t)tm * G::WGM + wr] = make_float2(m, s);
+    fwd_column<G, XENT, j>(p, t, vw, lab, words, acc,
+                           p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
+  });
+}
+
+// many tokens: a persistent workgroup on each CU
+template <typename G, bool XENT>
+struct FwdJob : FwdArgs {
+  int64_t lda, ldb;
+  int tiles;
+  __device__ explicit FwdJob(const FwdArgs& a) : FwdArgs(a), lda(a.ldw), ldb(a.ldh) {
+    tiles = a.nm * a.nn;
   }
+  __device__ void place(int lin, int64_t& v0, int64_t& t0, int& tm) const {
+    int tn;
+    g_band(lin, nm, nn, tm, tn);
+    v0 = (int64_t)tm * G::BM;
+    t0 = (int64_t)tn * G::BN;
+  }
+  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+    int64_t v0, t0;
+    int tm;
+    place(lin, v0, t0, tm);
+    A = GOperand{W + v0 * ldw, ldw, V - v0, C, nullptr};
+    B = GOperand{h + t0 * ldh, ldh, T - t0, C, nullptr};
+    k = 0;
+    nch = (int)((C + G_K - 1) / G_K);
+  }
+  // the labels (or the mask words) of the wavefront's 64 rows
+  __device__ void side(int lin, char* priv) const {
+    int64_t v0, t0;
+    int tm;
+    place(lin, v0, t0, tm);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t t = t0 + (wave % G::WGN) * G::WN, left = T - t;
+    if (XENT) {
+      const char* y = (const char*)(ls.labels + t);
+      g_load_lds_words(priv, y, left * 8, lane);
+      g_load_lds_words(priv + 256, y + 256, left * 8 - 256, lane);
+    } else {
+      const int64_t vw = v0 + (wave / G::WGN) * G::WM;
+      const i4_t rs = g_rsrc((const uint16_t*)(ls.mask + t * ls.ldm + (vw >> 5)),
+                             left > 0 ? ((left < G::WN ? left : G::WN) - 1) * ls.ldm * 4 + 16 : 0);
+      g_load_lds(priv, rs, (unsigned)(lane * ls.ldm * 4));
+    }
+  }
+  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+    static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows of 128 tokens");
+    int64_t v0, t0;
+    int tm;
+    place(lin, v0, t0, tm);
+    const int lane = g_lane();
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wr = wave / G::WGN;
+    const int64_t vw = v0 + wr * G::WM;
+    g_each<G::NJ>([&](auto jj) __attribute__((always_inline)) {
+      constexpr int j = decltype(jj)::value;
+      const int n = 16 * j + (lane & 15);
+      const int64_t t = t0 + (wave % G::WGN) * G::WN + n;
+      int lab = -1;
+      uint32_t words[G::WM / 32] = {};
+      if (XENT) {
+        const int64_t y = ((const int64_t*)priv)[n];
+        lab = t < T && y >= vw && y < vw + G::WM ? (int)(y - vw) : -1;
+      } else {
+        const uint4 w = ((const uint4*)priv)[n];
+        words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
+      }
+      fwd_column<G, XENT, j>(*this, t, vw, lab, words, acc,
+                             part + t * npart + (int64_t)tm * G::WGM + wr);
+    });
+  }
+};
+
+template <typename T8, typename G, bool XENT>
+__global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+  g_run<T8, G>(smem, FwdJob<G, XENT>(p));
 }
 
 // The saved state of a forward, in floats: a [T], lse [T], one factor (1 or
@@ -200,7 +332,7 @@ __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ pa
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) ms_join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
-  const float a = m + logf(s);                         // -inf where every token is listed
+  const float a = LN2 * (m + log2f(s));                // -inf where every token is listed
   float loss, lse;
   bool on;
   if (XENT) {
@@ -217,13 +349,13 @@ __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ pa
     float tm = -INFINITY, ts = 0.f, np = 0.f;
     for (int i = lane; i < k; i += 64)
       if (st.sidx[t * k + i] != PAD_IDX) {
-        ms_join(tm, ts, st.zt[t * k + i], 1.f);
+        ms_join(tm, ts, st.zt[t * k + i] * LOG2E, 1.f);
         np += 1.f;
       }
 #pragma unroll
     for (int d = 32; d; d >>= 1) ms_join(tm, ts, __shfl_xor(tm, d), __shfl_xor(ts, d));
     on = wave_sum_f(np) > 0.f;
-    lse = log_add(a, tm + logf(ts));
+    lse = log_add(a, LN2 * (tm + log2f(ts)));
     float l = 0.f;
     for (int i = lane; i < k; i += 64) {
       const float p = st.p[t * k + i];
@@ -397,8 +529,9 @@ __global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T, int k,
                                                   const int64_t* __restrict__ labels,
                                                   int64_t ignore, const float* __restrict__ g,
                                                   int per_row, const float* __restrict__ gmax,
-                                                  float zscale, float scale, float* rowb,
-                                                  float* ratio, uint64_t* live, float* fac) {
+                                                  float zscale, float scale, float* a2,
+                                                  float* rowb, float* ratio, uint64_t* live,
+                                                  float* fac) {
   const int64_t t = (int64_t)blockIdx.x * 64 + threadIdx.x;
   float r = 0.f;
   const float big = per_row ? gmax[0] : 1.f;
@@ -410,6 +543,7 @@ __global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T, int k,
     r = r * zscale;
     const float a = st.a[t], qt = expf(a - st.lse[t]);
     ratio[t] = r;
+    a2[t] = a * LOG2E;
     rowb[t] = r == 0.f ? 0.f : r * (XENT ? qt : st.mass[t] * qt - st.pt[t]);
   }
   const uint64_t bits = __ballot(!(r == 0.f));
@@ -418,42 +552,126 @@ __global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T, int k,
 }
 
 // dz of a piece of the vocabulary: dz[t][v - vbeg] = rowb exp(z - a), zeros
-// in the columns past the vocabulary; the listed tokens' own follow (k_dz_listed).
+// in the columns past the vocabulary (and where rowb is 0, whatever z is); the
+// listed tokens' own follow (k_dz_listed).  a2 = a in units of log 2.
+struct DzArgs {
+  const uint16_t *h, *W;
+  int64_t ldh, ldw, T, nv, C;
+  float scale;
+  const float *a2, *rowb;
+  int nm, nn;
+  uint16_t* dz;
+  int64_t ldz;
+};
+
+// 4 consecutive tokens from v on, of row t
+template <typename T8>
+__device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2, float b,
+                                         int64_t left) {
+  uint16_t o[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    o[r] = to16<T8>(b * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], scale2, -a2)));
+  if (left < 4) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r >= left) o[r] = 0;
+  }
+  const uint2 u = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
+  return b == 0.f ? make_uint2(0u, 0u) : u;
+}
+
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dz(
-    const uint16_t* __restrict__ h, int64_t ldh, const uint16_t* __restrict__ W, int64_t ldw,
-    int64_t T, int64_t nv, int64_t C, float scale, const float* __restrict__ a,
-    const float* __restrict__ rowb, int nm, int nn, uint16_t* dz, int64_t ldz) {
+__global__ __launch_bounds__(G_THREADS) void k_head_dz(const DzArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   int tm, tn;
-  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
+  g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
   const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
-  const GOperand A{W + v0 * ldw, ldw, nv - v0, C, nullptr};
-  const GOperand B{h + t0 * ldh, ldh, T - t0, C, nullptr};
+  const GOperand A{p.W + v0 * p.ldw, p.ldw, p.nv - v0, p.C, nullptr};
+  const GOperand B{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
   f4_t acc[G::MI][G::NJ];
-  g_tile<T8, G>(smem, A, B, 0, C, acc);
+  g_tile<T8, G>(smem, A, B, 0, p.C, acc);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int64_t vw = v0 + (wave / G::WGN) * G::WM;
+  const float scale2 = p.scale * LOG2E;
 #pragma unroll
   for (int j = 0; j < G::NJ; ++j) {
     const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
-    if (t >= T) continue;
-    const float b = rowb[t], at = a[t];
+    if (t >= p.T) continue;
+    const float b = p.rowb[t], a2 = p.a2[t];
 #pragma unroll
     for (int i = 0; i < G::MI; ++i) {
-      const int64_t v = vw + 16 * i + 4 * (lane >> 4);
-      uint16_t o[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = b * g_exp(acc[i][j][r] * scale - at);
-        o[r] = b == 0.f || v + r >= nv ? 0 : to16<T8>(x);
-      }
-      if (v < ldz)
-        *(uint2*)(dz + t * ldz + v) = make_uint2(o[0] | (uint32_t)o[1] << 16,
-                                                 o[2] | (uint32_t)o[3] << 16);
+      const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below ldz
+      *(uint2*)(p.dz + t * p.ldz + v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v);
     }
   }
+}
+
+template <typename T8, typename G>
+struct DzJob : DzArgs {
+  int64_t lda, ldb;
+  int tiles;
+  __device__ explicit DzJob(const DzArgs& a) : DzArgs(a), lda(a.ldw), ldb(a.ldh) {
+    tiles = a.nm * a.nn;
+  }
+  __device__ void place(int lin, int64_t& v0, int64_t& t0) const {
+    int tm, tn;
+    g_band(lin, nm, nn, tm, tn);
+    v0 = (int64_t)tm * G::BM;
+    t0 = (int64_t)tn * G::BN;
+  }
+  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+    int64_t v0, t0;
+    place(lin, v0, t0);
+    A = GOperand{W + v0 * ldw, ldw, nv - v0, C, nullptr};
+    B = GOperand{h + t0 * ldh, ldh, T - t0, C, nullptr};
+    k = 0;
+    nch = (int)((C + G_K - 1) / G_K);
+  }
+  __device__ void side(int lin, char* priv) const {
+    int64_t v0, t0;
+    place(lin, v0, t0);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t t = t0 + (wave % G::WGN) * G::WN, left = (T - t) * 4;
+    g_load_lds_words(priv, a2 + t, left, lane);
+    g_load_lds_words(priv + 256, rowb + t, left, lane);
+  }
+  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+    static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows");
+    int64_t v0, t0;
+    place(lin, v0, t0);
+    const int lane = g_lane(), n16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t vw = v0 + (wave / G::WGN) * G::WM, tw = t0 + (wave % G::WGN) * G::WN;
+    const float scale2 = scale * LOG2E;
+    float at[G::NJ], b[G::NJ];
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) {
+      at[j] = ((const float*)priv)[16 * j + n16];
+      b[j] = ((const float*)(priv + 256))[16 * j + n16];
+    }
+    const bool whole = vw + G::WM <= nv;
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) {
+      uint2 u[G::MI];
+#pragma unroll
+      for (int i = 0; i < G::MI; ++i)
+        u[i] = dz_pack<T8>(acc[i][j], scale2, at[j], b[j],
+                           whole ? 4 : nv - (vw + 16 * i + 4 * (lane >> 4)));
+      g_rows_out<G>(priv, u, [&](int r, int m, const uint4& x) {
+        const int64_t t = tw + 16 * j + r;
+        if (t < T) *(uint4*)(dz + t * ldz + vw + m) = x;         // vw + 128 <= ldz
+      });
+    }
+  }
+};
+
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+  g_run<T8, G>(smem, DzJob<T8, G>(p));
 }
 
 // the listed tokens' dz within [vbeg, vbeg + nv)
@@ -474,41 +692,93 @@ __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
   dz[t * ldz + v - vbeg] = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
 }
 
-// dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the split's v
-template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dh(
-    const uint16_t* __restrict__ W, int64_t ldw, const uint16_t* __restrict__ dz, int64_t ldz,
-    int64_t T, int64_t nv, int64_t C, int64_t span, int nm, int nn, float* P, int add) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
-  int tm, tn;
-  const int lin = g_xcd(blockIdx.x, gridDim.x), split = lin / (nm * nn);
-  g_band(lin - split * nm * nn, nm, nn, tm, tn);
-  const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
-  const int64_t kb = split * span, ke = kb + span < nv ? kb + span : nv;
-  const GOperand A{W + c0, ldw, C - c0, nv, nullptr};
-  const GOperand B{dz + t0 * ldz, ldz, T - t0, ldz, nullptr};
-  f4_t acc[G::MI][G::NJ];
-  g_tile<T8, G>(smem, A, B, kb, ke, acc);
-  const int lane = threadIdx.x & 63;
+// dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the
+// split's v (span of them, a multiple of 64)
+struct DhArgs {
+  const uint16_t *W, *dz;
+  int64_t ldw, ldz, T, nv, C, span;
+  int nm, nn, ns;
+  float* P;
+  int add;
+};
+
+template <typename G>
+__device__ __forceinline__ void dh_finish(const DhArgs& p, int64_t c0, int64_t t0, int split,
+                                          const f4_t (&acc)[G::MI][G::NJ]) {
+  const int lane = g_lane();
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  P += (int64_t)split * T * C;
+  float* P = p.P + (int64_t)split * p.T * p.C;
 #pragma unroll
   for (int j = 0; j < G::NJ; ++j) {
     const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
-    if (t >= T) continue;
+    if (t >= p.T) continue;
 #pragma unroll
     for (int i = 0; i < G::MI; ++i) {
       const int64_t c = c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4);
-      if (c >= C) continue;
-      float4* q = (float4*)(P + t * C + c);
+      if (c >= p.C) continue;
+      float4* q = (float4*)(P + t * p.C + c);
       float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-      if (add) {
+      if (p.add) {
         const float4 u = *q;
         v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
       }
       *q = v;
     }
   }
+}
+
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dh(const DhArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
+  int tm, tn;
+  const int lin = g_xcd(blockIdx.x, gridDim.x), split = lin / (p.nm * p.nn);
+  g_band(lin - split * p.nm * p.nn, p.nm, p.nn, tm, tn);
+  const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
+  const int64_t kb = split * p.span, ke = kb + p.span < p.nv ? kb + p.span : p.nv;
+  const GOperand A{p.W + c0, p.ldw, p.C - c0, p.nv, nullptr};
+  const GOperand B{p.dz + t0 * p.ldz, p.ldz, p.T - t0, p.ldz, nullptr};
+  f4_t acc[G::MI][G::NJ];
+  g_tile<T8, G>(smem, A, B, kb, ke, acc);
+  dh_finish<G>(p, c0, t0, split, acc);
+}
+
+template <typename G>
+struct DhJob : DhArgs {
+  int64_t lda, ldb;
+  int tiles;
+  __device__ explicit DhJob(const DhArgs& a) : DhArgs(a), lda(a.ldw), ldb(a.ldz) {
+    tiles = a.nm * a.nn * a.ns;
+  }
+  __device__ void place(int lin, int64_t& c0, int64_t& t0, int& split) const {
+    int tm, tn;
+    split = lin / (nm * nn);
+    g_band(lin - split * nm * nn, nm, nn, tm, tn);
+    c0 = (int64_t)tm * G::BM;
+    t0 = (int64_t)tn * G::BN;
+  }
+  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+    int64_t c0, t0;
+    int split;
+    place(lin, c0, t0, split);
+    A = GOperand{W + c0, ldw, C - c0, nv, nullptr};
+    B = GOperand{dz + t0 * ldz, ldz, T - t0, ldz, nullptr};
+    k = split * span;
+    const int64_t n = nv - k < span ? nv - k : span;   // > 0 for every split of a launch
+    nch = (int)((n + G_K - 1) / G_K);
+  }
+  __device__ void side(int, char*) const {}
+  __device__ void finish(int lin, char*, f4_t (&acc)[G::MI][G::NJ]) const {
+    int64_t c0, t0;
+    int split;
+    place(lin, c0, t0, split);
+    dh_finish<G>(*this, c0, t0, split, acc);
+  }
+};
+
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+  g_run<T8, G>(smem, DhJob<G>(p));
 }
 
 // dh = fac * (P[0] + P[1] + ...), rounded once; 4 channels a thread
@@ -532,35 +802,64 @@ __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int
 }
 
 // dW[v][c] = fac * sum_t dz[t][v] h[t][c] of a piece's rows v
+struct DwArgs {
+  const uint16_t *h, *dz;
+  int64_t ldh, ldz, T, nv, C;
+  const uint64_t* live;
+  int nm, nn;
+  const float* fac;
+  uint16_t* dW;
+  int64_t ldo;
+};
+
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dw(
-    const uint16_t* __restrict__ h, int64_t ldh, const uint64_t* __restrict__ live,
-    const uint16_t* __restrict__ dz, int64_t ldz, int64_t T, int64_t nv, int64_t C, int nm,
-    int nn, const float* __restrict__ fac, uint16_t* dW, int64_t ldo) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
-  int tm, tn;
-  g_band(g_xcd(blockIdx.x, gridDim.x), nm, nn, tm, tn);
-  const int64_t c0 = (int64_t)tm * G::BM, v0 = (int64_t)tn * G::BN;
-  const GOperand A{h + c0, ldh, C - c0, T, live};
-  const GOperand B{dz + v0, ldz, ldz - v0, T, nullptr};
-  f4_t acc[G::MI][G::NJ];
-  g_tile<T8, G>(smem, A, B, 0, T, acc);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const float f = fac[0];
+struct DwJob : DwArgs {
+  int64_t lda, ldb;
+  int tiles;
+  float f;
+  __device__ explicit DwJob(const DwArgs& a) : DwArgs(a), lda(a.ldh), ldb(a.ldz), f(a.fac[0]) {
+    tiles = a.nm * a.nn;
+  }
+  __device__ void place(int lin, int64_t& c0, int64_t& v0) const {
+    int tm, tn;
+    g_band(lin, nm, nn, tm, tn);
+    c0 = (int64_t)tm * G::BM;
+    v0 = (int64_t)tn * G::BN;
+  }
+  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+    int64_t c0, v0;
+    place(lin, c0, v0);
+    A = GOperand{h + c0, ldh, C - c0, T, live};
+    B = GOperand{dz + v0, ldz, ldz - v0, T, nullptr};
+    k = 0;
+    nch = (int)((T + G_K - 1) / G_K);
+  }
+  __device__ void side(int, char*) const {}
+  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+    int64_t c0, v0;
+    place(lin, c0, v0);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t cw = c0 + (wave / G::WGN) * G::WM, vw = v0 + (wave % G::WGN) * G::WN;
 #pragma unroll
-  for (int j = 0; j < G::NJ; ++j) {
-    const int64_t v = v0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
-    if (v >= nv) continue;
+    for (int j = 0; j < G::NJ; ++j) {
+      uint2 u[G::MI];
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i) {
-      const int64_t c = c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4);
-      if (c >= C) continue;
-      *(uint2*)(dW + v * ldo + c) = make_uint2(
-          to16<T8>(f * acc[i][j][0]) | (uint32_t)to16<T8>(f * acc[i][j][1]) << 16,
-          to16<T8>(f * acc[i][j][2]) | (uint32_t)to16<T8>(f * acc[i][j][3]) << 16);
+      for (int i = 0; i < G::MI; ++i)
+        u[i] = make_uint2(
+            to16<T8>(f * acc[i][j][0]) | (uint32_t)to16<T8>(f * acc[i][j][1]) << 16,
+            to16<T8>(f * acc[i][j][2]) | (uint32_t)to16<T8>(f * acc[i][j][3]) << 16);
+      g_rows_out<G>(priv, u, [&](int r, int m, const uint4& x) {
+        const int64_t v = vw + 16 * j + r;
+        if (v < nv && cw + m < C) *(uint4*)(dW + v * ldo + cw + m) = x;   // C: a multiple of 8
+      });
     }
   }
+};
+
+template <typename T8, typename G>
+__global__ __launch_bounds__(G_THREADS) void k_head_dw(const DwArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+  g_run<T8, G>(smem, DwJob<T8, G>(p));
 }
 
 // ---------------------------------------------------------------------------
@@ -624,18 +923,20 @@ struct FwdWs {
 };
 
 struct GradWs {
-  int64_t piece;
-  int ns;
+  int64_t piece, span;
+  int ns;                  // splits of dh's sums over the first (largest) piece
   uint16_t* dz;
-  float *P, *rowb, *ratio, *fac, *gmax;
+  float *P, *a2, *rowb, *ratio, *fac, *gmax;
   uint64_t* live;
   size_t bytes;
   GradWs(void* ws, size_t cap, int64_t T, int64_t V, int64_t C, bool& ok) {
     WsCarver w(ws, cap);
     piece = piece_of(T, V);
-    ns = dh_splits(T, C, piece);
+    span = cdiv(cdiv(piece < V ? piece : V, dh_splits(T, C, piece)), G_K) * G_K;
+    ns = (int)cdiv(piece < V ? piece : V, span);
     dz = w.take<uint16_t>((size_t)(T * piece));
     P = w.take<float>((size_t)(T * C) * ns);
+    a2 = w.take<float>((size_t)T);
     rowb = w.take<float>((size_t)T);
     ratio = w.take<float>((size_t)T);
     fac = w.take<float>(1);
@@ -660,24 +961,33 @@ static int check_head(const void* h, int64_t ldh, const void* W, int64_t ldw, in
   return CRBQ_OK;
 }
 
+// Workgroups of a persistent launch: one per CU (160 KB of LDS each).
+static unsigned persistent(int64_t tiles) {
+  constexpr int CUS = 256;
+  return (unsigned)(tiles < CUS ? tiles : CUS);
+}
+
 template <typename T8, typename G, bool XENT>
-static void launch_fwd(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw, int64_t T,
-                       int64_t V, int64_t C, float scale, const Listed& ls, const FwdWs& w,
-                       float* zt, hipStream_t s) {
-  const int nm = (int)cdiv(V, G::BM), nn = (int)cdiv(T, G::BN);
-  k_head_fwd<T8, G, XENT><<<(unsigned)((int64_t)nm * nn), G_THREADS, 0, s>>>(
-      h, ldh, W, ldw, T, V, C, scale, ls, nm, nn, w.part, n_part(T, V), zt);
+static void launch_fwd(FwdArgs p, hipStream_t s) {
+  p.nm = (int)cdiv(p.V, G::BM);
+  p.nn = (int)cdiv(p.T, G::BN);
+  const int64_t tiles = (int64_t)p.nm * p.nn;
+  if constexpr (G::NS == 2)
+    k_head_fwd_p<T8, G, XENT><<<persistent(tiles), G_THREADS, 0, s>>>(p);
+  else
+    k_head_fwd<T8, G, XENT><<<(unsigned)tiles, G_THREADS, 0, s>>>(p);
 }
 
 template <typename T8, bool XENT>
 static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T, int64_t V,
                     int64_t C, float scale, const Listed& ls, int64_t ignore, int reduction,
                     float* loss, const State& st, const FwdWs& w, hipStream_t s) {
-  const uint16_t *hh = (const uint16_t*)h, *ww = (const uint16_t*)W;
+  const FwdArgs p{(const uint16_t*)h, (const uint16_t*)W, ldh, ldw, T, V, C, scale, ls, 0, 0,
+                  w.part, n_part(T, V), st.zt};
   switch (token_tile(T)) {
-    case 0: launch_fwd<T8, ZS, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s); break;
-    case 1: launch_fwd<T8, ZM, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s); break;
-    default: launch_fwd<T8, ZL, XENT>(hh, ldh, ww, ldw, T, V, C, scale, ls, w, st.zt, s);
+    case 0: launch_fwd<T8, ZS, XENT>(p, s); break;
+    case 1: launch_fwd<T8, ZM, XENT>(p, s); break;
+    default: launch_fwd<T8, ZL, XENT>(p, s);
   }
   CRBQ_LAUNCH_CHECK();
   float* rows = reduction ? w.rows : loss;
@@ -703,7 +1013,7 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
   }
   const float zs = dz_scale<T8>();
   k_grad_rows<XENT><<<(unsigned)cdiv(T, 64), 64, 0, s>>>(st, T, k, labels, ignore, g, per_row,
-                                                         w.gmax, zs, scale, w.rowb, w.ratio,
+                                                         w.gmax, zs, scale, w.a2, w.rowb, w.ratio,
                                                          w.live, w.fac);
   CRBQ_LAUNCH_CHECK();
   const int nt = (int)cdiv(T, GZ::BN);
@@ -711,23 +1021,30 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
     const int64_t nv = V - v < w.piece ? V - v : w.piece, ldz = cdiv(nv, 256) * 256;
     const uint16_t* Wv = W + v * ldw;
     const int nm = (int)cdiv(nv, GZ::BM);
-    k_head_dz<T8, GZ><<<(unsigned)(nm * nt), G_THREADS, 0, s>>>(
-        h, ldh, Wv, ldw, T, nv, C, scale, st.a, w.rowb, nm, nt, w.dz, ldz);
+    const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, ldz};
+    if constexpr (GZ::NS == 2)
+      k_head_dz_p<T8, GZ><<<persistent((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
+    else
+      k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
     CRBQ_LAUNCH_CHECK();
     k_dz_listed<T8, XENT><<<(unsigned)cdiv(XENT ? T : T * k, 256), 256, 0, s>>>(
         st, T, k, labels, w.ratio, v, nv, w.dz, ldz);
     CRBQ_LAUNCH_CHECK();
     if (dh) {
       const int mh = (int)cdiv(C, GH::BM);
-      const int64_t span = cdiv(cdiv(w.piece, w.ns), 64) * 64;
-      k_head_dh<T8, GH><<<(unsigned)(mh * nt * w.ns), G_THREADS, 0, s>>>(
-          Wv, ldw, w.dz, ldz, T, nv, C, span, mh, nt, w.P, v > 0);
+      const DhArgs q{Wv, w.dz, ldw, ldz, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
+                     v > 0};
+      const int64_t tiles = (int64_t)mh * nt * q.ns;
+      if constexpr (GH::NS == 2)
+        k_head_dh_p<T8, GH><<<persistent(tiles), G_THREADS, 0, s>>>(q);
+      else
+        k_head_dh<T8, GH><<<(unsigned)tiles, G_THREADS, 0, s>>>(q);
       CRBQ_LAUNCH_CHECK();
     }
     if (dW) {
       const int mw = (int)cdiv(C, WL::BM), nw = (int)cdiv(nv, WL::BN);
-      k_head_dw<T8, WL><<<(unsigned)(mw * nw), G_THREADS, 0, s>>>(
-          h, ldh, w.live, w.dz, ldz, T, nv, C, mw, nw, w.fac, dW + v * ldo, ldo);
+      k_head_dw<T8, WL><<<persistent((int64_t)mw * nw), G_THREADS, 0, s>>>(
+          DwArgs{h, w.dz, ldh, ldz, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
       CRBQ_LAUNCH_CHECK();
     }
   }
