@@ -223,13 +223,14 @@ struct FwdJob : FwdArgs {
   __device__ explicit FwdJob(const FwdArgs& a) : FwdArgs(a), lda(a.ldw), ldb(a.ldh) {
     tiles = a.nm * a.nn;
   }
-  __device__ void place(int lin, int64_t& v0, int64_t& t0, int& tm) const {
+  __device__ __forceinline__ void place(int lin, int64_t& v0, int64_t& t0, int& tm) const {
     int tn;
     g_band(lin, nm, nn, tm, tn);
     v0 = (int64_t)tm * G::BM;
     t0 = (int64_t)tn * G::BN;
   }
-  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+  __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
+                                       int& nch) const {
     int64_t v0, t0;
     int tm;
     place(lin, v0, t0, tm);
@@ -239,7 +240,7 @@ struct FwdJob : FwdArgs {
     nch = (int)((C + G_K - 1) / G_K);
   }
   // the labels (or the mask words) of the wavefront's 64 rows
-  __device__ void side(int lin, char* priv) const {
+  __device__ __forceinline__ void side(int lin, char* priv) const {
     int64_t v0, t0;
     int tm;
     place(lin, v0, t0, tm);
@@ -257,7 +258,7 @@ struct FwdJob : FwdArgs {
       g_load_lds(priv, rs, (unsigned)(lane * ls.ldm * 4));
     }
   }
-  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
     static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows of 128 tokens");
     int64_t v0, t0;
     int tm;
@@ -615,13 +616,14 @@ struct DzJob : DzArgs {
   __device__ explicit DzJob(const DzArgs& a) : DzArgs(a), lda(a.ldw), ldb(a.ldh) {
     tiles = a.nm * a.nn;
   }
-  __device__ void place(int lin, int64_t& v0, int64_t& t0) const {
+  __device__ __forceinline__ void place(int lin, int64_t& v0, int64_t& t0) const {
     int tm, tn;
     g_band(lin, nm, nn, tm, tn);
     v0 = (int64_t)tm * G::BM;
     t0 = (int64_t)tn * G::BN;
   }
-  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+  __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
+                                       int& nch) const {
     int64_t v0, t0;
     place(lin, v0, t0);
     A = GOperand{W + v0 * ldw, ldw, nv - v0, C, nullptr};
@@ -629,7 +631,7 @@ struct DzJob : DzArgs {
     k = 0;
     nch = (int)((C + G_K - 1) / G_K);
   }
-  __device__ void side(int lin, char* priv) const {
+  __device__ __forceinline__ void side(int lin, char* priv) const {
     int64_t v0, t0;
     place(lin, v0, t0);
     const int lane = threadIdx.x & 63;
@@ -638,7 +640,7 @@ struct DzJob : DzArgs {
     g_load_lds_words(priv, a2 + t, left, lane);
     g_load_lds_words(priv + 256, rowb + t, left, lane);
   }
-  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
     static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows");
     int64_t v0, t0;
     place(lin, v0, t0);
@@ -749,14 +751,15 @@ struct DhJob : DhArgs {
   __device__ explicit DhJob(const DhArgs& a) : DhArgs(a), lda(a.ldw), ldb(a.ldz) {
     tiles = a.nm * a.nn * a.ns;
   }
-  __device__ void place(int lin, int64_t& c0, int64_t& t0, int& split) const {
+  __device__ __forceinline__ void place(int lin, int64_t& c0, int64_t& t0, int& split) const {
     int tm, tn;
     split = lin / (nm * nn);
     g_band(lin - split * nm * nn, nm, nn, tm, tn);
     c0 = (int64_t)tm * G::BM;
     t0 = (int64_t)tn * G::BN;
   }
-  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+  __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
+                                       int& nch) const {
     int64_t c0, t0;
     int split;
     place(lin, c0, t0, split);
@@ -766,8 +769,8 @@ struct DhJob : DhArgs {
     const int64_t n = nv - k < span ? nv - k : span;   // > 0 for every split of a launch
     nch = (int)((n + G_K - 1) / G_K);
   }
-  __device__ void side(int, char*) const {}
-  __device__ void finish(int lin, char*, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void side(int, char*) const {}
+  __device__ __forceinline__ void finish(int lin, char*, f4_t (&acc)[G::MI][G::NJ]) const {
     int64_t c0, t0;
     int split;
     place(lin, c0, t0, split);
@@ -820,13 +823,14 @@ struct DwJob : DwArgs {
   __device__ explicit DwJob(const DwArgs& a) : DwArgs(a), lda(a.ldh), ldb(a.ldz), f(a.fac[0]) {
     tiles = a.nm * a.nn;
   }
-  __device__ void place(int lin, int64_t& c0, int64_t& v0) const {
+  __device__ __forceinline__ void place(int lin, int64_t& c0, int64_t& v0) const {
     int tm, tn;
     g_band(lin, nm, nn, tm, tn);
     c0 = (int64_t)tm * G::BM;
     v0 = (int64_t)tn * G::BN;
   }
-  __device__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k, int& nch) const {
+  __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
+                                       int& nch) const {
     int64_t c0, v0;
     place(lin, c0, v0);
     A = GOperand{h + c0, ldh, C - c0, T, live};
@@ -834,8 +838,8 @@ struct DwJob : DwArgs {
     k = 0;
     nch = (int)((T + G_K - 1) / G_K);
   }
-  __device__ void side(int, char*) const {}
-  __device__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void side(int, char*) const {}
+  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
     int64_t c0, v0;
     place(lin, c0, v0);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
