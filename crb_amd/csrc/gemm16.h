@@ -1,6 +1,6 @@
 // 16-bit matrix-product tiles of the output-head kernels (head.hip).
 //
-// A workgroup of 8 wavefronts sums D[m][n] = sum_k A[m][k] B[n][k] over a
+// A workgroup sums D[m][n] = sum_k A[m][k] B[n][k] over a
 // BM x BN tile on v_mfma_f32_16x16x32_{f16,bf16} (fp32 accumulate).  Each
 // operand comes in one of two layouts:
 //   K-contiguous (KC): element (row, k) at P[row * ld + k];
@@ -31,7 +31,6 @@ typedef __fp16 tr4_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef __attribute__((address_space(3))) tr4_t lds_tr4_t;
 
 constexpr int G_K = 64;                 // k per stage
-constexpr int G_THREADS = 512;
 constexpr int64_t G_MAX_LD = (int64_t)1 << 22;   // 256 rows * ld * 2 bytes < 2^31
 
 template <typename T8>
@@ -76,11 +75,11 @@ __device__ __forceinline__ i4_t g_rsrc(const uint16_t* base, int64_t nrec) {
 // Row permutation of a K-strided stage (of 16-byte chunks, within 16).
 __device__ __forceinline__ int g_swz(int t) { return ((t & 3) | ((t >> 1) & 4)) << 1; }
 
-template <int R, bool KC>
+template <int R, bool KC, int NW>
 struct GStage {
   static constexpr int BYTES = R * G_K * 2;
   static constexpr int LOADS = BYTES / 1024;                     // 1 KB each
-  static constexpr int PER_WAVE = LOADS >= 8 ? LOADS / 8 : 1;    // fewer: some are issued twice
+  static constexpr int PER_WAVE = LOADS >= NW ? LOADS / NW : 1;  // fewer: some are issued twice
   static constexpr int ROWS_PER_LOAD = KC ? 8 : 512 / R;
   static_assert(KC ? R % 16 == 0 : (R == 128 || R == 256), "stage shape");
 
@@ -127,14 +126,15 @@ __device__ __forceinline__ T8 g_tr_frag(const char* p) {
   return __builtin_bit_cast(T8, v);
 }
 
-// Tile geometry: WGM x WGN wavefronts, NS stages in LDS (NS - 1 in flight).
-template <int BM_, int BN_, int WGM_, int NS_, bool AKC_, bool BKC_>
+// Tile geometry: WGM x WGN wavefronts, NS stages in LDS.
+template <int BM_, int BN_, int WGM_, int WGN_, int NS_, bool AKC_, bool BKC_>
 struct GTile {
-  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = 8 / WGM_, NS = NS_;
+  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, NS = NS_;
+  static constexpr int NW = WGM * WGN, THREADS = 64 * NW;
   static constexpr bool AKC = AKC_, BKC = BKC_;
   static constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 16, NJ = WN / 16;
-  using SA = GStage<BM, AKC>;
-  using SB = GStage<BN, BKC>;
+  using SA = GStage<BM, AKC, NW>;
+  using SB = GStage<BN, BKC, NW>;
   static constexpr int STAGE = SA::BYTES + SB::BYTES;
   static constexpr int LDS = NS * STAGE;
   static constexpr int LW = SA::PER_WAVE + SB::PER_WAVE;         // loads of a wavefront, a stage
@@ -244,6 +244,8 @@ __device__ __forceinline__ void g_each(const F& f) {
   }
 }
 
+constexpr int G_PRIV = 32 * 1024;       // LDS beside the stages of g_run, in equal shares
+
 // The lane, for an epilogue: opaque, so that what an epilogue computes from it
 // is computed there and not kept in registers over the products.
 __device__ __forceinline__ int g_lane() {
@@ -317,7 +319,7 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
 // gap: tiles lin, lin + gridDim, ... of job.tiles.
 //   job.tile(lin, A, B, k_beg, nch)  a tile's operands, first k and stages (>= 1)
 //   job.side(lin, priv)              loads what the tile's epilogue needs into the
-//                                    wavefront's own 4 KB of LDS (g_load_lds*)
+//                                    wavefront's own share of G_PRIV (g_load_lds*)
 //   job.finish(lin, priv, acc)       the epilogue
 // Two stages in LDS.  While the MFMAs of one half stage run, the fragments of
 // the next half are read into the other register set.  One barrier a stage,
@@ -327,12 +329,11 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
 // read): no MFMA waits for an LDS read that could only start behind a
 // barrier.  The next tile's first stages are loaded under this tile's last, so
 // its loads run under the epilogue too.
-constexpr int G_PRIV = 4096;
 template <typename T8, typename G, typename Job>
 __device__ __forceinline__ void g_run(char* smem, const Job& job) {
-  static_assert(G::NS == 2, "two stages");
+  static_assert(G::NS == 2 && G::NJ <= G::MI, "two stages");
   const GLane<T8, G> L(job.lda, job.ldb);
-  char* priv = smem + G::LDS + L.wave * G_PRIV;
+  char* priv = smem + G::LDS + L.wave * (G_PRIV / G::NW);
   const int nwg = gridDim.x, first = g_xcd(blockIdx.x, nwg);
   // the stage to be loaded next: c of tile ll
   int ll = first, lc = 0, ln = 0;
@@ -381,9 +382,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
       const int at = par * G::STAGE, nx = G::STAGE - at;
       const auto s = source();
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j) b1[j] = L.fragB(smem, at, 1, j);
-#pragma unroll
       for (int i = 0; i < G::MI; ++i) {
+        if (i < G::NJ) b1[i] = L.fragB(smem, at, 1, i);
         a1[i] = L.fragA(smem, at, 1, i);
 #pragma unroll
         for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a0[i], b0[j], acc[i][j]);
@@ -392,9 +392,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
       g_wait_vm<0>();
       g_sync_lds();
 #pragma unroll
-      for (int j = 0; j < G::NJ; ++j) b0[j] = L.fragB(smem, nx, 0, j);
-#pragma unroll
       for (int i = 0; i < G::MI; ++i) {
+        if (i < G::NJ) b0[i] = L.fragB(smem, nx, 0, i);
         a0[i] = L.fragA(smem, nx, 0, i);
 #pragma unroll
         for (int q = 0; q < G::LW; ++q)

@@ -184,7 +184,7 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
 
 // few tokens: one tile a workgroup, the weight's loads deep in flight
 template <typename T8, typename G, bool XENT>
-__global__ __launch_bounds__(G_THREADS) void k_head_fwd(const FwdArgs p) {
+__global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   int tm, tn;
   g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
@@ -249,17 +249,22 @@ struct FwdJob : FwdArgs {
     const int64_t t = t0 + (wave % G::WGN) * G::WN, left = T - t;
     if (XENT) {
       const char* y = (const char*)(ls.labels + t);
-      g_load_lds_words(priv, y, left * 8, lane);
-      g_load_lds_words(priv + 256, y + 256, left * 8 - 256, lane);
+#pragma unroll
+      for (int b = 0; b < G::WN * 8; b += 256)
+        g_load_lds_words(priv + b, y + b, left * 8 - b, lane);
     } else {
       const int64_t vw = v0 + (wave / G::WGN) * G::WM;
-      const i4_t rs = g_rsrc((const uint16_t*)(ls.mask + t * ls.ldm + (vw >> 5)),
-                             left > 0 ? ((left < G::WN ? left : G::WN) - 1) * ls.ldm * 4 + 16 : 0);
-      g_load_lds(priv, rs, (unsigned)(lane * ls.ldm * 4));
+      const int64_t rows = left < G::WN ? left : G::WN;
+#pragma unroll
+      for (int b = 0; b < G::WN; b += 64)
+        g_load_lds(priv + b * 16,
+                   g_rsrc((const uint16_t*)(ls.mask + t * ls.ldm + (vw >> 5)),
+                          rows > 0 ? (rows - 1) * ls.ldm * 4 + 16 : 0),
+                   (unsigned)((b + lane) * ls.ldm * 4));
     }
   }
   __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
-    static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows of 128 tokens");
+    static_assert(G::WN % 64 == 0 && G::WM == 128, "side() holds rows of 128 tokens");
     int64_t v0, t0;
     int tm;
     place(lin, v0, t0, tm);
@@ -287,8 +292,8 @@ struct FwdJob : FwdArgs {
 };
 
 template <typename T8, typename G, bool XENT>
-__global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+__global__ __launch_bounds__(G::THREADS) void k_head_fwd_p(const FwdArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
   g_run<T8, G>(smem, FwdJob<G, XENT>(p));
 }
 
@@ -583,7 +588,7 @@ __device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2
 }
 
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dz(const DzArgs p) {
+__global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   int tm, tn;
   g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
@@ -637,11 +642,14 @@ struct DzJob : DzArgs {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t t = t0 + (wave % G::WGN) * G::WN, left = (T - t) * 4;
-    g_load_lds_words(priv, a2 + t, left, lane);
-    g_load_lds_words(priv + 256, rowb + t, left, lane);
+#pragma unroll
+    for (int b = 0; b < G::WN * 4; b += 256) {
+      g_load_lds_words(priv + b, (const char*)(a2 + t) + b, left - b, lane);
+      g_load_lds_words(priv + G::WN * 4 + b, (const char*)(rowb + t) + b, left - b, lane);
+    }
   }
   __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
-    static_assert(G::WN == 64 && G::WM == 128, "side() holds 64 rows");
+    static_assert(G::WN % 64 == 0 && G::WM == 128, "side() holds whole words");
     int64_t v0, t0;
     place(lin, v0, t0);
     const int lane = g_lane(), n16 = lane & 15;
@@ -652,7 +660,7 @@ struct DzJob : DzArgs {
 #pragma unroll
     for (int j = 0; j < G::NJ; ++j) {
       at[j] = ((const float*)priv)[16 * j + n16];
-      b[j] = ((const float*)(priv + 256))[16 * j + n16];
+      b[j] = ((const float*)priv)[G::WN + 16 * j + n16];
     }
     const bool whole = vw + G::WM <= nv;
 #pragma unroll
@@ -671,8 +679,8 @@ struct DzJob : DzArgs {
 };
 
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+__global__ __launch_bounds__(G::THREADS) void k_head_dz_p(const DzArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
   g_run<T8, G>(smem, DzJob<T8, G>(p));
 }
 
@@ -730,7 +738,7 @@ __device__ __forceinline__ void dh_finish(const DhArgs& p, int64_t c0, int64_t t
 }
 
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dh(const DhArgs p) {
+__global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
   int tm, tn;
   const int lin = g_xcd(blockIdx.x, gridDim.x), split = lin / (p.nm * p.nn);
@@ -779,8 +787,8 @@ struct DhJob : DhArgs {
 };
 
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+__global__ __launch_bounds__(G::THREADS) void k_head_dh_p(const DhArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
   g_run<T8, G>(smem, DhJob<G>(p));
 }
 
@@ -861,8 +869,8 @@ struct DwJob : DwArgs {
 };
 
 template <typename T8, typename G>
-__global__ __launch_bounds__(G_THREADS) void k_head_dw(const DwArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + 8 * G_PRIV];
+__global__ __launch_bounds__(G::THREADS) void k_head_dw(const DwArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
   g_run<T8, G>(smem, DwJob<T8, G>(p));
 }
 
@@ -871,13 +879,13 @@ __global__ __launch_bounds__(G_THREADS) void k_head_dw(const DwArgs p) {
 // ---------------------------------------------------------------------------
 // Tiles of the products (m x n): vocabulary x tokens for z, channels x tokens
 // for dh, channels x vocabulary for dW.
-using ZL = GTile<256, 256, 2, 2, true, true>;
-using ZM = GTile<256, 64, 4, 4, true, true>;
-using ZS = GTile<256, 16, 8, 4, true, true>;
-using HL = GTile<256, 256, 2, 2, false, true>;
-using HM = GTile<256, 64, 4, 4, false, true>;
-using HS = GTile<256, 16, 8, 4, false, true>;
-using WL = GTile<256, 256, 2, 2, false, false>;
+using ZL = GTile<256, 256, 2, 4, 2, true, true>;
+using ZM = GTile<256, 64, 4, 2, 4, true, true>;
+using ZS = GTile<256, 16, 8, 1, 4, true, true>;
+using HL = GTile<256, 256, 2, 4, 2, false, true>;
+using HM = GTile<256, 64, 4, 2, 4, false, true>;
+using HS = GTile<256, 16, 8, 1, 4, false, true>;
+using WL = GTile<256, 256, 2, 4, 2, false, false>;
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -977,9 +985,9 @@ static void launch_fwd(FwdArgs p, hipStream_t s) {
   p.nn = (int)cdiv(p.T, G::BN);
   const int64_t tiles = (int64_t)p.nm * p.nn;
   if constexpr (G::NS == 2)
-    k_head_fwd_p<T8, G, XENT><<<persistent(tiles), G_THREADS, 0, s>>>(p);
+    k_head_fwd_p<T8, G, XENT><<<persistent(tiles), G::THREADS, 0, s>>>(p);
   else
-    k_head_fwd<T8, G, XENT><<<(unsigned)tiles, G_THREADS, 0, s>>>(p);
+    k_head_fwd<T8, G, XENT><<<(unsigned)tiles, G::THREADS, 0, s>>>(p);
 }
 
 template <typename T8, bool XENT>
@@ -1027,9 +1035,9 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
     const int nm = (int)cdiv(nv, GZ::BM);
     const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, ldz};
     if constexpr (GZ::NS == 2)
-      k_head_dz_p<T8, GZ><<<persistent((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
+      k_head_dz_p<T8, GZ><<<persistent((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
     else
-      k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
+      k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
     CRBQ_LAUNCH_CHECK();
     k_dz_listed<T8, XENT><<<(unsigned)cdiv(XENT ? T : T * k, 256), 256, 0, s>>>(
         st, T, k, labels, w.ratio, v, nv, w.dz, ldz);
@@ -1040,14 +1048,14 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
                      v > 0};
       const int64_t tiles = (int64_t)mh * nt * q.ns;
       if constexpr (GH::NS == 2)
-        k_head_dh_p<T8, GH><<<persistent(tiles), G_THREADS, 0, s>>>(q);
+        k_head_dh_p<T8, GH><<<persistent(tiles), GH::THREADS, 0, s>>>(q);
       else
-        k_head_dh<T8, GH><<<(unsigned)tiles, G_THREADS, 0, s>>>(q);
+        k_head_dh<T8, GH><<<(unsigned)tiles, GH::THREADS, 0, s>>>(q);
       CRBQ_LAUNCH_CHECK();
     }
     if (dW) {
       const int mw = (int)cdiv(C, WL::BM), nw = (int)cdiv(nv, WL::BN);
-      k_head_dw<T8, WL><<<persistent((int64_t)mw * nw), G_THREADS, 0, s>>>(
+      k_head_dw<T8, WL><<<persistent((int64_t)mw * nw), WL::THREADS, 0, s>>>(
           DwArgs{h, w.dz, ldh, ldz, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
       CRBQ_LAUNCH_CHECK();
     }
