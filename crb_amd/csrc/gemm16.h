@@ -244,8 +244,6 @@ __device__ __forceinline__ void g_each(const F& f) {
   }
 }
 
-constexpr int G_PRIV = 32 * 1024;       // LDS beside the stages of g_run, in equal shares
-
 // The lane, for an epilogue: opaque, so that what an epilogue computes from it
 // is computed there and not kept in registers over the products.
 __device__ __forceinline__ int g_lane() {
@@ -315,96 +313,325 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
   g_sync_lds();
 }
 
-// A workgroup's share of a launch's tiles, one after the other without a
-// gap: tiles lin, lin + gridDim, ... of job.tiles.
-//   job.tile(lin, A, B, k_beg, nch)  a tile's operands, first k and stages (>= 1)
-//   job.side(lin, priv)              loads what the tile's epilogue needs into the
-//                                    wavefront's own share of G_PRIV (g_load_lds*)
-//   job.finish(lin, priv, acc)       the epilogue
-// Two stages in LDS.  While the MFMAs of one half stage run, the fragments of
-// the next half are read into the other register set.  One barrier a stage,
-// between its halves: there every wavefront has read all of the stage (so the
-// stage after the next may be loaded over it), and the loads of the next
-// stage, issued a whole stage before, have arrived (so its fragments may be
-// read): no MFMA waits for an LDS read that could only start behind a
-// barrier.  The next tile's first stages are loaded under this tile's last, so
-// its loads run under the epilogue too.
-template <typename T8, typename G, typename Job>
+// ---------------------------------------------------------------------------
+// 256 x 256 tiles, persistent workgroups of 8 wavefronts (2 along m, 4 along n).
+//
+// A stage (64 k of both operands, 64 KB; two in LDS) consists of 4 + 4 units of 64
+// rows, each 8 KB: 64 rows of 128 bytes (KC) or 64 k rows of 128 bytes (K-strided),
+// whole lines of memory either way, one 1 KB load of each wavefront.  The output of
+// wavefront (wr, wc) is interleaved so that a unit serves all wavefronts at one time:
+//   m = 64 (i >> 1) + 32 wr + 16 (i & 1) + 4 (lane >> 4) + r,   i = 0..7
+//   n = 128 (j >> 1) + 32 wc + 16 (j & 1) + (lane & 15),        j = 0..3
+// A stage runs in four quarters, quarter u on A's unit u (16 MFMAs) and on B's
+// fragments of the stage, which are held in registers.  Fragments are read
+// from LDS a quarter ahead (A) or a stage ahead (B: units 0 and 1 in quarter
+// 1, units 2 and 3 in quarter 3).  After each half stage, a barrier: the units
+// read in it are free, and the loads of the half before the last have
+// arrived.  So every half issues 4 loads of each wavefront, evenly spaced, and
+// each has between 2 and 3 halves (2048 to 3072 cycles of MFMAs) to arrive:
+//   first half of stage c:   A(c + 2) unit 0, A(c + 1) unit 3, B(c + 2) units 2, 3
+//   second half:             A(c + 2) units 1, 2,              B(c + 3) units 0, 1
+// (With one barrier a stage and each stage loaded as a whole in the half
+// after it, the MFMAs were busy 64 % of the time, the loads being waited
+// for; issued earlier within that half they stood in each other's way.)
+// The stages of consecutive tiles follow on each other without a gap, so a tile's
+// first loads run under the last stages and the epilogue of the one before.
+// ---------------------------------------------------------------------------
+constexpr int G_UNIT = 8192, G_STAGE = 8 * G_UNIT, G_RING = 2 * G_STAGE;
+constexpr int G_THREADS = 512;
+constexpr int G_PRIV = 4096;            // LDS of each wavefront beside the stages
+constexpr int G_LDS = G_RING + 8 * G_PRIV;
+struct GAcc {
+  f4_t v[8][4];
+};
+__device__ __forceinline__ int g_m(int i, int wave, int lane) {
+  return 64 * (i >> 1) + 32 * (wave >> 2) + 16 * (i & 1) + 4 * (lane >> 4);
+}
+__device__ __forceinline__ int g_n(int j, int wave, int lane) {
+  return 128 * (j >> 1) + 32 * (wave & 3) + 16 * (j & 1) + (lane & 15);
+}
+
+// bits 1 and 3 of a K-strided unit's k row permute its 32-byte groups
+__device__ __forceinline__ int g_grp(int t) { return ((t >> 1) & 1) | ((t >> 2) & 2); }
+
+template <bool KC>
+struct GUnits {
+  unsigned voff;           // this lane's offset in a unit's load
+  int kc8, row;            // KC: its first k; K-strided: its k row
+  int f0, f1;              // fragment addresses (KC: of half 0, 1 of k; K-strided: of 16 rows 0, 1)
+  // w: this wavefront's 32-row block in a unit
+  __device__ GUnits(int64_t ld, int wave, int lane, int w) {
+    const int r = 8 * wave + (lane >> 3), c = lane & 7, r16 = lane & 15, gq = lane >> 4;
+    if (KC) {
+      kc8 = (c ^ (r & 7)) * 8;
+      voff = (unsigned)((r * ld + kc8) * 2);
+      f0 = (32 * w + r16) * 128 + ((gq ^ (r16 & 7)) << 4);
+      f1 = f0 ^ 64;
+    } else {
+      kc8 = 0;
+      voff = (unsigned)((r * ld + ((((c >> 1) ^ g_grp(r)) << 1) | (c & 1)) * 8) * 2);
+      const int t = 8 * gq + (r16 >> 2);
+      f0 = t * 128 + (((2 * w) ^ g_grp(t)) << 5) + (r16 & 3) * 8;
+      f1 = f0 ^ 32;
+    }
+    row = r;
+  }
+  // fragment of half h of k, 16 rows e (0, 1) of the wavefront's block, from the unit at `at`
+  template <typename T8>
+  __device__ T8 frag(const char* smem, int at, int h, int e) const {
+    if constexpr (KC) return *(const T8*)(smem + at + (h ? f1 : f0) + e * 16 * 128);
+    else return g_tr_frag<T8, 128>(smem + at + (e ? f1 : f0) + h * 32 * 128);
+  }
+};
+
+// A value the compiler takes for unknown from here on: what depends on it is
+// not computed earlier and kept (scalar registers are as short as vector
+// registers during the products).
+template <typename T>
+__device__ __forceinline__ T g_fresh(T v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+// The kernel's only argument, a struct Args, read where it is needed.
+template <typename Args>
+__device__ __forceinline__ Args g_args() {
+  typedef __attribute__((address_space(4))) const uint32_t cword;
+  static_assert(sizeof(Args) % 4 == 0, "whole words");
+  struct Words {
+    uint32_t w[sizeof(Args) / 4];
+  } a;
+  cword* q = (cword*)g_fresh(__builtin_amdgcn_kernarg_segment_ptr());
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(Args) / 4; ++i) a.w[i] = q[i];
+  return __builtin_bit_cast(Args, a);
+}
+
+__device__ __forceinline__ int g_uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename T>
+__device__ __forceinline__ T* g_uni(T* q) {
+  const uint64_t v = (uint64_t)q;
+  return (T*)((uint64_t)(uint32_t)g_uni((int)(uint32_t)v) |
+              (uint64_t)(uint32_t)g_uni((int)(v >> 32)) << 32);
+}
+
+// Where the loads of one operand stand within a tile.
+template <bool KC>
+struct GCursor {
+  const uint16_t* p;       // the stage's first element
+  int rows, k;             // rows (at most 256) and k's left from there; k <= 0: none
+  __device__ void open(const GOperand& o, int64_t k0) {
+    const int64_t kl = o.K - k0;
+    p = g_uni(o.p + (KC ? k0 : k0 * o.ld));
+    rows = g_uni((int)(o.rows < 256 ? o.rows : 256));
+    k = g_uni((int)(kl < (1 << 30) ? kl : (1 << 30)));
+  }
+  __device__ void advance(int64_t ld) {
+    p += KC ? (int64_t)G_K : G_K * ld;
+    k -= G_K;
+  }
+  // descriptor of the whole stage (rows < 256 x 2^22 elements: below 2^31 bytes)
+  __device__ i4_t rsrc(int ld) const {
+    int n;
+    if (KC) n = (rows - 1) * ld + (k < G_K ? k : G_K);
+    else n = ((k < G_K ? k : G_K) - 1) * ld + rows;
+    return g_rsrc(p, k > 0 ? n * 2 : 0);
+  }
+};
+
+// (an instruction's offset counts for its LDS address too)
+template <int U>
+__device__ __forceinline__ void g_load_unit(const void* dst, i4_t rs, unsigned voff) {
+  const unsigned d = __builtin_amdgcn_readfirstlane(
+      (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)dst) - U * 128;
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen offset:%2 lds" ::"v"(voff), "s"(rs),
+               "n"(U * 128), "{m0}"(d));
+}
+
+template <typename T8, bool AKC, bool BKC, typename Job>
 __device__ __forceinline__ void g_run(char* smem, const Job& job) {
-  static_assert(G::NS == 2 && G::NJ <= G::MI, "two stages");
-  const GLane<T8, G> L(job.lda, job.ldb);
-  char* priv = smem + G::LDS + L.wave * (G_PRIV / G::NW);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lda = g_uni((int)job.lda()), ldb = g_uni((int)job.ldb());
+  const int tiles = g_uni(job.tiles());
+  const GUnits<AKC> UA(lda, wave, lane, wave >> 2);
+  const GUnits<BKC> UB(ldb, wave, lane, wave & 1);
+  const int bw = ((wave >> 1) & 1) * G_UNIT;           // n: 32 wc = 64 (wc >> 1) + 32 (wc & 1)
+  char* priv = smem + G_RING + wave * G_PRIV;
+  char* mine = smem + wave * 1024;                     // this wavefront's kilobyte of a unit
   const int nwg = gridDim.x, first = g_xcd(blockIdx.x, nwg);
-  // the stage to be loaded next: c of tile ll
-  int ll = first, lc = 0, ln = 0;
-  int64_t lk = 0;
-  GOperand A, B;
-  auto open = [&]() {
-    if (ll < job.tiles) job.tile(ll, A, B, lk, ln);
+  if (first >= tiles) return;                          // no tile at all
+
+  // The stages in load order: stage lc of a tile of ln; then the next tile, whose
+  // operands are at hand.  A tile has at least 4 stages (the last ones
+  // empty if need be), so that it is enough to look at one tile ahead, at
+  // the end of each.
+  GCursor<AKC> ca, na;
+  GCursor<BKC> cb, nb;
+  const uint64_t *cl = nullptr, *nl = nullptr;
+  int lc = 0, ln = 0, nn = 0;
+  auto peek = [&](int lin) __attribute__((always_inline)) {      // the next tile: na, nb, nl, nn
+    GOperand A, B;
+    int64_t k;
+    na.k = nb.k = 0;
+    nn = 1 << 30;
+    nl = nullptr;
+    na.rows = nb.rows = 1;
+    na.p = nb.p = nullptr;
+    if (lin < tiles) {
+      job.tile(lin, A, B, k, nn);
+      nn = g_uni(nn < 4 ? 4 : nn);
+      na.open(A, k);
+      nb.open(B, k);
+      if (!AKC && A.live) nl = A.live + k / G_K;
+    }
   };
-  auto source = [&]() {
-    const auto s = L.source(A, B, lk + (int64_t)lc * G_K, ll < job.tiles);
+  struct Stage {
+    i4_t ra, rb;
+    int k;                 // KC operands: k's left
+    uint64_t live;
+  };
+  auto next = [&]() __attribute__((always_inline)) {
+    Stage s{ca.rsrc(lda), cb.rsrc(ldb), BKC ? cb.k : ca.k, ~0ull};
+    if (!AKC && cl) s.live = ca.k > 0 ? cl[lc] : 0;
+    ca.advance(lda);
+    cb.advance(ldb);
     if (++lc == ln) {
+      ca = na;
+      cb = nb;
+      cl = nl;
+      ln = nn;
       lc = 0;
-      ll += nwg;
-      open();
     }
     return s;
   };
-  open();
-  if (ll >= job.tiles) return;                         // no tile at all
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const auto s = source();
-#pragma unroll
-    for (int q = 0; q < G::LW; ++q) L.load(smem + c * G::STAGE, q, s);
+  constexpr unsigned OUT = 0x80000000u;
+  auto loadA = [&](auto uu, const Stage& s, int buf) __attribute__((always_inline)) {
+    constexpr int u = decltype(uu)::value;
+    char* d = mine + buf * G_STAGE + u * G_UNIT;
+    if constexpr (AKC)
+      g_load_unit<0>(d, s.ra, (UA.kc8 < s.k ? UA.voff : OUT) + (unsigned)(u * 128 * lda));
+    else
+      g_load_unit<u>(d, s.ra, Job::MASKED && !((s.live >> UA.row) & 1) ? OUT : UA.voff);
+  };
+  auto loadB = [&](auto uu, const Stage& s, int buf) __attribute__((always_inline)) {
+    constexpr int u = decltype(uu)::value;
+    char* d = mine + buf * G_STAGE + (4 + u) * G_UNIT;
+    if constexpr (BKC)
+      g_load_unit<0>(d, s.rb, (UB.kc8 < s.k ? UB.voff : OUT) + (unsigned)(u * 128 * ldb));
+    else
+      g_load_unit<u>(d, s.rb, UB.voff);
+  };
+  // A fragment (h, e) of unit u; B fragment (h, j)
+  auto fragA = [&](int buf, int u, int h, int e) __attribute__((always_inline)) -> T8 {
+    return UA.template frag<T8>(smem, buf * G_STAGE + u * G_UNIT, h, e);
+  };
+  auto fragB = [&](int buf, int h, int j) __attribute__((always_inline)) -> T8 {
+    return UB.template frag<T8>(smem, buf * G_STAGE + (4 + 2 * (j >> 1)) * G_UNIT + bw, h, j & 1);
+  };
+  constexpr std::integral_constant<int, 0> _0{};
+  constexpr std::integral_constant<int, 1> _1{};
+  constexpr std::integral_constant<int, 2> _2{};
+  constexpr std::integral_constant<int, 3> _3{};
+
+  peek(first);
+  ca = na;
+  cb = nb;
+  cl = nl;
+  ln = nn;
+  int nch = nn;                                        // stages of the tile at work
+  peek(first + nwg);
+  // stage 0, what stage 1 needs early, then B's units 0 and 1 of stage 2 over stage 0's
+  Stage s1, s2;
+  {
+    const Stage s0 = next();
+    s1 = next();
+    s2 = next();
+    g_each<4>([&](auto uu) __attribute__((always_inline)) {
+      loadA(uu, s0, 0);
+      loadB(uu, s0, 0);
+      loadB(uu, s1, 1);
+      if constexpr (decltype(uu)::value < 3) loadA(uu, s1, 1);
+    });
   }
-  g_wait_vm<G::LW>();
+  g_wait_vm<0>();
   g_sync_lds();
+  T8 a0[4], a1[4], b0[8], b1[8];                       // [2 h + e], [4 h + j]
+#pragma unroll
+  for (int q = 0; q < 8; ++q) b0[q] = fragB(0, q >> 2, q & 3);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) a0[q] = fragA(0, 0, q >> 1, q & 1);
+  g_sync_lds();
+  loadB(_0, s2, 0);
+  loadB(_1, s2, 0);
+
+  GAcc acc;
+  // quarter u: 16 MFMAs on a; side(q) between them
+  auto quarter = [&](auto uu, const T8(&a)[4], const T8(&b)[8], auto&& side)
+      __attribute__((always_inline)) {
+    constexpr int u = decltype(uu)::value;
+    g_each<4>([&](auto qq) __attribute__((always_inline)) {
+      constexpr int q = decltype(qq)::value, h = q >> 1, i = 2 * u + (q & 1);
+      side(q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc.v[i][j] = g_mfma<T8>(a[q], b[4 * h + j], acc.v[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // a stage from buffer p; s1, s2: stages c + 1, c + 2
+  auto stage = [&](int p, T8(&b)[8], T8(&bn)[8]) __attribute__((always_inline)) {
+    const int o = p ^ 1;
+    quarter(_0, a0, b, [&](int q) __attribute__((always_inline)) {
+      a1[q] = fragA(p, 1, q >> 1, q & 1);
+      if (q == 0) loadA(_3, s1, o);
+      if (q == 2) loadA(_0, s2, p);
+    });
+    const Stage s3 = next();
+    quarter(_1, a1, b, [&](int q) __attribute__((always_inline)) {
+      a0[q] = fragA(p, 2, q >> 1, q & 1);
+      bn[4 * (q >> 1) + (q & 1)] = fragB(o, q >> 1, q & 1);
+      if (q == 0) loadB(_2, s2, p);
+      if (q == 2) loadB(_3, s2, p);
+    });
+    g_wait_vm<8>();
+    g_sync_lds();
+    quarter(_2, a0, b, [&](int q) __attribute__((always_inline)) {
+      a1[q] = fragA(p, 3, q >> 1, q & 1);
+      if (q == 0) loadA(_1, s2, p);
+      if (q == 2) loadA(_2, s2, p);
+    });
+    quarter(_3, a1, b, [&](int q) __attribute__((always_inline)) {
+      a0[q] = fragA(o, 0, q >> 1, q & 1);
+      bn[4 * (q >> 1) + 2 + (q & 1)] = fragB(o, q >> 1, 2 + (q & 1));
+      if (q == 0) loadB(_0, s3, o);
+      if (q == 2) loadB(_1, s3, o);
+    });
+    g_wait_vm<8>();
+    g_sync_lds();
+    s1 = s2;
+    s2 = s3;
+  };
   int par = 0;                                         // the stage's buffer
-  for (int lin = first; lin < job.tiles; lin += nwg) {
-    // read again behind an epilogue, which needs the registers
-    T8 a0[G::MI], b0[G::NJ], a1[G::MI], b1[G::NJ];
+  for (int lin = first; lin < tiles; lin += nwg) {
 #pragma unroll
-    for (int j = 0; j < G::NJ; ++j) b0[j] = L.fragB(smem, par * G::STAGE, 0, j);
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i) a0[i] = L.fragA(smem, par * G::STAGE, 0, i);
-    f4_t acc[G::MI][G::NJ];
-    g_zero<G>(acc);
-    int nch;
-    {
-      GOperand ta, tb;
-      int64_t tk;
-      job.tile(lin, ta, tb, tk, nch);
-    }
+      for (int j = 0; j < 4; ++j) acc.v[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
     job.side(lin, priv);
-    for (int c = 0; c < nch; ++c) {
-      const int at = par * G::STAGE, nx = G::STAGE - at;
-      const auto s = source();
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i) {
-        if (i < G::NJ) b1[i] = L.fragB(smem, at, 1, i);
-        a1[i] = L.fragA(smem, at, 1, i);
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a0[i], b0[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      g_wait_vm<0>();
-      g_sync_lds();
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i) {
-        if (i < G::NJ) b0[i] = L.fragB(smem, nx, 0, i);
-        a0[i] = L.fragA(smem, nx, 0, i);
-#pragma unroll
-        for (int q = 0; q < G::LW; ++q)
-          if (q * G::MI / G::LW == i) L.load(smem + at, q, s);
-#pragma unroll
-        for (int j = 0; j < G::NJ; ++j) acc[i][j] = g_mfma<T8>(a1[i], b1[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      par ^= 1;
+    int c = 0;
+    for (; c + 2 <= nch; c += 2) {
+      stage(par, b0, b1);
+      stage(par ^ 1, b1, b0);
     }
+    if (c < nch) {
+      stage(par, b0, b1);
+      par ^= 1;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) b0[q] = b1[q];
+    }
+    nch = ln;                                          // the cursor is in the next tile
     job.finish(lin, priv, acc);
+    peek(lin + 2 * nwg);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // priv is free for the next side()
   }
   g_wait_vm<0>();
@@ -420,21 +647,23 @@ __device__ __forceinline__ void g_load_lds_words(const void* dst, const void* p,
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(rs), "{m0}"(d));
 }
 
-// 16 rows (n) of a tile's 16-bit output, MI * 16 elements each, through the wavefront's
-// own LDS: in as each lane's 4 consecutive elements of one row, out as
-// 16-byte stores of whole rows.  put(row, m, 8 elements) stores.
-template <typename G, typename F>
-__device__ __forceinline__ void g_rows_out(char* priv, const uint2 (&v)[G::MI], F&& put) {
-  static_assert(G::MI == 8, "rows of 256 bytes");
+// 16 rows (n) of a wavefront's 16-bit output of a 256 x 256 tile (128 elements each, m
+// as above) through its own LDS: in as each lane's 4 consecutive
+// elements of one row, out as 16-byte stores, 64 bytes of a row side by
+// side.  put(row, m, 8 elements) stores.
+template <typename F>
+__device__ __forceinline__ void g_rows_out(char* priv, const uint2 (&v)[8], F&& put) {
   const int lane = g_lane(), n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
-  for (int i = 0; i < G::MI; ++i)
+  for (int i = 0; i < 8; ++i)
     *(uint2*)(priv + n * 256 + (((2 * i + (g >> 1)) ^ n) << 4) + (g & 1) * 8) = v[i];
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int r = 4 * q + g;
-    put(r, n * 8, *(const uint4*)(priv + r * 256 + ((n ^ r) << 4)));
+    put(r, 64 * (n >> 2) + 32 * (wave >> 2) + 8 * (n & 3),
+        *(const uint4*)(priv + r * 256 + ((n ^ r) << 4)));
   }
   asm volatile("" ::: "memory");
 }

@@ -110,17 +110,18 @@ __device__ __forceinline__ int64_t list_slot(const Listed& ls, int64_t t, int v)
   return t * ls.k + lo;
 }
 
-// Column t (n) of a wavefront's tile: listed tokens and what lies behind
-// the vocabulary become -inf (the listed ones' z is written), then the
-// maximum and the sum of exponentials over its MI * 16 tokens from vw on.
+// Column t (n) of a wavefront's tile, MI times 16 tokens, the i-th 16 of them
+// from v0 + off(i) on: listed tokens and what lies behind the vocabulary
+// become -inf (the listed ones' z is written), then the maximum and the sum
+// of exponentials.  lab: the label's place behind v0; words: each i's 16 mask bits.
 // In units of log 2: exp z = 2^(acc * scale2), so an exponential is one
 // multiply-add and one v_exp; the listed tokens and the end are looked for
 // only where a wavefront has any.  Bound by the v_exp (16 cycles a wavefront)
 // and the 2 to 3 vector operations beside each.
-template <typename G, bool XENT, int j>
-__device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t vw, int lab,
-                                           const uint32_t (&words)[G::WM / 32],
-                                           f4_t (&acc)[G::MI][G::NJ], float2* out) {
+template <int MI, int NJ, bool XENT, int j, typename Off>
+__device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t v0, Off off,
+                                           int lab, const uint32_t (&words)[(MI + 1) / 2],
+                                           f4_t (&acc)[MI][NJ], float2* out) {
   const int lane = g_lane(), g4 = (lane >> 4) * 4;
   const bool ok = t < p.T;
   bool any;
@@ -129,44 +130,44 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   } else {
     uint32_t w = 0;
 #pragma unroll
-    for (int q = 0; q < G::WM / 32; ++q) w |= words[q];
+    for (int q = 0; q < (MI + 1) / 2; ++q) w |= words[q];
     any = w != 0;
   }
   const float fin = p.scale < 0.f ? INFINITY : -INFINITY;        // scale * fin = -inf
   if (__any(any)) {
-    g_each<G::MI>([&](auto ii) __attribute__((always_inline)) {
+    g_each<MI>([&](auto ii) __attribute__((always_inline)) {
       constexpr int i = decltype(ii)::value;
-      const uint32_t nib = XENT ? (uint32_t)(lab >> 2 == 4 * i + (lane >> 4))
+      const int o = off(i) + g4;
+      const uint32_t nib = XENT ? (uint32_t)(lab >> 2 == o >> 2)
                                 : (words[i / 2] >> (16 * (i & 1) + g4)) & 15u;
       if (nib)
         g_each<4>([&](auto rr) __attribute__((always_inline)) {
           constexpr int r = decltype(rr)::value;
-          const int o = 16 * i + g4 + r;
-          if (XENT ? o == lab : (nib >> r) & 1u) {
-            p.zt[XENT ? t : list_slot(p.ls, t, (int)(vw + o))] = acc[i][j][r] * p.scale;
+          if (XENT ? o + r == lab : (nib >> r) & 1u) {
+            p.zt[XENT ? t : list_slot(p.ls, t, (int)(v0 + o + r))] = acc[i][j][r] * p.scale;
             acc[i][j][r] = fin;
           }
         });
     });
   }
-  if (vw + G::WM > p.V) {
-    const int end = p.V > vw ? (int)(p.V - vw) : 0;
+  if (v0 + off(MI - 1) + 16 > p.V) {
+    const int end = (int)(p.V - v0);
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (16 * i + g4 + r >= end) acc[i][j][r] = fin;
+        if (off(i) + g4 + r >= end) acc[i][j][r] = fin;
   }
   const float scale2 = p.scale * LOG2E;
   float m = fin;
   if (p.scale < 0.f) {
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fminf(m, acc[i][j][r]);
   } else {
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
   }
@@ -174,7 +175,7 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   const float mb = m == -INFINITY ? 0.f : m;           // nothing left: 2^-inf = 0
   float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < G::MI; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       s[r & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], scale2, -mb));
@@ -210,91 +211,93 @@ __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
 #pragma unroll
       for (int w = 0; w < G::WM / 32; ++w) words[w] = p.ls.mask[t * p.ls.ldm + (vw >> 5) + w];
     }
-    fwd_column<G, XENT, j>(p, t, vw, lab, words, acc,
-                           p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
+    fwd_column<G::MI, G::NJ, XENT, j>(p, t, vw, [](int i) { return 16 * i; }, lab, words, acc,
+                                      p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
   });
 }
 
-// many tokens: a persistent workgroup on each CU
-template <typename G, bool XENT>
-struct FwdJob : FwdArgs {
-  int64_t lda, ldb;
-  int tiles;
-  __device__ explicit FwdJob(const FwdArgs& a) : FwdArgs(a), lda(a.ldw), ldb(a.ldh) {
-    tiles = a.nm * a.nn;
+// many tokens: persistent workgroups
+template <bool XENT>
+struct FwdJob {
+  static constexpr bool MASKED = false;
+  __device__ static int64_t lda() { return g_args<FwdArgs>().ldw; }
+  __device__ static int64_t ldb() { return g_args<FwdArgs>().ldh; }
+  __device__ static int tiles() {
+    const FwdArgs p = g_args<FwdArgs>();
+    return p.nm * p.nn;
   }
-  __device__ __forceinline__ void place(int lin, int64_t& v0, int64_t& t0, int& tm) const {
+  __device__ __forceinline__ static void place(const FwdArgs& p, int lin, int64_t& v0, int64_t& t0, int& tm) {
     int tn;
-    g_band(lin, nm, nn, tm, tn);
-    v0 = (int64_t)tm * G::BM;
-    t0 = (int64_t)tn * G::BN;
+    g_band(lin, p.nm, p.nn, tm, tn);
+    v0 = (int64_t)tm * 256;
+    t0 = (int64_t)tn * 256;
   }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
+    const FwdArgs p = g_args<FwdArgs>();
     int64_t v0, t0;
     int tm;
-    place(lin, v0, t0, tm);
-    A = GOperand{W + v0 * ldw, ldw, V - v0, C, nullptr};
-    B = GOperand{h + t0 * ldh, ldh, T - t0, C, nullptr};
+    place(p, lin, v0, t0, tm);
+    A = GOperand{p.W + v0 * p.ldw, p.ldw, p.V - v0, p.C, nullptr};
+    B = GOperand{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
     k = 0;
-    nch = (int)((C + G_K - 1) / G_K);
+    nch = (int)((p.C + G_K - 1) / G_K);
   }
-  // the labels (or the mask words) of the wavefront's 64 rows
+  // the labels (or the tile's 8 mask words) of the wavefront's 2 x 32 rows
   __device__ __forceinline__ void side(int lin, char* priv) const {
+    const FwdArgs p = g_args<FwdArgs>();
     int64_t v0, t0;
     int tm;
-    place(lin, v0, t0, tm);
+    place(p, lin, v0, t0, tm);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t t = t0 + (wave % G::WGN) * G::WN, left = T - t;
-    if (XENT) {
-      const char* y = (const char*)(ls.labels + t);
 #pragma unroll
-      for (int b = 0; b < G::WN * 8; b += 256)
-        g_load_lds_words(priv + b, y + b, left * 8 - b, lane);
-    } else {
-      const int64_t vw = v0 + (wave / G::WGN) * G::WM;
-      const int64_t rows = left < G::WN ? left : G::WN;
-#pragma unroll
-      for (int b = 0; b < G::WN; b += 64)
-        g_load_lds(priv + b * 16,
-                   g_rsrc((const uint16_t*)(ls.mask + t * ls.ldm + (vw >> 5)),
-                          rows > 0 ? (rows - 1) * ls.ldm * 4 + 16 : 0),
-                   (unsigned)((b + lane) * ls.ldm * 4));
+    for (int b = 0; b < 2; ++b) {
+      const int64_t t = t0 + 128 * b + 32 * (wave & 3), left = p.T - t;
+      if (XENT) {
+        g_load_lds_words(priv + 256 * b, p.ls.labels + t, left * 8, lane);
+      } else {
+        const int64_t rows = left < 32 ? left : 32;
+        g_load_lds(priv + 1024 * b,
+                   g_rsrc((const uint16_t*)(p.ls.mask + t * p.ls.ldm + (v0 >> 5)),
+                          rows > 0 ? ((rows - 1) * p.ls.ldm + 8) * 4 : 0),
+                   (unsigned)((lane >> 1) * p.ls.ldm * 4 + (lane & 1) * 16));
+      }
     }
   }
-  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
-    static_assert(G::WN % 64 == 0 && G::WM == 128, "side() holds rows of 128 tokens");
+  __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
+    const FwdArgs p = g_args<FwdArgs>();
     int64_t v0, t0;
     int tm;
-    place(lin, v0, t0, tm);
+    place(p, lin, v0, t0, tm);
     const int lane = g_lane();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wr = wave / G::WGN;
-    const int64_t vw = v0 + wr * G::WM;
-    g_each<G::NJ>([&](auto jj) __attribute__((always_inline)) {
+    const int wr = wave >> 2;
+    g_each<4>([&](auto jj) __attribute__((always_inline)) {
       constexpr int j = decltype(jj)::value;
-      const int n = 16 * j + (lane & 15);
-      const int64_t t = t0 + (wave % G::WGN) * G::WN + n;
+      const int64_t t = t0 + g_n(j, wave, lane);
+      const int row = 16 * (j & 1) + (lane & 15);      // of 32
       int lab = -1;
-      uint32_t words[G::WM / 32] = {};
+      uint32_t words[4] = {};
       if (XENT) {
-        const int64_t y = ((const int64_t*)priv)[n];
-        lab = t < T && y >= vw && y < vw + G::WM ? (int)(y - vw) : -1;
+        const int64_t y = ((const int64_t*)(priv + 256 * (j >> 1)))[row];
+        lab = t < p.T && y >= v0 && y < v0 + 256 ? (int)(y - v0) : -1;
       } else {
-        const uint4 w = ((const uint4*)priv)[n];
-        words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
+        const uint32_t* w = (const uint32_t*)(priv + 1024 * (j >> 1)) + row * 8 + wr;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) words[q] = w[2 * q];
       }
-      fwd_column<G, XENT, j>(*this, t, vw, lab, words, acc,
-                             part + t * npart + (int64_t)tm * G::WGM + wr);
+      fwd_column<8, 4, XENT, j>(
+          p, t, v0, [&](int i) { return 64 * (i >> 1) + 32 * wr + 16 * (i & 1); }, lab, words,
+          acc.v, p.part + t * p.npart + (int64_t)tm * 2 + wr);
     });
   }
 };
 
-template <typename T8, typename G, bool XENT>
-__global__ __launch_bounds__(G::THREADS) void k_head_fwd_p(const FwdArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
-  g_run<T8, G>(smem, FwdJob<G, XENT>(p));
+template <typename T8, bool XENT>
+__global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs) {
+  __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
+  g_run<T8, true, true>(smem, FwdJob<XENT>());
 }
 
 // The saved state of a forward, in floats: a [T], lse [T], one factor (1 or
@@ -614,74 +617,79 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
   }
 }
 
-template <typename T8, typename G>
-struct DzJob : DzArgs {
-  int64_t lda, ldb;
-  int tiles;
-  __device__ explicit DzJob(const DzArgs& a) : DzArgs(a), lda(a.ldw), ldb(a.ldh) {
-    tiles = a.nm * a.nn;
+template <typename T8>
+struct DzJob {
+  static constexpr bool MASKED = false;
+  __device__ static int64_t lda() { return g_args<DzArgs>().ldw; }
+  __device__ static int64_t ldb() { return g_args<DzArgs>().ldh; }
+  __device__ static int tiles() {
+    const DzArgs p = g_args<DzArgs>();
+    return p.nm * p.nn;
   }
-  __device__ __forceinline__ void place(int lin, int64_t& v0, int64_t& t0) const {
+  __device__ __forceinline__ static void place(const DzArgs& p, int lin, int64_t& v0, int64_t& t0) {
     int tm, tn;
-    g_band(lin, nm, nn, tm, tn);
-    v0 = (int64_t)tm * G::BM;
-    t0 = (int64_t)tn * G::BN;
+    g_band(lin, p.nm, p.nn, tm, tn);
+    v0 = (int64_t)tm * 256;
+    t0 = (int64_t)tn * 256;
   }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
+    const DzArgs p = g_args<DzArgs>();
     int64_t v0, t0;
-    place(lin, v0, t0);
-    A = GOperand{W + v0 * ldw, ldw, nv - v0, C, nullptr};
-    B = GOperand{h + t0 * ldh, ldh, T - t0, C, nullptr};
+    place(p, lin, v0, t0);
+    A = GOperand{p.W + v0 * p.ldw, p.ldw, p.nv - v0, p.C, nullptr};
+    B = GOperand{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
     k = 0;
-    nch = (int)((C + G_K - 1) / G_K);
+    nch = (int)((p.C + G_K - 1) / G_K);
   }
+  // a2 and rowb of the wavefront's 2 x 32 rows (64 words are loaded for each 32)
   __device__ __forceinline__ void side(int lin, char* priv) const {
+    const DzArgs p = g_args<DzArgs>();
     int64_t v0, t0;
-    place(lin, v0, t0);
+    place(p, lin, v0, t0);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t t = t0 + (wave % G::WGN) * G::WN, left = (T - t) * 4;
 #pragma unroll
-    for (int b = 0; b < G::WN * 4; b += 256) {
-      g_load_lds_words(priv + b, (const char*)(a2 + t) + b, left - b, lane);
-      g_load_lds_words(priv + G::WN * 4 + b, (const char*)(rowb + t) + b, left - b, lane);
+    for (int b = 0; b < 2; ++b) {
+      const int64_t t = t0 + 128 * b + 32 * (wave & 3), left = (p.T - t) * 4;
+      g_load_lds_words(priv + 512 * b, p.a2 + t, left, lane);
+      g_load_lds_words(priv + 512 * b + 256, p.rowb + t, left, lane);
     }
   }
-  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
-    static_assert(G::WN % 64 == 0 && G::WM == 128, "side() holds whole words");
+  __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
+    const DzArgs p = g_args<DzArgs>();
     int64_t v0, t0;
-    place(lin, v0, t0);
-    const int lane = g_lane(), n16 = lane & 15;
+    place(p, lin, v0, t0);
+    const int lane = g_lane();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t vw = v0 + (wave / G::WGN) * G::WM, tw = t0 + (wave % G::WGN) * G::WN;
-    const float scale2 = scale * LOG2E;
-    float at[G::NJ], b[G::NJ];
+    const float scale2 = p.scale * LOG2E;
+    float at[4], b[4];
 #pragma unroll
-    for (int j = 0; j < G::NJ; ++j) {
-      at[j] = ((const float*)priv)[16 * j + n16];
-      b[j] = ((const float*)priv)[G::WN + 16 * j + n16];
+    for (int j = 0; j < 4; ++j) {
+      const float* q = (const float*)(priv + 512 * (j >> 1)) + 16 * (j & 1) + (lane & 15);
+      at[j] = q[0];
+      b[j] = q[64];
     }
-    const bool whole = vw + G::WM <= nv;
+    const bool whole = v0 + 256 <= p.nv;
+    g_each<4>([&](auto jj) __attribute__((always_inline)) {
+      constexpr int j = decltype(jj)::value;
+      uint2 u[8];
 #pragma unroll
-    for (int j = 0; j < G::NJ; ++j) {
-      uint2 u[G::MI];
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i)
-        u[i] = dz_pack<T8>(acc[i][j], scale2, at[j], b[j],
-                           whole ? 4 : nv - (vw + 16 * i + 4 * (lane >> 4)));
-      g_rows_out<G>(priv, u, [&](int r, int m, const uint4& x) {
-        const int64_t t = tw + 16 * j + r;
-        if (t < T) *(uint4*)(dz + t * ldz + vw + m) = x;         // vw + 128 <= ldz
+      for (int i = 0; i < 8; ++i)
+        u[i] = dz_pack<T8>(acc.v[i][j], scale2, at[j], b[j],
+                           whole ? 4 : p.nv - (v0 + g_m(i, wave, lane)));
+      g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
+        const int64_t t = t0 + g_n(j, wave, 0) + r;
+        if (t < p.T) *(uint4*)(p.dz + t * p.ldz + v0 + m) = x;         // v0 + 256 <= ldz
       });
-    }
+    });
   }
 };
 
-template <typename T8, typename G>
-__global__ __launch_bounds__(G::THREADS) void k_head_dz_p(const DzArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
-  g_run<T8, G>(smem, DzJob<T8, G>(p));
+template <typename T8>
+__global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs) {
+  __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
+  g_run<T8, true, true>(smem, DzJob<T8>());
 }
 
 // the listed tokens' dz within [vbeg, vbeg + nv)
@@ -712,29 +720,17 @@ struct DhArgs {
   int add;
 };
 
-template <typename G>
-__device__ __forceinline__ void dh_finish(const DhArgs& p, int64_t c0, int64_t t0, int split,
-                                          const f4_t (&acc)[G::MI][G::NJ]) {
-  const int lane = g_lane();
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  float* P = p.P + (int64_t)split * p.T * p.C;
-#pragma unroll
-  for (int j = 0; j < G::NJ; ++j) {
-    const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
-    if (t >= p.T) continue;
-#pragma unroll
-    for (int i = 0; i < G::MI; ++i) {
-      const int64_t c = c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4);
-      if (c >= p.C) continue;
-      float4* q = (float4*)(P + t * p.C + c);
-      float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-      if (p.add) {
-        const float4 u = *q;
-        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-      }
-      *q = v;
-    }
+// 4 channels c.. of row t
+__device__ __forceinline__ void dh_add(const DhArgs& p, int split, int64_t t, int64_t c,
+                                       const f4_t& a) {
+  if (t >= p.T || c >= p.C) return;
+  float4* q = (float4*)(p.P + ((int64_t)split * p.T + t) * p.C + c);
+  float4 v = make_float4(a[0], a[1], a[2], a[3]);
+  if (p.add) {
+    const float4 u = *q;
+    v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
   }
+  *q = v;
 }
 
 template <typename T8, typename G>
@@ -749,47 +745,63 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
   const GOperand B{p.dz + t0 * p.ldz, p.ldz, p.T - t0, p.ldz, nullptr};
   f4_t acc[G::MI][G::NJ];
   g_tile<T8, G>(smem, A, B, kb, ke, acc);
-  dh_finish<G>(p, c0, t0, split, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+      dh_add(p, split, t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15),
+             c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4), acc[i][j]);
 }
 
-template <typename G>
-struct DhJob : DhArgs {
-  int64_t lda, ldb;
-  int tiles;
-  __device__ explicit DhJob(const DhArgs& a) : DhArgs(a), lda(a.ldw), ldb(a.ldz) {
-    tiles = a.nm * a.nn * a.ns;
+struct DhJob {
+  static constexpr bool MASKED = false;
+  __device__ static int64_t lda() { return g_args<DhArgs>().ldw; }
+  __device__ static int64_t ldb() { return g_args<DhArgs>().ldz; }
+  __device__ static int tiles() {
+    const DhArgs p = g_args<DhArgs>();
+    return p.nm * p.nn * p.ns;
   }
-  __device__ __forceinline__ void place(int lin, int64_t& c0, int64_t& t0, int& split) const {
+  __device__ __forceinline__ static void place(const DhArgs& p, int lin, int64_t& c0, int64_t& t0, int& split) {
     int tm, tn;
-    split = lin / (nm * nn);
-    g_band(lin - split * nm * nn, nm, nn, tm, tn);
-    c0 = (int64_t)tm * G::BM;
-    t0 = (int64_t)tn * G::BN;
+    split = lin / (p.nm * p.nn);
+    g_band(lin - split * p.nm * p.nn, p.nm, p.nn, tm, tn);
+    c0 = (int64_t)tm * 256;
+    t0 = (int64_t)tn * 256;
   }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
+    const DhArgs p = g_args<DhArgs>();
     int64_t c0, t0;
     int split;
-    place(lin, c0, t0, split);
-    A = GOperand{W + c0, ldw, C - c0, nv, nullptr};
-    B = GOperand{dz + t0 * ldz, ldz, T - t0, ldz, nullptr};
-    k = split * span;
-    const int64_t n = nv - k < span ? nv - k : span;   // > 0 for every split of a launch
+    place(p, lin, c0, t0, split);
+    A = GOperand{p.W + c0, p.ldw, p.C - c0, p.nv, nullptr};
+    B = GOperand{p.dz + t0 * p.ldz, p.ldz, p.T - t0, p.ldz, nullptr};
+    k = split * p.span;
+    const int64_t n = p.nv - k < p.span ? p.nv - k : p.span;   // > 0 for every split of a launch
     nch = (int)((n + G_K - 1) / G_K);
   }
   __device__ __forceinline__ void side(int, char*) const {}
-  __device__ __forceinline__ void finish(int lin, char*, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void finish(int lin, char*, GAcc& acc) const {
+    const DhArgs p = g_args<DhArgs>();
     int64_t c0, t0;
     int split;
-    place(lin, c0, t0, split);
-    dh_finish<G>(*this, c0, t0, split, acc);
+    place(p, lin, c0, t0, split);
+    const int lane = g_lane();
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        dh_add(p, split, t0 + g_n(j, wave, lane), c0 + g_m(i, wave, lane), acc.v[i][j]);
   }
 };
 
-template <typename T8, typename G>
-__global__ __launch_bounds__(G::THREADS) void k_head_dh_p(const DhArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
-  g_run<T8, G>(smem, DhJob<G>(p));
+template <typename T8>
+__global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs) {
+  __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
+  g_run<T8, false, true>(smem, DhJob());
 }
 
 // dh = fac * (P[0] + P[1] + ...), rounded once; 4 channels a thread
@@ -823,55 +835,60 @@ struct DwArgs {
   int64_t ldo;
 };
 
-template <typename T8, typename G>
-struct DwJob : DwArgs {
-  int64_t lda, ldb;
-  int tiles;
-  float f;
-  __device__ explicit DwJob(const DwArgs& a) : DwArgs(a), lda(a.ldh), ldb(a.ldz), f(a.fac[0]) {
-    tiles = a.nm * a.nn;
+template <typename T8>
+struct DwJob {
+  static constexpr bool MASKED = true;
+  __device__ static int64_t lda() { return g_args<DwArgs>().ldh; }
+  __device__ static int64_t ldb() { return g_args<DwArgs>().ldz; }
+  __device__ static int tiles() {
+    const DwArgs p = g_args<DwArgs>();
+    return p.nm * p.nn;
   }
-  __device__ __forceinline__ void place(int lin, int64_t& c0, int64_t& v0) const {
+  __device__ __forceinline__ static void place(const DwArgs& p, int lin, int64_t& c0, int64_t& v0) {
     int tm, tn;
-    g_band(lin, nm, nn, tm, tn);
-    c0 = (int64_t)tm * G::BM;
-    v0 = (int64_t)tn * G::BN;
+    g_band(lin, p.nm, p.nn, tm, tn);
+    c0 = (int64_t)tm * 256;
+    v0 = (int64_t)tn * 256;
   }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
+    const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
-    place(lin, c0, v0);
-    A = GOperand{h + c0, ldh, C - c0, T, live};
-    B = GOperand{dz + v0, ldz, ldz - v0, T, nullptr};
+    place(p, lin, c0, v0);
+    A = GOperand{p.h + c0, p.ldh, p.C - c0, p.T, p.live};
+    B = GOperand{p.dz + v0, p.ldz, p.ldz - v0, p.T, nullptr};
     k = 0;
-    nch = (int)((T + G_K - 1) / G_K);
+    nch = (int)((p.T + G_K - 1) / G_K);
   }
   __device__ __forceinline__ void side(int, char*) const {}
-  __device__ __forceinline__ void finish(int lin, char* priv, f4_t (&acc)[G::MI][G::NJ]) const {
+  __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
+    const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
-    place(lin, c0, v0);
+    place(p, lin, c0, v0);
+    const float f = p.fac[0];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t cw = c0 + (wave / G::WGN) * G::WM, vw = v0 + (wave % G::WGN) * G::WN;
+    g_each<4>([&](auto jj) __attribute__((always_inline)) {
+      constexpr int j = decltype(jj)::value;
+      uint2 u[8];
 #pragma unroll
-    for (int j = 0; j < G::NJ; ++j) {
-      uint2 u[G::MI];
-#pragma unroll
-      for (int i = 0; i < G::MI; ++i)
-        u[i] = make_uint2(
-            to16<T8>(f * acc[i][j][0]) | (uint32_t)to16<T8>(f * acc[i][j][1]) << 16,
-            to16<T8>(f * acc[i][j][2]) | (uint32_t)to16<T8>(f * acc[i][j][3]) << 16);
-      g_rows_out<G>(priv, u, [&](int r, int m, const uint4& x) {
-        const int64_t v = vw + 16 * j + r;
-        if (v < nv && cw + m < C) *(uint4*)(dW + v * ldo + cw + m) = x;   // C: a multiple of 8
+      for (int i = 0; i < 8; ++i) {
+        const f4_t& a = acc.v[i][j];
+        u[i] = make_uint2(to16<T8>(f * a[0]) | (uint32_t)to16<T8>(f * a[1]) << 16,
+                          to16<T8>(f * a[2]) | (uint32_t)to16<T8>(f * a[3]) << 16);
+      }
+      g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
+        const int64_t v = v0 + g_n(j, wave, 0) + r;
+        if (v < p.nv && c0 + m < p.C)                            // C: a multiple of 8
+          *(uint4*)(p.dW + v * p.ldo + c0 + m) = x;
       });
-    }
+    });
   }
 };
 
-template <typename T8, typename G>
-__global__ __launch_bounds__(G::THREADS) void k_head_dw(const DwArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[G::LDS + G_PRIV];
-  g_run<T8, G>(smem, DwJob<T8, G>(p));
+template <typename T8>
+__global__ __launch_bounds__(G_THREADS) void k_head_dw(const DwArgs) {
+  __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
+  g_run<T8, false, false>(smem, DwJob<T8>());
 }
 
 // ---------------------------------------------------------------------------
@@ -879,20 +896,20 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dw(const DwArgs p) {
 // ---------------------------------------------------------------------------
 // Tiles of the products (m x n): vocabulary x tokens for z, channels x tokens
 // for dh, channels x vocabulary for dW.
-using ZL = GTile<256, 256, 2, 4, 2, true, true>;
 using ZM = GTile<256, 64, 4, 2, 4, true, true>;
 using ZS = GTile<256, 16, 8, 1, 4, true, true>;
-using HL = GTile<256, 256, 2, 4, 2, false, true>;
 using HM = GTile<256, 64, 4, 2, 4, false, true>;
 using HS = GTile<256, 16, 8, 1, 4, false, true>;
-using WL = GTile<256, 256, 2, 4, 2, false, false>;
+struct Big {               // the persistent 256 x 256 tiles
+  static constexpr int BM = 256, BN = 256, WGM = 2;
+};
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // tokens per tile: 0 = 16, 1 = 64, 2 = 256
 static int token_tile(int64_t T) { return T <= 16 ? 0 : T <= 64 ? 1 : 2; }
 static int64_t n_part(int64_t T, int64_t V) {
-  static const int wgm[3] = {ZS::WGM, ZM::WGM, ZL::WGM};
+  static const int wgm[3] = {ZS::WGM, ZM::WGM, Big::WGM};
   return cdiv(V, 256) * wgm[token_tile(T)];
 }
 static int64_t mask_words(int64_t V) { return cdiv(V, 256) * 8; }
@@ -984,8 +1001,8 @@ static void launch_fwd(FwdArgs p, hipStream_t s) {
   p.nm = (int)cdiv(p.V, G::BM);
   p.nn = (int)cdiv(p.T, G::BN);
   const int64_t tiles = (int64_t)p.nm * p.nn;
-  if constexpr (G::NS == 2)
-    k_head_fwd_p<T8, G, XENT><<<persistent(tiles), G::THREADS, 0, s>>>(p);
+  if constexpr (std::is_same<G, Big>::value)
+    k_head_fwd_p<T8, XENT><<<persistent(tiles), G_THREADS, 0, s>>>(p);
   else
     k_head_fwd<T8, G, XENT><<<(unsigned)tiles, G::THREADS, 0, s>>>(p);
 }
@@ -999,7 +1016,7 @@ static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int6
   switch (token_tile(T)) {
     case 0: launch_fwd<T8, ZS, XENT>(p, s); break;
     case 1: launch_fwd<T8, ZM, XENT>(p, s); break;
-    default: launch_fwd<T8, ZL, XENT>(p, s);
+    default: launch_fwd<T8, Big, XENT>(p, s);
   }
   CRBQ_LAUNCH_CHECK();
   float* rows = reduction ? w.rows : loss;
@@ -1034,8 +1051,8 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
     const uint16_t* Wv = W + v * ldw;
     const int nm = (int)cdiv(nv, GZ::BM);
     const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, ldz};
-    if constexpr (GZ::NS == 2)
-      k_head_dz_p<T8, GZ><<<persistent((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
+    if constexpr (std::is_same<GZ, Big>::value)
+      k_head_dz_p<T8><<<persistent((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
     else
       k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
     CRBQ_LAUNCH_CHECK();
@@ -1047,15 +1064,15 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
       const DhArgs q{Wv, w.dz, ldw, ldz, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
                      v > 0};
       const int64_t tiles = (int64_t)mh * nt * q.ns;
-      if constexpr (GH::NS == 2)
-        k_head_dh_p<T8, GH><<<persistent(tiles), GH::THREADS, 0, s>>>(q);
+      if constexpr (std::is_same<GH, Big>::value)
+        k_head_dh_p<T8><<<persistent(tiles), G_THREADS, 0, s>>>(q);
       else
         k_head_dh<T8, GH><<<(unsigned)tiles, GH::THREADS, 0, s>>>(q);
       CRBQ_LAUNCH_CHECK();
     }
     if (dW) {
-      const int mw = (int)cdiv(C, WL::BM), nw = (int)cdiv(nv, WL::BN);
-      k_head_dw<T8, WL><<<persistent((int64_t)mw * nw), WL::THREADS, 0, s>>>(
+      const int mw = (int)cdiv(C, 256), nw = (int)cdiv(nv, 256);
+      k_head_dw<T8><<<persistent((int64_t)mw * nw), G_THREADS, 0, s>>>(
           DwArgs{h, w.dz, ldh, ldz, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
       CRBQ_LAUNCH_CHECK();
     }
@@ -1084,7 +1101,7 @@ static int head_grad_t(const void* h, int64_t ldh, const void* W, int64_t ldw, i
       return head_grad<T8, ZM, HM, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
                                          g, per_row, oh, ldd, ow, ldo, w, s);
     default:
-      return head_grad<T8, ZL, HL, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
+      return head_grad<T8, Big, Big, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
                                          g, per_row, oh, ldd, ow, ldo, w, s);
   }
 }
