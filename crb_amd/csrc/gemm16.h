@@ -59,6 +59,7 @@ __device__ __forceinline__ void g_wait_vm() {
 struct GOperand {
   const uint16_t* p;       // KC: &P[row0 * ld]; K-strided: &P[row0]
   int64_t ld;
+  int64_t kstep;           // elements from one 64 k to the next: 64 (KC), 64 ld (K-strided)
   int64_t rows;            // rows (outputs) from row0 to the end; K-strided: even
   int64_t K;               // k's that exist; KC: a multiple of 8
   const uint64_t* live;    // K-strided only, may be null: bit k % 64 of word k / 64 clear =
@@ -99,14 +100,10 @@ struct GStage {
   __device__ static i4_t rsrc(const GOperand& o, int64_t k0, int64_t K) {
     const int64_t kl = K - k0;
     int64_t n = 0;
-    if (KC) {
-      const int64_t rows = o.rows < R ? o.rows : R;
-      if (kl > 0) n = ((rows - 1) * o.ld + kl) * 2;
-      return g_rsrc(o.p + (kl > 0 ? k0 : 0), n);
-    }
-    const int64_t rows = kl < G_K ? kl : G_K;
-    if (kl > 0) n = ((rows - 1) * o.ld + o.rows) * 2;
-    return g_rsrc(o.p + (kl > 0 ? k0 * o.ld : 0), n);
+    const int64_t ks = kl < G_K ? kl : G_K;
+    if (kl > 0) n = KC ? (((o.rows < R ? o.rows : R) - 1) * o.ld + ks) * 2
+                       : ((ks - 1) * o.ld + o.rows) * 2;
+    return g_rsrc(o.p + (kl > 0 ? k0 / G_K * o.kstep : 0), n);
   }
 };
 
@@ -414,19 +411,28 @@ __device__ __forceinline__ T* g_uni(T* q) {
               (uint64_t)(uint32_t)g_uni((int)(v >> 32)) << 32);
 }
 
+// How g_run takes an operand: K-contiguous, K-strided, and both of a matrix
+// [k or row blocks of 64][rows or k][64] in blocks, whose units of 64 x 64 are 8 KB in
+// one piece.  Blocked operands are not range-checked: they have to hold
+// every element of the tiles and stages asked for.
+enum GLayout { G_KC, G_KS, G_KC_BLOCKED, G_KS_BLOCKED };
+constexpr bool g_is_kc(GLayout l) { return l == G_KC || l == G_KC_BLOCKED; }
+constexpr bool g_is_blocked(GLayout l) { return l == G_KC_BLOCKED || l == G_KS_BLOCKED; }
+
 // Where the loads of one operand stand within a tile.
-template <bool KC>
+template <GLayout L>
 struct GCursor {
+  static constexpr bool KC = g_is_kc(L);
   const uint16_t* p;       // the stage's first element
   int rows, k;             // rows (at most 256) and k's left from there; k <= 0: none
   __device__ void open(const GOperand& o, int64_t k0) {
     const int64_t kl = o.K - k0;
-    p = g_uni(o.p + (KC ? k0 : k0 * o.ld));
+    p = g_uni(o.p + k0 / G_K * o.kstep);
     rows = g_uni((int)(o.rows < 256 ? o.rows : 256));
     k = g_uni((int)(kl < (1 << 30) ? kl : (1 << 30)));
   }
-  __device__ void advance(int64_t ld) {
-    p += KC ? (int64_t)G_K : G_K * ld;
+  __device__ void advance(int kstep) {
+    p += kstep;
     k -= G_K;
   }
   // descriptor of the whole stage (rows < 256 x 2^22 elements: below 2^31 bytes)
@@ -434,24 +440,20 @@ struct GCursor {
     int n;
     if (KC) n = (rows - 1) * ld + (k < G_K ? k : G_K);
     else n = ((k < G_K ? k : G_K) - 1) * ld + rows;
+    if (g_is_blocked(L)) n = 0x3fffffff;
     return g_rsrc(p, k > 0 ? n * 2 : 0);
   }
 };
 
-// (an instruction's offset counts for its LDS address too)
-template <int U>
-__device__ __forceinline__ void g_load_unit(const void* dst, i4_t rs, unsigned voff) {
-  const unsigned d = __builtin_amdgcn_readfirstlane(
-      (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)dst) - U * 128;
-  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen offset:%2 lds" ::"v"(voff), "s"(rs),
-               "n"(U * 128), "{m0}"(d));
-}
-
-template <typename T8, bool AKC, bool BKC, typename Job>
+template <typename T8, GLayout LA, GLayout LB, typename Job>
 __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  constexpr bool AKC = g_is_kc(LA), BKC = g_is_kc(LB);
+  // row strides, and the elements from one 64 k to the next, from one unit to the next
   const int lda = g_uni((int)job.lda()), ldb = g_uni((int)job.ldb());
+  const int ka = g_uni((int)job.kstep_a()), kb = g_uni((int)job.kstep_b());
+  const int ua = g_uni((int)job.unit_a()) * 2, ub = g_uni((int)job.unit_b()) * 2;
   const int tiles = g_uni(job.tiles());
   const GUnits<AKC> UA(lda, wave, lane, wave >> 2);
   const GUnits<BKC> UB(ldb, wave, lane, wave & 1);
@@ -465,8 +467,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   // operands are at hand.  A tile has at least 4 stages (the last ones
   // empty if need be), so that it is enough to look at one tile ahead, at
   // the end of each.
-  GCursor<AKC> ca, na;
-  GCursor<BKC> cb, nb;
+  GCursor<LA> ca, na;
+  GCursor<LB> cb, nb;
   const uint64_t *cl = nullptr, *nl = nullptr;
   int lc = 0, ln = 0, nn = 0;
   auto peek = [&](int lin) __attribute__((always_inline)) {      // the next tile: na, nb, nl, nn
@@ -493,8 +495,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   auto next = [&]() __attribute__((always_inline)) {
     Stage s{ca.rsrc(lda), cb.rsrc(ldb), BKC ? cb.k : ca.k, ~0ull};
     if (!AKC && cl) s.live = ca.k > 0 ? cl[lc] : 0;
-    ca.advance(lda);
-    cb.advance(ldb);
+    ca.advance(ka);
+    cb.advance(kb);
     if (++lc == ln) {
       ca = na;
       cb = nb;
@@ -508,18 +510,15 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   auto loadA = [&](auto uu, const Stage& s, int buf) __attribute__((always_inline)) {
     constexpr int u = decltype(uu)::value;
     char* d = mine + buf * G_STAGE + u * G_UNIT;
-    if constexpr (AKC)
-      g_load_unit<0>(d, s.ra, (UA.kc8 < s.k ? UA.voff : OUT) + (unsigned)(u * 128 * lda));
-    else
-      g_load_unit<u>(d, s.ra, Job::MASKED && !((s.live >> UA.row) & 1) ? OUT : UA.voff);
+    const bool in = AKC ? UA.kc8 < s.k : !Job::MASKED || ((s.live >> UA.row) & 1);
+    g_load_lds(d, s.ra, (in ? UA.voff : OUT) + (unsigned)(u * ua));
   };
   auto loadB = [&](auto uu, const Stage& s, int buf) __attribute__((always_inline)) {
     constexpr int u = decltype(uu)::value;
     char* d = mine + buf * G_STAGE + (4 + u) * G_UNIT;
-    if constexpr (BKC)
-      g_load_unit<0>(d, s.rb, (UB.kc8 < s.k ? UB.voff : OUT) + (unsigned)(u * 128 * ldb));
-    else
-      g_load_unit<u>(d, s.rb, UB.voff);
+    // (a blocked K-strided B may hold anything behind A's last k)
+    const bool in = LB == G_KC_BLOCKED || (BKC ? UB.kc8 : UB.row) < s.k;
+    g_load_lds(d, s.rb, (in ? UB.voff : OUT) + (unsigned)(u * ub));
   };
   // A fragment (h, e) of unit u; B fragment (h, j)
   auto fragA = [&](int buf, int u, int h, int e) __attribute__((always_inline)) -> T8 {

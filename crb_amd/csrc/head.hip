@@ -190,8 +190,8 @@ __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
   int tm, tn;
   g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
   const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
-  const GOperand A{p.W + v0 * p.ldw, p.ldw, p.V - v0, p.C, nullptr};
-  const GOperand B{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
+  const GOperand A{p.W + v0 * p.ldw, p.ldw, G_K, p.V - v0, p.C, nullptr};
+  const GOperand B{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
   f4_t acc[G::MI][G::NJ];
   g_tile<T8, G>(smem, A, B, 0, p.C, acc);
   const int lane = threadIdx.x & 63;
@@ -222,6 +222,10 @@ struct FwdJob {
   static constexpr bool MASKED = false;
   __device__ static int64_t lda() { return g_args<FwdArgs>().ldw; }
   __device__ static int64_t ldb() { return g_args<FwdArgs>().ldh; }
+  __device__ static int64_t kstep_a() { return G_K; }
+  __device__ static int64_t kstep_b() { return G_K; }
+  __device__ static int64_t unit_a() { return G_K * lda(); }
+  __device__ static int64_t unit_b() { return G_K * ldb(); }
   __device__ static int tiles() {
     const FwdArgs p = g_args<FwdArgs>();
     return p.nm * p.nn;
@@ -238,8 +242,8 @@ struct FwdJob {
     int64_t v0, t0;
     int tm;
     place(p, lin, v0, t0, tm);
-    A = GOperand{p.W + v0 * p.ldw, p.ldw, p.V - v0, p.C, nullptr};
-    B = GOperand{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
+    A = GOperand{p.W + v0 * p.ldw, p.ldw, G_K, p.V - v0, p.C, nullptr};
+    B = GOperand{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
     k = 0;
     nch = (int)((p.C + G_K - 1) / G_K);
   }
@@ -297,7 +301,7 @@ struct FwdJob {
 template <typename T8, bool XENT>
 __global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs) {
   __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
-  g_run<T8, true, true>(smem, FwdJob<XENT>());
+  g_run<T8, G_KC, G_KC>(smem, FwdJob<XENT>());
 }
 
 // The saved state of a forward, in floats: a [T], lse [T], one factor (1 or
@@ -570,8 +574,20 @@ struct DzArgs {
   const float *a2, *rowb;
   int nm, nn;
   uint16_t* dz;
-  int64_t ldz;
+  int64_t zstep;
 };
+
+// A piece's dz in memory: blocks of 64 columns, each dz_rows(T) rows of 128
+// bytes, so that a unit of either product that reads it is 8 KB in one
+// piece (row by row, dW's loads went 64 KB from row to row: 0.53 of the time
+// with busy MFMAs against 0.72 of dh's).  The columns of whole tiles are
+// written, zeros behind nv; the rows behind T are not, and dh's tiles, which
+// read them, do not keep what comes of them.
+__host__ __device__ __forceinline__ int64_t dz_cols(int64_t nv) { return (nv + 255) / 256 * 256; }
+__host__ __device__ __forceinline__ int64_t dz_rows(int64_t T) { return (T + 255) / 256 * 256; }
+__device__ __forceinline__ uint16_t* dz_at(uint16_t* dz, int64_t zstep, int64_t t, int64_t v) {
+  return dz + v / G_K * zstep + t * G_K + v % G_K;
+}
 
 // 4 consecutive tokens from v on, of row t
 template <typename T8>
@@ -596,8 +612,8 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
   int tm, tn;
   g_band(g_xcd(blockIdx.x, gridDim.x), p.nm, p.nn, tm, tn);
   const int64_t v0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
-  const GOperand A{p.W + v0 * p.ldw, p.ldw, p.nv - v0, p.C, nullptr};
-  const GOperand B{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
+  const GOperand A{p.W + v0 * p.ldw, p.ldw, G_K, p.nv - v0, p.C, nullptr};
+  const GOperand B{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
   f4_t acc[G::MI][G::NJ];
   g_tile<T8, G>(smem, A, B, 0, p.C, acc);
   const int lane = threadIdx.x & 63;
@@ -611,8 +627,8 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
     const float b = p.rowb[t], a2 = p.a2[t];
 #pragma unroll
     for (int i = 0; i < G::MI; ++i) {
-      const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below ldz
-      *(uint2*)(p.dz + t * p.ldz + v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v);
+      const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below dz_cols
+      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v);
     }
   }
 }
@@ -622,6 +638,10 @@ struct DzJob {
   static constexpr bool MASKED = false;
   __device__ static int64_t lda() { return g_args<DzArgs>().ldw; }
   __device__ static int64_t ldb() { return g_args<DzArgs>().ldh; }
+  __device__ static int64_t kstep_a() { return G_K; }
+  __device__ static int64_t kstep_b() { return G_K; }
+  __device__ static int64_t unit_a() { return G_K * lda(); }
+  __device__ static int64_t unit_b() { return G_K * ldb(); }
   __device__ static int tiles() {
     const DzArgs p = g_args<DzArgs>();
     return p.nm * p.nn;
@@ -637,8 +657,8 @@ struct DzJob {
     const DzArgs p = g_args<DzArgs>();
     int64_t v0, t0;
     place(p, lin, v0, t0);
-    A = GOperand{p.W + v0 * p.ldw, p.ldw, p.nv - v0, p.C, nullptr};
-    B = GOperand{p.h + t0 * p.ldh, p.ldh, p.T - t0, p.C, nullptr};
+    A = GOperand{p.W + v0 * p.ldw, p.ldw, G_K, p.nv - v0, p.C, nullptr};
+    B = GOperand{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
     k = 0;
     nch = (int)((p.C + G_K - 1) / G_K);
   }
@@ -680,7 +700,7 @@ struct DzJob {
                            whole ? 4 : p.nv - (v0 + g_m(i, wave, lane)));
       g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
         const int64_t t = t0 + g_n(j, wave, 0) + r;
-        if (t < p.T) *(uint4*)(p.dz + t * p.ldz + v0 + m) = x;         // v0 + 256 <= ldz
+        if (t < p.T) *(uint4*)dz_at(p.dz, p.zstep, t, v0 + m) = x;
       });
     });
   }
@@ -689,7 +709,7 @@ struct DzJob {
 template <typename T8>
 __global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs) {
   __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
-  g_run<T8, true, true>(smem, DzJob<T8>());
+  g_run<T8, G_KC, G_KC>(smem, DzJob<T8>());
 }
 
 // the listed tokens' dz within [vbeg, vbeg + nv)
@@ -697,7 +717,7 @@ template <typename T8, bool XENT>
 __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
                                                    const int64_t* __restrict__ labels,
                                                    const float* __restrict__ ratio, int64_t vbeg,
-                                                   int64_t nv, uint16_t* dz, int64_t ldz) {
+                                                   int64_t nv, uint16_t* dz, int64_t zstep) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t t = XENT ? e : e / k;
   if (t >= T) return;
@@ -707,14 +727,14 @@ __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
   float d;
   if (XENT) d = -expf(st.a[t] - lse);
   else d = st.mass[t] * expf(st.zt[e] - lse) - st.p[e];
-  dz[t * ldz + v - vbeg] = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
+  *dz_at(dz, zstep, t, v - vbeg) = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
 }
 
 // dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the
 // split's v (span of them, a multiple of 64)
 struct DhArgs {
   const uint16_t *W, *dz;
-  int64_t ldw, ldz, T, nv, C, span;
+  int64_t ldw, zstep, T, nv, C, span;
   int nm, nn, ns;
   float* P;
   int add;
@@ -741,8 +761,8 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
   g_band(lin - split * p.nm * p.nn, p.nm, p.nn, tm, tn);
   const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
   const int64_t kb = split * p.span, ke = kb + p.span < p.nv ? kb + p.span : p.nv;
-  const GOperand A{p.W + c0, p.ldw, p.C - c0, p.nv, nullptr};
-  const GOperand B{p.dz + t0 * p.ldz, p.ldz, p.T - t0, p.ldz, nullptr};
+  const GOperand A{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, p.nv, nullptr};
+  const GOperand B{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
   f4_t acc[G::MI][G::NJ];
   g_tile<T8, G>(smem, A, B, kb, ke, acc);
   const int lane = threadIdx.x & 63;
@@ -758,7 +778,11 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
 struct DhJob {
   static constexpr bool MASKED = false;
   __device__ static int64_t lda() { return g_args<DhArgs>().ldw; }
-  __device__ static int64_t ldb() { return g_args<DhArgs>().ldz; }
+  __device__ static int64_t ldb() { return G_K; }
+  __device__ static int64_t kstep_a() { return G_K * lda(); }
+  __device__ static int64_t kstep_b() { return g_args<DhArgs>().zstep; }
+  __device__ static int64_t unit_a() { return G_K; }
+  __device__ static int64_t unit_b() { return G_K * G_K; }
   __device__ static int tiles() {
     const DhArgs p = g_args<DhArgs>();
     return p.nm * p.nn * p.ns;
@@ -776,8 +800,8 @@ struct DhJob {
     int64_t c0, t0;
     int split;
     place(p, lin, c0, t0, split);
-    A = GOperand{p.W + c0, p.ldw, p.C - c0, p.nv, nullptr};
-    B = GOperand{p.dz + t0 * p.ldz, p.ldz, p.T - t0, p.ldz, nullptr};
+    A = GOperand{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, p.nv, nullptr};
+    B = GOperand{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
     k = split * p.span;
     const int64_t n = p.nv - k < p.span ? p.nv - k : p.span;   // > 0 for every split of a launch
     nch = (int)((n + G_K - 1) / G_K);
@@ -801,7 +825,7 @@ struct DhJob {
 template <typename T8>
 __global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs) {
   __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
-  g_run<T8, false, true>(smem, DhJob());
+  g_run<T8, G_KS, G_KC_BLOCKED>(smem, DhJob());
 }
 
 // dh = fac * (P[0] + P[1] + ...), rounded once; 4 channels a thread
@@ -827,7 +851,7 @@ __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int
 // dW[v][c] = fac * sum_t dz[t][v] h[t][c] of a piece's rows v
 struct DwArgs {
   const uint16_t *h, *dz;
-  int64_t ldh, ldz, T, nv, C;
+  int64_t ldh, zstep, T, nv, C;
   const uint64_t* live;
   int nm, nn;
   const float* fac;
@@ -839,7 +863,11 @@ template <typename T8>
 struct DwJob {
   static constexpr bool MASKED = true;
   __device__ static int64_t lda() { return g_args<DwArgs>().ldh; }
-  __device__ static int64_t ldb() { return g_args<DwArgs>().ldz; }
+  __device__ static int64_t ldb() { return G_K; }
+  __device__ static int64_t kstep_a() { return G_K * lda(); }
+  __device__ static int64_t kstep_b() { return G_K * G_K; }
+  __device__ static int64_t unit_a() { return G_K; }
+  __device__ static int64_t unit_b() { return g_args<DwArgs>().zstep; }
   __device__ static int tiles() {
     const DwArgs p = g_args<DwArgs>();
     return p.nm * p.nn;
@@ -855,8 +883,8 @@ struct DwJob {
     const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
     place(p, lin, c0, v0);
-    A = GOperand{p.h + c0, p.ldh, p.C - c0, p.T, p.live};
-    B = GOperand{p.dz + v0, p.ldz, p.ldz - v0, p.T, nullptr};
+    A = GOperand{p.h + c0, p.ldh, G_K * p.ldh, p.C - c0, p.T, p.live};
+    B = GOperand{p.dz + v0 / G_K * p.zstep, G_K, G_K * G_K, 256, p.T, nullptr};
     k = 0;
     nch = (int)((p.T + G_K - 1) / G_K);
   }
@@ -888,7 +916,7 @@ struct DwJob {
 template <typename T8>
 __global__ __launch_bounds__(G_THREADS) void k_head_dw(const DwArgs) {
   __shared__ __attribute__((aligned(1024))) char smem[G_LDS];
-  g_run<T8, false, false>(smem, DwJob<T8>());
+  g_run<T8, G_KS, G_KS_BLOCKED>(smem, DwJob<T8>());
 }
 
 // ---------------------------------------------------------------------------
@@ -963,7 +991,7 @@ struct GradWs {
     piece = piece_of(T, V);
     span = cdiv(cdiv(piece < V ? piece : V, dh_splits(T, C, piece)), G_K) * G_K;
     ns = (int)cdiv(piece < V ? piece : V, span);
-    dz = w.take<uint16_t>((size_t)(T * piece));
+    dz = w.take<uint16_t>((size_t)(dz_rows(T) * piece));
     P = w.take<float>((size_t)(T * C) * ns);
     a2 = w.take<float>((size_t)T);
     rowb = w.take<float>((size_t)T);
@@ -983,7 +1011,7 @@ static int check_head(const void* h, int64_t ldh, const void* W, int64_t ldw, in
                       int64_t T, int64_t V, int64_t C) {
   if (dtype != CRBQ_F16 && dtype != CRBQ_BF16) return CRBQ_ERR_ARG;
   if (T < 1 || V < 1 || C < 8 || (C & 7) || V >= ((int64_t)1 << 31) - 256 ||
-      T >= ((int64_t)1 << 31) - 256)
+      T >= ((int64_t)1 << 22))
     return CRBQ_ERR_ARG;
   if (bad_matrix(h, ldh, C) || bad_matrix(W, ldw, C)) return CRBQ_ERR_ARG;
   if (cdiv(V, 256) * cdiv(T, 16) >= ((int64_t)1 << 31)) return CRBQ_ERR_ARG;
@@ -1046,22 +1074,23 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
                                                          w.live, w.fac);
   CRBQ_LAUNCH_CHECK();
   const int nt = (int)cdiv(T, GZ::BN);
+  const int64_t zstep = dz_rows(T) * G_K;
   for (int64_t v = 0; v < V; v += w.piece) {
-    const int64_t nv = V - v < w.piece ? V - v : w.piece, ldz = cdiv(nv, 256) * 256;
+    const int64_t nv = V - v < w.piece ? V - v : w.piece;
     const uint16_t* Wv = W + v * ldw;
     const int nm = (int)cdiv(nv, GZ::BM);
-    const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, ldz};
+    const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, zstep};
     if constexpr (std::is_same<GZ, Big>::value)
       k_head_dz_p<T8><<<persistent((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
     else
       k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
     CRBQ_LAUNCH_CHECK();
     k_dz_listed<T8, XENT><<<(unsigned)cdiv(XENT ? T : T * k, 256), 256, 0, s>>>(
-        st, T, k, labels, w.ratio, v, nv, w.dz, ldz);
+        st, T, k, labels, w.ratio, v, nv, w.dz, zstep);
     CRBQ_LAUNCH_CHECK();
     if (dh) {
       const int mh = (int)cdiv(C, GH::BM);
-      const DhArgs q{Wv, w.dz, ldw, ldz, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
+      const DhArgs q{Wv, w.dz, ldw, zstep, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
                      v > 0};
       const int64_t tiles = (int64_t)mh * nt * q.ns;
       if constexpr (std::is_same<GH, Big>::value)
@@ -1073,7 +1102,7 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
     if (dW) {
       const int mw = (int)cdiv(C, 256), nw = (int)cdiv(nv, 256);
       k_head_dw<T8><<<persistent((int64_t)mw * nw), G_THREADS, 0, s>>>(
-          DwArgs{h, w.dz, ldh, ldz, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
+          DwArgs{h, w.dz, ldh, zstep, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
       CRBQ_LAUNCH_CHECK();
     }
   }

@@ -357,7 +357,7 @@ int crbq_linear_packed(const uint8_t* codes, int64_t ldc, const void* lut, const
  * No counterpart in the reference, whose perplexity forms all logits and
  * calls a cross entropy (eval_ppl_utils.py:626-636).  Hidden states h [T][C]
  * and the head's weight W [V][C], both fp16 or both bf16 (16-byte aligned,
- * row strides multiples of 8 below 2^22, C a multiple of 8); logits
+ * row strides multiples of 8 below 2^22, C a multiple of 8, T below 2^22); logits
  * z = scale * h W^T are computed piece by piece in fp32 and never kept.
  *
  * crbq_head_xent: loss_t = log sum_v exp z[t][v] - z[t][labels[t]].
