@@ -484,7 +484,7 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
       nn = g_uni(nn < 4 ? 4 : nn);
       na.open(A, k);
       nb.open(B, k);
-      if (!AKC && A.live) nl = A.live + k / G_K;
+      if (!AKC && A.live) nl = g_uni(A.live + k / G_K);
     }
   };
   struct Stage {
@@ -494,7 +494,9 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   };
   auto next = [&]() __attribute__((always_inline)) {
     Stage s{ca.rsrc(lda), cb.rsrc(ldb), BKC ? cb.k : ca.k, ~0ull};
-    if (!AKC && cl) s.live = ca.k > 0 ? cl[lc] : 0;
+    // (a scalar load: a vector load's wait would be for all stages in flight)
+    if (!AKC && cl)
+      s.live = ca.k > 0 ? ((const __attribute__((address_space(4))) uint64_t*)cl)[lc] : 0;
     ca.advance(ka);
     cb.advance(kb);
     if (++lc == ln) {
