@@ -127,13 +127,13 @@ _SIGS = {
     "crbq_head_xent": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp, c_i64,
                                ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
     "crbq_head_xent_grad": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp,
-                                    c_i64, ctypes.c_float, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp,
-                                    c_i64, c_vp, c_size, c_vp]),
+                                    ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64,
+                                    c_vp, c_size, c_vp]),
     "crbq_head_distill": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_vp,
                                   c_i32, c_i64, c_vp, c_i64, c_i32, c_vp, ctypes.c_float,
                                   ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_size, c_vp]),
     "crbq_head_distill_grad": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64,
-                                       c_i32, ctypes.c_float, ctypes.c_float, c_vp, c_vp, c_i32,
+                                       c_i32, ctypes.c_float, ctypes.c_float, c_i32, c_vp, c_vp,
                                        c_vp, c_i64, c_vp, c_i64, c_vp, c_size, c_vp]),
     "crbq_top_logits": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_i32, ctypes.c_float, c_vp,
                                 c_vp, c_vp, c_vp]),

@@ -464,8 +464,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   if (first >= tiles) return;                          // no tile at all
 
   // The stages in load order: stage lc of a tile of ln; then the next tile, whose
-  // operands are at hand.  A tile has at least 4 stages (the last ones
-  // empty if need be), so that it is enough to look at one tile ahead, at
+  // operands are at hand.  A tile has at least 4 stages (the last ones behind
+  // A's last k, so zeros, if need be), so that it is enough to look at one tile ahead, at
   // the end of each.
   GCursor<LA> ca, na;
   GCursor<LB> cb, nb;

@@ -304,49 +304,72 @@ __global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs) {
   g_run<T8, G_KC, G_KC>(smem, FwdJob<XENT>());
 }
 
-// The saved state of a forward, in floats: a [T], lse [T], one factor (1 or
-// 1 / the rows a mean is over), one unused; then cross entropy: z of the
-// label [T]; distillation: p_T [T], sum of p log p over the listed entries
-// [T], m [T], and of the lists' distinct tokens z [T][k], p [T][k] and, ascending,
-// the tokens themselves (int32) [T][k].
+// The saved state of a forward: live rows (a bit each, 64-bit words), one
+// factor (1, or 1 / the rows a mean is over) and one float unused; per row a,
+// lse, the factor of exp(z - a) in dz and the row's weight there (both times
+// dz_scale; 0 for a row left out); then cross entropy: z of the label;
+// distillation: p_T, the sum of p log p over the listed entries, m, and of the
+// lists' distinct tokens z [T][k], p [T][k] and, ascending, the tokens
+// themselves (int32) [T][k].  live is written with a sum or mean only.
 struct State {
-  float *a, *lse, *inv, *pt, *ent, *mass, *zt, *p;
+  uint64_t* live;
+  float *inv, *a, *lse, *rowb, *ratio, *pt, *ent, *mass, *zt, *p;
   int32_t* sidx;
   __host__ __device__ State(float* b, int64_t T, int64_t k) {
-    a = b;
+    live = (uint64_t*)b;
+    inv = b + (T + 63) / 64 * 2;
+    a = inv + 2;
     lse = a + T;
-    inv = lse + T;
-    pt = inv + 2;
+    rowb = lse + T;
+    ratio = rowb + T;
+    pt = ratio + T;
     ent = pt + T;
     mass = ent + T;
     zt = k ? mass + T : pt;
     p = zt + T * k;
     sidx = (int32_t*)(p + T * k);
   }
+  static int64_t floats(int64_t T, int64_t k) {
+    return (T + 63) / 64 * 2 + 2 + (k ? (3 * k + 7) * T : 5 * T);
+  }
 };
 
-// Joins a row's partial sums and finishes its loss; a wavefront a row.  A
-// row that is left out (ignored label, empty list) has loss 0; rows[t] < 0
-// never holds otherwise, so its count flag goes beside it.
-template <bool XENT>
+// Joins a row's partial sums and finishes its loss; WPR wavefronts a row (a
+// whole workgroup where rows are few: one wavefront alone takes 26 us for the 4008
+// pairs of one row of 128256 tokens).  A row that is left out (ignored label,
+// empty list) has loss 0 and live 0.
+template <bool XENT, int WPR>
 __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ part, int64_t npart,
                                                    int64_t T, int64_t V, int k,
                                                    const int64_t* __restrict__ labels,
-                                                   int64_t ignore, State st, float* rows,
-                                                   uint8_t* live, int reduction) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && reduction == 0) st.inv[0] = 1.f;
+                                                   int64_t ignore, State st, float zscale,
+                                                   float* rows, uint8_t* live) {
+  __shared__ float2 red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (blockIdx.x == 0 && threadIdx.x == 0) st.inv[0] = 1.f;
   if (t >= T) return;
   float m = -INFINITY, s = 0.f;
-  for (int64_t i = lane; i < npart; i += 64) {
-    const float2 p = part[t * npart + i];
-    ms_join(m, s, p.x, p.y);
+  const float2* pt = part + t * npart;
+  int64_t i = WPR == 4 ? threadIdx.x : lane;
+  for (; i + 3 * 64 * WPR < npart; i += 4 * 64 * WPR) {
+    float2 q[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) q[d] = pt[i + d * 64 * WPR];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) ms_join(m, s, q[d].x, q[d].y);
   }
+  for (; i < npart; i += 64 * WPR) ms_join(m, s, pt[i].x, pt[i].y);
 #pragma unroll
   for (int d = 32; d; d >>= 1) ms_join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  if (WPR == 4) {
+    if (lane == 0) red[wave] = make_float2(m, s);
+    __syncthreads();
+    if (wave) return;
+    for (int w = 1; w < 4; ++w) ms_join(m, s, red[w].x, red[w].y);
+  }
   const float a = LN2 * (m + log2f(s));                // -inf where every token is listed
-  float loss, lse;
+  float loss, lse, tail;                               // tail: the factor of exp(z - a)
   bool on;
   if (XENT) {
     const int64_t y = labels[t];
@@ -357,7 +380,7 @@ __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ pa
     loss = d > 0.f ? d + log1pf(expf(-d)) : log1pf(expf(d));
     lse = in ? z + loss : NAN;
     if (d != d) loss = d;
-    if (!on) loss = 0.f;
+    tail = expf(a - lse);
   } else {
     float tm = -INFINITY, ts = 0.f, np = 0.f;
     for (int i = lane; i < k; i += 64)
@@ -375,34 +398,39 @@ __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ pa
       if (st.sidx[t * k + i] != PAD_IDX && !(p == 0.f)) l += p * (lse - st.zt[t * k + i]);
     }
     loss = wave_sum_f(l) + st.ent[t];
-    float pt = st.pt[t];
+    float pt = st.pt[t], mass = st.mass[t];
     if (a == -INFINITY) {                              // no token is left for the tail
-      if (lane == 0) {
-        st.mass[t] -= pt;
-        st.pt[t] = 0.f;
-      }
+      mass -= pt;
       pt = 0.f;
+      if (lane == 0) st.mass[t] = mass;
     }
     if (!(pt == 0.f)) loss += pt * (logf(pt) - a + lse);
-    if (!on) loss = 0.f;
+    tail = mass * expf(a - lse) - pt;
   }
   if (lane == 0) {
     st.a[t] = a;
     st.lse[t] = lse;
-    rows[t] = loss;
+    st.rowb[t] = on ? zscale * tail : 0.f;
+    st.ratio[t] = on ? zscale : 0.f;
+    rows[t] = on ? loss : 0.f;
     if (live) live[t] = on;
   }
 }
 
-// Sum or mean of the rows' losses, in a fixed order, by one workgroup.
+// Sum or mean of the rows' losses, in a fixed order, and the live rows' bits,
+// by one workgroup.
 __global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ rows,
                                                       const uint8_t* __restrict__ live, int64_t T,
-                                                      int mean, float* loss, float* inv) {
+                                                      int mean, float* loss, State st) {
   __shared__ float ls[16], lc[16];
   float s = 0.f, c = 0.f;
-  for (int64_t t = threadIdx.x; t < T; t += 1024) {
-    s += rows[t];
-    c += live[t] ? 1.f : 0.f;
+  for (int64_t t0 = threadIdx.x & ~63; t0 < T; t0 += 1024) {
+    const int64_t t = t0 + (threadIdx.x & 63);
+    const bool on = t < T && live[t];
+    const uint64_t bits = __ballot(on);
+    if (t < T) s += rows[t];
+    c += on ? 1.f : 0.f;
+    if ((threadIdx.x & 63) == 0) st.live[t0 / 64] = bits;
   }
   s = wave_sum_f(s);
   c = wave_sum_f(c);
@@ -418,18 +446,13 @@ __global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ 
       c += lc[w];
     }
     loss[0] = mean ? s / c : s;                        // a mean over no row: NaN
-    inv[0] = mean ? (c > 0.f ? 1.f / c : 0.f) : 1.f;
+    st.inv[0] = mean ? (c > 0.f ? 1.f / c : 0.f) : 1.f;
   }
 }
 
-__global__ void k_fill_u32(uint32_t* p, int64_t n, uint32_t v) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x)
-    p[i] = v;
-}
-
 // The teacher's list of each row: tokens ascending, probabilities, the
-// bits of the forward product.  One wavefront a row.  Tokens outside
+// bits of the forward product (the row's words are cleared first).  One
+// wavefront a row.  Tokens outside
 // [0, V) are empty slots; of one listed twice the list holds one entry with
 // the sum of its probabilities.
 constexpr int LIST_MAX = 256;
@@ -439,11 +462,15 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
                                              const float* __restrict__ tlse, float itemp,
                                              int64_t V, int k, State st, uint32_t* mask,
                                              int64_t ldm) {
-  __shared__ int ix[LIST_MAX];
-  __shared__ float pr[LIST_MAX];
+  __shared__ __attribute__((aligned(16))) int ix[LIST_MAX];
+  __shared__ __attribute__((aligned(16))) float pr[LIST_MAX];
   const int lane = threadIdx.x;
   const int64_t t = blockIdx.x;
+  uint4* words = (uint4*)(mask + t * ldm);             // ldm is a multiple of 8
+  for (int64_t i = lane; i < ldm / 4; i += 64) words[i] = make_uint4(0u, 0u, 0u, 0u);
   float m = -INFINITY;
+  const int k4 = (k + 3) & ~3;
+  if (lane < k4 - k) ix[k + lane] = -1;                // read by fours
   for (int i = lane; i < k; i += 64) {
     const int v = idx[t * ldi + i];
     const float x = (float)val[t * ldv + i] * itemp;
@@ -478,12 +505,18 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
     prob[q] = 0.f;
     if (i < k && ix[i] >= 0) {
       bool first = true;
-      for (int j = 0; j < k; ++j)
-        if (ix[j] == ix[i]) {
-          if (j < i) first = false;
-          prob[q] += pr[j];
-        }
-      mine[q] = first ? ix[i] : -1;
+      const int me = ix[i];
+      for (int j = 0; j < k4; j += 4) {
+        const int4 o = *(const int4*)&ix[j];
+        const int w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (w[e] == me) {
+            if (j + e < i) first = false;
+            prob[q] += pr[j + e];
+          }
+      }
+      mine[q] = first ? me : -1;
     }
   }
   __syncthreads();
@@ -500,7 +533,12 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
   for (int q = 0; q < LIST_MAX / 64; ++q)
     if (mine[q] >= 0) {
       int rank = 0;
-      for (int j = 0; j < k; ++j) rank += ix[j] >= 0 && ix[j] < mine[q];
+      for (int j = 0; j < k4; j += 4) {
+        const int4 o = *(const int4*)&ix[j];
+        // (as unsigned numbers the empty slots, -1, are above all)
+        rank += ((uint32_t)o.x < (uint32_t)mine[q]) + ((uint32_t)o.y < (uint32_t)mine[q]) +
+                ((uint32_t)o.z < (uint32_t)mine[q]) + ((uint32_t)o.w < (uint32_t)mine[q]);
+      }
       st.sidx[t * k + rank] = mine[q];
       st.p[t * k + rank] = prob[q] * norm;
       atomicOr(mask + t * ldm + (mine[q] >> 5), 1u << (mine[q] & 31));
@@ -531,47 +569,47 @@ __global__ __launch_bounds__(1024) void k_absmax(const float* __restrict__ g, in
   }
 }
 
-// Row coefficients: dz of a row = coef (q - p) is stored relative to the
-// largest one, times dz_scale; *fac undoes both where the sums are rounded.
-// live: bit t set where the row's coefficient is not 0 (the other rows of h
-// are read as zeros: a masked row's NaN stays out of dW).
-// rowb[t] = the row's factor of exp(z - a); ratio[t] its share of the largest
-// coefficient, times dz_scale.
-template <bool XENT>
-__global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T, int k,
-                                                  const int64_t* __restrict__ labels,
-                                                  int64_t ignore, const float* __restrict__ g,
-                                                  int per_row, const float* __restrict__ gmax,
-                                                  float zscale, float scale, float* a2,
-                                                  float* rowb, float* ratio, uint64_t* live,
-                                                  float* fac) {
+// A gradient for each row: the row's dz is stored relative to the largest one
+// (undone where the sums are rounded).  live: bit t set where the row's gradient
+// is not 0 (the other rows of h are read as zeros: a masked row's NaN stays out
+// of dW).
+__global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T,
+                                                  const float* __restrict__ g,
+                                                  const float* __restrict__ gmax, float* rowb,
+                                                  float* ratio, uint64_t* live) {
   const int64_t t = (int64_t)blockIdx.x * 64 + threadIdx.x;
   float r = 0.f;
-  const float big = per_row ? gmax[0] : 1.f;
   if (t < T) {
-    bool on = true;
-    if (XENT) on = labels[t] != ignore;
-    else on = st.sidx[t * k] != PAD_IDX;               // sorted: an empty list starts empty
-    if (on) r = per_row ? (big == 0.f ? 0.f : g[t] / big) : 1.f;
-    r = r * zscale;
-    const float a = st.a[t], qt = expf(a - st.lse[t]);
+    const float big = gmax[0];
+    const float own = st.ratio[t];
+    const float w = own == 0.f || big == 0.f ? 0.f : g[t] / big;
+    r = own * w;
     ratio[t] = r;
-    a2[t] = a * LOG2E;
-    rowb[t] = r == 0.f ? 0.f : r * (XENT ? qt : st.mass[t] * qt - st.pt[t]);
+    rowb[t] = r == 0.f ? 0.f : st.rowb[t] * w;
   }
   const uint64_t bits = __ballot(!(r == 0.f));
   if (threadIdx.x == 0) live[blockIdx.x] = bits;
-  if (t == 0) fac[0] = (per_row ? big : g[0] * st.inv[0]) * (scale / zscale);
 }
 
+// What undoes the scaling of dz: f0 f1 mul (the loss's gradient or the largest
+// of the rows', 1 / the rows of a mean, scale / dz_scale).
+struct Factor {
+  const float *f0, *f1;
+  float mul;
+  __device__ float get() const { return f0[0] * f1[0] * mul; }
+};
+
 // dz of a piece of the vocabulary: dz[t][v - vbeg] = rowb exp(z - a), zeros
-// in the columns past the vocabulary (and where rowb is 0, whatever z is); the
-// listed tokens' own follow (k_dz_listed).  a2 = a in units of log 2.
+// in the columns past the vocabulary (and where rowb is 0, whatever z is).  A
+// label's own dz is -rowb (cross entropy); the listed tokens' of a
+// distillation follow (k_dz_listed).
 struct DzArgs {
   const uint16_t *h, *W;
   int64_t ldh, ldw, T, nv, C;
   float scale;
-  const float *a2, *rowb;
+  const float *a, *rowb;
+  const int64_t* labels;   // may be null
+  int64_t vbeg;
   int nm, nn;
   uint16_t* dz;
   int64_t zstep;
@@ -589,14 +627,21 @@ __device__ __forceinline__ uint16_t* dz_at(uint16_t* dz, int64_t zstep, int64_t 
   return dz + v / G_K * zstep + t * G_K + v % G_K;
 }
 
-// 4 consecutive tokens from v on, of row t
+// 4 consecutive tokens of a row, `left` of them within the vocabulary, the
+// label lab tokens on from the first
 template <typename T8>
 __device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2, float b,
-                                         int64_t left) {
+                                         int64_t left, int lab) {
   uint16_t o[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     o[r] = to16<T8>(b * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], scale2, -a2)));
+  if ((unsigned)lab < 4u) {
+    const uint16_t y = to16<T8>(-b);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r == lab) o[r] = y;
+  }
   if (left < 4) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -624,11 +669,14 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
   for (int j = 0; j < G::NJ; ++j) {
     const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
     if (t >= p.T) continue;
-    const float b = p.rowb[t], a2 = p.a2[t];
+    const float b = p.rowb[t], a2 = p.a[t] * LOG2E;
+    const int64_t y = p.labels ? p.labels[t] - p.vbeg : -1;
 #pragma unroll
     for (int i = 0; i < G::MI; ++i) {
       const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below dz_cols
-      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v);
+      const int64_t o = y - v;
+      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v,
+                                                        o >= 0 && o < 4 ? (int)o : -1);
     }
   }
 }
@@ -662,7 +710,7 @@ struct DzJob {
     k = 0;
     nch = (int)((p.C + G_K - 1) / G_K);
   }
-  // a2 and rowb of the wavefront's 2 x 32 rows (64 words are loaded for each 32)
+  // a, rowb and label of the wavefront's 2 x 32 rows (64 words of each)
   __device__ __forceinline__ void side(int lin, char* priv) const {
     const DzArgs p = g_args<DzArgs>();
     int64_t v0, t0;
@@ -672,8 +720,9 @@ struct DzJob {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int64_t t = t0 + 128 * b + 32 * (wave & 3), left = (p.T - t) * 4;
-      g_load_lds_words(priv + 512 * b, p.a2 + t, left, lane);
-      g_load_lds_words(priv + 512 * b + 256, p.rowb + t, left, lane);
+      g_load_lds_words(priv + 768 * b, p.a + t, left, lane);
+      g_load_lds_words(priv + 768 * b + 256, p.rowb + t, left, lane);
+      if (p.labels) g_load_lds_words(priv + 768 * b + 512, p.labels + t, left * 2, lane);
     }
   }
   __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
@@ -683,12 +732,17 @@ struct DzJob {
     const int lane = g_lane();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const float scale2 = p.scale * LOG2E;
+    const int64_t vt = p.vbeg + v0;                    // the tile's first token
     float at[4], b[4];
+    int lab[4];                                        // the label's place in the tile
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float* q = (const float*)(priv + 512 * (j >> 1)) + 16 * (j & 1) + (lane & 15);
-      at[j] = q[0];
-      b[j] = q[64];
+      const char* q = priv + 768 * (j >> 1);
+      const int row = 16 * (j & 1) + (lane & 15);
+      at[j] = ((const float*)q)[row] * LOG2E;
+      b[j] = ((const float*)q)[64 + row];
+      const int64_t y = p.labels ? ((const int64_t*)(q + 512))[row] - vt : -1;
+      lab[j] = y >= 0 && y < 256 ? (int)y : -4;
     }
     const bool whole = v0 + 256 <= p.nv;
     g_each<4>([&](auto jj) __attribute__((always_inline)) {
@@ -697,7 +751,8 @@ struct DzJob {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         u[i] = dz_pack<T8>(acc.v[i][j], scale2, at[j], b[j],
-                           whole ? 4 : p.nv - (v0 + g_m(i, wave, lane)));
+                           whole ? 4 : p.nv - (v0 + g_m(i, wave, lane)),
+                           lab[j] - g_m(i, wave, lane));
       g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
         const int64_t t = t0 + g_n(j, wave, 0) + r;
         if (t < p.T) *(uint4*)dz_at(p.dz, p.zstep, t, v0 + m) = x;
@@ -712,21 +767,16 @@ __global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs) {
   g_run<T8, G_KC, G_KC>(smem, DzJob<T8>());
 }
 
-// the listed tokens' dz within [vbeg, vbeg + nv)
-template <typename T8, bool XENT>
+// the listed tokens' dz within [vbeg, vbeg + nv) (distillation)
+template <typename T8>
 __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
-                                                   const int64_t* __restrict__ labels,
                                                    const float* __restrict__ ratio, int64_t vbeg,
                                                    int64_t nv, uint16_t* dz, int64_t zstep) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t t = XENT ? e : e / k;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, t = e / k;
   if (t >= T) return;
-  const int64_t v = XENT ? labels[t] : (int64_t)st.sidx[e];
-  if (v < vbeg || v >= vbeg + nv || (!XENT && v == PAD_IDX)) return;
-  const float r = ratio[t], lse = st.lse[t];
-  float d;
-  if (XENT) d = -expf(st.a[t] - lse);
-  else d = st.mass[t] * expf(st.zt[e] - lse) - st.p[e];
+  const int64_t v = st.sidx[e];
+  if (v == PAD_IDX || v < vbeg || v >= vbeg + nv) return;
+  const float r = ratio[t], d = st.mass[t] * expf(st.zt[e] - st.lse[t]) - st.p[e];
   *dz_at(dz, zstep, t, v - vbeg) = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
 }
 
@@ -800,11 +850,11 @@ struct DhJob {
     int64_t c0, t0;
     int split;
     place(p, lin, c0, t0, split);
-    A = GOperand{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, p.nv, nullptr};
-    B = GOperand{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
     k = split * p.span;
-    const int64_t n = p.nv - k < p.span ? p.nv - k : p.span;   // > 0 for every split of a launch
-    nch = (int)((n + G_K - 1) / G_K);
+    const int64_t end = p.nv < k + p.span ? p.nv : k + p.span;   // > k for every split of a launch
+    A = GOperand{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, end, nullptr};
+    B = GOperand{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
+    nch = (int)((end - k + G_K - 1) / G_K);
   }
   __device__ __forceinline__ void side(int, char*) const {}
   __device__ __forceinline__ void finish(int lin, char*, GAcc& acc) const {
@@ -828,13 +878,13 @@ __global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs) {
   g_run<T8, G_KS, G_KC_BLOCKED>(smem, DhJob());
 }
 
-// dh = fac * (P[0] + P[1] + ...), rounded once; 4 channels a thread
+// dh = factor * (P[0] + P[1] + ...), rounded once; 4 channels a thread
 template <typename T8>
 __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int ns, int64_t T,
-                                                int64_t C, const float* __restrict__ fac,
-                                                uint16_t* dh, int64_t ldd) {
+                                                int64_t C, Factor fac, uint16_t* dh,
+                                                int64_t ldd) {
   const int64_t n4 = T * (C / 4);
-  const float f = fac[0];
+  const float f = fac.get();
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n4; e += (int64_t)gridDim.x * 256) {
     float4 v = *(const float4*)(P + e * 4);
     for (int s = 1; s < ns; ++s) {
@@ -848,13 +898,13 @@ __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int
   }
 }
 
-// dW[v][c] = fac * sum_t dz[t][v] h[t][c] of a piece's rows v
+// dW[v][c] = factor * sum_t dz[t][v] h[t][c] of a piece's rows v
 struct DwArgs {
   const uint16_t *h, *dz;
   int64_t ldh, zstep, T, nv, C;
   const uint64_t* live;
   int nm, nn;
-  const float* fac;
+  Factor fac;
   uint16_t* dW;
   int64_t ldo;
 };
@@ -893,7 +943,7 @@ struct DwJob {
     const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
     place(p, lin, c0, v0);
-    const float f = p.fac[0];
+    const float f = p.fac.get();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     g_each<4>([&](auto jj) __attribute__((always_inline)) {
       constexpr int j = decltype(jj)::value;
@@ -951,15 +1001,23 @@ static int64_t piece_of(int64_t T, int64_t V) {
   const int64_t all = cdiv(V, 256) * 256;
   return p < all ? p : all;
 }
-// Parts that dh's sum over a piece is split into, to fill 256 CUs.
+// Parts that dh's sums over a piece are split into: the fewest rounds of 256
+// workgroups times the 64-k stages of a part (1.2 us each, 6 more a tile), and
+// the fp32 partial sums, written and read back at about 4 TB/s.
 static int dh_splits(int64_t T, int64_t C, int64_t piece) {
   static const int bn[3] = {16, 64, 256};
-  const int64_t tiles = cdiv(C, 256) * cdiv(T, bn[token_tile(T)]);
-  int64_t s = 512 / tiles;
-  const int64_t most = piece / 512;                    // 8 stages each at least
-  if (s > most) s = most;
-  if (s > 32) s = 32;
-  return (int)(s < 1 ? 1 : s);
+  const int64_t tiles = cdiv(C, 256) * cdiv(T, bn[token_tile(T)]), stages = cdiv(piece, G_K);
+  int64_t best = 1;
+  double least = 0.;
+  for (int64_t s = 1; s <= 256 && s * 4 <= stages; ++s) {
+    const double t = (double)cdiv(tiles * s, 256) * ((double)cdiv(stages, s) * 1.2 + 6.) +
+                     2e-6 * (double)(T * C) * (double)s;
+    if (s == 1 || t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return (int)best;
 }
 
 struct FwdWs {
@@ -983,7 +1041,7 @@ struct GradWs {
   int64_t piece, span;
   int ns;                  // splits of dh's sums over the first (largest) piece
   uint16_t* dz;
-  float *P, *a2, *rowb, *ratio, *fac, *gmax;
+  float *P, *rowb, *ratio, *gmax;
   uint64_t* live;
   size_t bytes;
   GradWs(void* ws, size_t cap, int64_t T, int64_t V, int64_t C, bool& ok) {
@@ -993,10 +1051,8 @@ struct GradWs {
     ns = (int)cdiv(piece < V ? piece : V, span);
     dz = w.take<uint16_t>((size_t)(dz_rows(T) * piece));
     P = w.take<float>((size_t)(T * C) * ns);
-    a2 = w.take<float>((size_t)T);
     rowb = w.take<float>((size_t)T);
     ratio = w.take<float>((size_t)T);
-    fac = w.take<float>(1);
     gmax = w.take<float>(1);
     live = w.take<uint64_t>((size_t)cdiv(T, 64));
     bytes = w.off;
@@ -1048,49 +1104,70 @@ static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int6
   }
   CRBQ_LAUNCH_CHECK();
   float* rows = reduction ? w.rows : loss;
-  k_head_join<XENT><<<(unsigned)cdiv(T, 4), 256, 0, s>>>(w.part, n_part(T, V), T, V, ls.k,
-                                                         ls.labels, ignore, st, rows,
-                                                         reduction ? w.live : nullptr, reduction);
+  uint8_t* live = reduction ? w.live : nullptr;
+  // 4 wavefronts a row up to 4 rows a CU
+  if (T <= 1024)
+    k_head_join<XENT, 4><<<(unsigned)T, 256, 0, s>>>(w.part, n_part(T, V), T, V, ls.k, ls.labels,
+                                                     ignore, st, dz_scale<T8>(), rows, live);
+  else
+    k_head_join<XENT, 1><<<(unsigned)cdiv(T, 4), 256, 0, s>>>(
+        w.part, n_part(T, V), T, V, ls.k, ls.labels, ignore, st, dz_scale<T8>(), rows, live);
   CRBQ_LAUNCH_CHECK();
   if (reduction) {
-    k_head_reduce<<<1, 1024, 0, s>>>(w.rows, w.live, T, reduction == CRBQ_MEAN, loss, st.inv);
+    k_head_reduce<<<1, 1024, 0, s>>>(w.rows, w.live, T, reduction == CRBQ_MEAN, loss, st);
     CRBQ_LAUNCH_CHECK();
   }
   return CRBQ_OK;
 }
 
-template <typename T8, typename GZ, typename GH, bool XENT>
-static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw, int64_t T,
-                     int64_t V, int64_t C, const int64_t* labels, int64_t ignore, int k,
-                     float scale, const State& st, const float* g, int per_row, uint16_t* dh,
-                     int64_t ldd, uint16_t* dW, int64_t ldo, const GradWs& w, hipStream_t s) {
-  if (per_row) {
-    k_absmax<<<1, 1024, 0, s>>>(g, T, w.gmax);
+struct GradCall {
+  const uint16_t *h, *W;
+  int64_t ldh, ldw, T, V, C;
+  const int64_t* labels;   // cross entropy; else null
+  int k;
+  float scale;
+  const float* g;
+  bool per_row;
+  uint16_t *dh, *dW;
+  int64_t ldd, ldo;
+};
+
+template <typename T8, typename GZ, typename GH>
+static int head_grad(const GradCall& c, const State& st, const GradWs& w, hipStream_t s) {
+  const int64_t T = c.T, V = c.V, C = c.C;
+  const float *rowb = st.rowb, *ratio = st.ratio;
+  const uint64_t* live = st.live;
+  if (c.per_row) {
+    k_absmax<<<1, 1024, 0, s>>>(c.g, T, w.gmax);
     CRBQ_LAUNCH_CHECK();
+    k_grad_rows<<<(unsigned)cdiv(T, 64), 64, 0, s>>>(st, T, c.g, w.gmax, w.rowb, w.ratio, w.live);
+    CRBQ_LAUNCH_CHECK();
+    rowb = w.rowb;
+    ratio = w.ratio;
+    live = w.live;
   }
-  const float zs = dz_scale<T8>();
-  k_grad_rows<XENT><<<(unsigned)cdiv(T, 64), 64, 0, s>>>(st, T, k, labels, ignore, g, per_row,
-                                                         w.gmax, zs, scale, w.a2, w.rowb, w.ratio,
-                                                         w.live, w.fac);
-  CRBQ_LAUNCH_CHECK();
+  const Factor fac{c.per_row ? w.gmax : c.g, st.inv, c.scale / dz_scale<T8>()};
   const int nt = (int)cdiv(T, GZ::BN);
   const int64_t zstep = dz_rows(T) * G_K;
   for (int64_t v = 0; v < V; v += w.piece) {
     const int64_t nv = V - v < w.piece ? V - v : w.piece;
-    const uint16_t* Wv = W + v * ldw;
+    const uint16_t* Wv = c.W + v * c.ldw;
     const int nm = (int)cdiv(nv, GZ::BM);
-    const DzArgs z{h, Wv, ldh, ldw, T, nv, C, scale, w.a2, w.rowb, nm, nt, w.dz, zstep};
+    const DzArgs z{c.h, Wv, c.ldh, c.ldw, T, nv, C, c.scale, st.a, rowb, c.labels, v, nm, nt, w.dz,
+                   zstep};
     if constexpr (std::is_same<GZ, Big>::value)
       k_head_dz_p<T8><<<persistent((int64_t)nm * nt), G_THREADS, 0, s>>>(z);
     else
       k_head_dz<T8, GZ><<<(unsigned)((int64_t)nm * nt), GZ::THREADS, 0, s>>>(z);
     CRBQ_LAUNCH_CHECK();
-    k_dz_listed<T8, XENT><<<(unsigned)cdiv(XENT ? T : T * k, 256), 256, 0, s>>>(
-        st, T, k, labels, w.ratio, v, nv, w.dz, zstep);
-    CRBQ_LAUNCH_CHECK();
-    if (dh) {
+    if (!c.labels) {
+      k_dz_listed<T8><<<(unsigned)cdiv(T * c.k, 256), 256, 0, s>>>(st, T, c.k, ratio, v, nv, w.dz,
+                                                                   zstep);
+      CRBQ_LAUNCH_CHECK();
+    }
+    if (c.dh) {
       const int mh = (int)cdiv(C, GH::BM);
-      const DhArgs q{Wv, w.dz, ldw, zstep, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
+      const DhArgs q{Wv, w.dz, c.ldw, zstep, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
                      v > 0};
       const int64_t tiles = (int64_t)mh * nt * q.ns;
       if constexpr (std::is_same<GH, Big>::value)
@@ -1099,42 +1176,32 @@ static int head_grad(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t 
         k_head_dh<T8, GH><<<(unsigned)tiles, GH::THREADS, 0, s>>>(q);
       CRBQ_LAUNCH_CHECK();
     }
-    if (dW) {
+    if (c.dW) {
       const int mw = (int)cdiv(C, 256), nw = (int)cdiv(nv, 256);
       k_head_dw<T8><<<persistent((int64_t)mw * nw), G_THREADS, 0, s>>>(
-          DwArgs{h, w.dz, ldh, zstep, T, nv, C, w.live, mw, nw, w.fac, dW + v * ldo, ldo});
+          DwArgs{c.h, w.dz, c.ldh, zstep, T, nv, C, live, mw, nw, fac, c.dW + v * c.ldo, c.ldo});
       CRBQ_LAUNCH_CHECK();
     }
   }
-  if (dh) {
+  if (c.dh) {
     const int64_t nb = cdiv(T * (C / 4), 256);
-    k_dh_out<T8><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, s>>>(w.P, w.ns, T, C, w.fac, dh,
-                                                                   ldd);
+    k_dh_out<T8><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, s>>>(w.P, w.ns, T, C, fac, c.dh,
+                                                                   c.ldd);
     CRBQ_LAUNCH_CHECK();
   }
   return CRBQ_OK;
 }
 
-template <typename T8, bool XENT>
-static int head_grad_t(const void* h, int64_t ldh, const void* W, int64_t ldw, int64_t T,
-                       int64_t V, int64_t C, const int64_t* labels, int64_t ignore, int k,
-                       float scale, const State& st, const float* g, int per_row, void* dh,
-                       int64_t ldd, void* dW, int64_t ldo, const GradWs& w, hipStream_t s) {
-  const uint16_t *hh = (const uint16_t*)h, *ww = (const uint16_t*)W;
-  uint16_t *oh = (uint16_t*)dh, *ow = (uint16_t*)dW;
-  switch (token_tile(T)) {
-    case 0:
-      return head_grad<T8, ZS, HS, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
-                                         g, per_row, oh, ldd, ow, ldo, w, s);
-    case 1:
-      return head_grad<T8, ZM, HM, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
-                                         g, per_row, oh, ldd, ow, ldo, w, s);
-    default:
-      return head_grad<T8, Big, Big, XENT>(hh, ldh, ww, ldw, T, V, C, labels, ignore, k, scale, st,
-                                         g, per_row, oh, ldd, ow, ldo, w, s);
+template <typename T8>
+static int head_grad_t(const GradCall& c, const State& st, const GradWs& w, hipStream_t s) {
+  switch (token_tile(c.T)) {
+    case 0: return head_grad<T8, ZS, HS>(c, st, w, s);
+    case 1: return head_grad<T8, ZM, HM>(c, st, w, s);
+    default: return head_grad<T8, Big, Big>(c, st, w, s);
   }
 }
 
+static bool bad_state(const void* p) { return !p || (((uintptr_t)p) & 7); }
 static bool bad_reduction(int r) { return r != CRBQ_NONE && r != CRBQ_MEAN && r != CRBQ_SUM; }
 
 }  // namespace crbq
@@ -1143,7 +1210,7 @@ using namespace crbq;
 
 extern "C" size_t crbq_head_state_floats(int64_t T, int64_t k) {
   if (T < 1 || k < 0 || k > CRBQ_HEAD_MAX_K) return 0;
-  return (size_t)(k ? (3 * k + 5) * T + 2 : 3 * T + 2);
+  return (size_t)State::floats(T, k);
 }
 
 extern "C" size_t crbq_head_workspace_size(int64_t T, int64_t V, int64_t C, int64_t k, int grad) {
@@ -1157,7 +1224,7 @@ extern "C" int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t
                               int64_t ignore_index, float scale, int reduction, float* loss,
                               float* state, void* ws, size_t ws_bytes, void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!labels || !loss || !state || bad_reduction(reduction)) return CRBQ_ERR_ARG;
+  if (!labels || !loss || bad_state(state) || bad_reduction(reduction)) return CRBQ_ERR_ARG;
   bool ok;
   const FwdWs w(ws, ws_bytes, T, V, 0, ok);
   if (!ok) return CRBQ_ERR_WORKSPACE;
@@ -1173,23 +1240,22 @@ extern "C" int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t
 
 extern "C" int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
                                    int dtype, int64_t T, int64_t V, int64_t C,
-                                   const int64_t* labels, int64_t ignore_index, float scale,
-                                   const float* state, const float* g, int g_per_row, void* dh,
-                                   int64_t ldd, void* dW, int64_t ldo, void* ws, size_t ws_bytes,
+                                   const int64_t* labels, float scale, int reduction,
+                                   const float* state, const float* g, void* dh, int64_t ldd,
+                                   void* dW, int64_t ldo, void* ws, size_t ws_bytes,
                                    void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!labels || !state || !g || (!dh && !dW)) return CRBQ_ERR_ARG;
+  if (!labels || bad_state(state) || !g || (!dh && !dW) || bad_reduction(reduction))
+    return CRBQ_ERR_ARG;
   if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
   bool ok;
   const GradWs w(ws, ws_bytes, T, V, C, ok);
   if (!ok) return CRBQ_ERR_WORKSPACE;
   const State st((float*)state, T, 0);
+  const GradCall c{(const uint16_t*)h, (const uint16_t*)W, ldh, ldw, T, V, C, labels, 0, scale, g,
+                   reduction == CRBQ_NONE, (uint16_t*)dh, (uint16_t*)dW, ldd, ldo};
   hipStream_t s = (hipStream_t)stream;
-  return dtype == CRBQ_F16
-             ? head_grad_t<h8_t, true>(h, ldh, W, ldw, T, V, C, labels, ignore_index, 1, scale, st,
-                                       g, g_per_row, dh, ldd, dW, ldo, w, s)
-             : head_grad_t<b8_t, true>(h, ldh, W, ldw, T, V, C, labels, ignore_index, 1, scale, st,
-                                       g, g_per_row, dh, ldd, dW, ldo, w, s);
+  return dtype == CRBQ_F16 ? head_grad_t<h8_t>(c, st, w, s) : head_grad_t<b8_t>(c, st, w, s);
 }
 
 extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int64_t ldw,
@@ -1199,7 +1265,7 @@ extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int6
                                  int reduction, float* loss, float* state, void* ws,
                                  size_t ws_bytes, void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!top_val || !top_idx || !loss || !state || bad_reduction(reduction) || k < 1 ||
+  if (!top_val || !top_idx || !loss || bad_state(state) || bad_reduction(reduction) || k < 1 ||
       k > CRBQ_HEAD_MAX_K || ldv < k || ldi < k || !(temperature > 0.f))
     return CRBQ_ERR_ARG;
   if (val_dtype != CRBQ_F32 && val_dtype != CRBQ_F16 && val_dtype != CRBQ_BF16)
@@ -1209,10 +1275,7 @@ extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int6
   if (!ok) return CRBQ_ERR_WORKSPACE;
   const State st(state, T, k);
   hipStream_t s = (hipStream_t)stream;
-  const int64_t ldm = mask_words(V), nw = T * ldm;
-  k_fill_u32<<<(unsigned)(cdiv(nw, 1024) < 2048 ? cdiv(nw, 1024) : 2048), 256, 0, s>>>(w.mask, nw,
-                                                                                       0u);
-  CRBQ_LAUNCH_CHECK();
+  const int64_t ldm = mask_words(V);
   const float it = 1.f / temperature;
   if (val_dtype == CRBQ_F32)
     k_list<float><<<(unsigned)T, 64, 0, s>>>((const float*)top_val, ldv, top_idx, ldi, top_lse, it,
@@ -1233,23 +1296,22 @@ extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int6
 
 extern "C" int crbq_head_distill_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
                                       int dtype, int64_t T, int64_t V, int64_t C, int k,
-                                      float scale, float temperature, const float* state,
-                                      const float* g, int g_per_row, void* dh, int64_t ldd,
+                                      float scale, float temperature, int reduction,
+                                      const float* state, const float* g, void* dh, int64_t ldd,
                                       void* dW, int64_t ldo, void* ws, size_t ws_bytes,
                                       void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!state || !g || (!dh && !dW) || k < 1 || k > CRBQ_HEAD_MAX_K || !(temperature > 0.f))
+  if (bad_state(state) || !g || (!dh && !dW) || k < 1 || k > CRBQ_HEAD_MAX_K ||
+      !(temperature > 0.f) || bad_reduction(reduction))
     return CRBQ_ERR_ARG;
   if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
   bool ok;
   const GradWs w(ws, ws_bytes, T, V, C, ok);
   if (!ok) return CRBQ_ERR_WORKSPACE;
   const State st((float*)state, T, k);
+  const GradCall c{(const uint16_t*)h, (const uint16_t*)W, ldh, ldw, T, V, C, nullptr, k,
+                   scale * (1.f / temperature), g, reduction == CRBQ_NONE, (uint16_t*)dh,
+                   (uint16_t*)dW, ldd, ldo};
   hipStream_t s = (hipStream_t)stream;
-  const float sc = scale * (1.f / temperature);
-  return dtype == CRBQ_F16
-             ? head_grad_t<h8_t, false>(h, ldh, W, ldw, T, V, C, nullptr, 0, k, sc, st, g,
-                                        g_per_row, dh, ldd, dW, ldo, w, s)
-             : head_grad_t<b8_t, false>(h, ldh, W, ldw, T, V, C, nullptr, 0, k, sc, st, g,
-                                        g_per_row, dh, ldd, dW, ldo, w, s);
+  return dtype == CRBQ_F16 ? head_grad_t<h8_t>(c, st, w, s) : head_grad_t<b8_t>(c, st, w, s);
 }

@@ -2,14 +2,17 @@
 // index) and the row's log-sum-exp: what a teacher leaves behind for
 // distillation instead of its logits.
 //
-// One workgroup of 1024 threads a row.  A first pass takes each thread's
-// largest logit; the k-th largest of these 1024 is a lower bound of the
-// row's k-th largest logit that only about k elements reach (with k of 1024
-// threads hit, -1024 log(1 - k / 1024) elements: 137 for k = 128).  A second
-// pass sums the exponentials against the row's maximum and collects the
-// elements at or above the bound, which are then ranked by counting.  Rows
-// whose ties leave more candidates than the list holds (a constant row, a
-// row masked to one value) are selected exactly, by digits of the key.
+// One workgroup of 1024 threads a row.  One pass over the row takes each
+// thread's largest logit and its sum of exponentials against that (rescaled
+// the few times the largest one rises): 8.5 vector instructions' time an
+// element, below the time its bytes take.  The k-th largest of
+// the 1024 maxima is a lower bound of the row's k-th largest logit that only about
+// k elements reach (with k of 1024 threads hit, -1024 log(1 - k / 1024)
+// elements: 137 for k = 128); the threads whose maximum reaches it read their
+// elements again and collect those that do, which are then ranked by
+// counting.  Rows whose ties leave more candidates than the list holds (a
+// constant row, a row masked to one value) and rows with a NaN are selected
+// exactly, by digits of the key.
 // Logits are compared as whole numbers in the order of the values (-0 as
 // +0, NaN above everything); the values written are the logits themselves.
 #include "common.h"
@@ -26,6 +29,7 @@ template <> struct TL<float> {
   typedef uint32_t bits;
   static constexpr int DIGITS = 4;
   __device__ static float f(uint32_t b) { return __builtin_bit_cast(float, b); }
+  __device__ static uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
   __device__ static uint32_t key(uint32_t b) {
     if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
     if (b == 0x80000000u) b = 0;
@@ -44,38 +48,65 @@ struct TL16 {
 };
 template <> struct TL<_Float16> : TL16<0x7c00> {
   __device__ static float f(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
+  __device__ static uint32_t bits_of(float x) {       // x is one of the logits
+    return __builtin_bit_cast(uint16_t, (_Float16)x);
+  }
 };
 template <> struct TL<__bf16> : TL16<0x7f80> {
   __device__ static float f(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
+  __device__ static uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x) >> 16; }
 };
 
-// f(index, bits) for every element of the row: 16-byte loads from the first
-// 16-byte boundary on (long rows), elements one by one before and behind.
-template <typename E, typename F>
-__device__ __forceinline__ void tl_each(const typename TL<E>::bits* __restrict__ x, int64_t V,
-                                        F&& f) {
+// A row as the threads share it: 16-byte groups from the first 16-byte boundary
+// on (long rows), elements one by one before and behind.
+template <typename E>
+struct TLRow {
   typedef typename TL<E>::bits B;
-  constexpr int N = 16 / sizeof(B);
-  const int tid = threadIdx.x;
-  if (V <= TL_SCALAR) {
-    for (int64_t i = tid; i < V; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
-    return;
+  static constexpr int N = 16 / sizeof(B);
+  const B* x;
+  int64_t V, nv;
+  int head;
+  const uint4* q;
+  __device__ TLRow(const B* row, int64_t V_) : x(row), V(V_) {
+    head = V <= TL_SCALAR ? (int)V : (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(B));
+    nv = (V - head) / N;
+    q = (const uint4*)(x + head);
   }
-  const int head = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(B));
-  const int64_t nv = (V - head) / N;
-  const uint4* __restrict__ q = (const uint4*)(x + head);
-  for (int64_t i = tid; i < nv; i += TL_THREADS) {
-    const uint4 u = q[i];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __device__ static uint32_t bits(const uint4& u, int e) {
+    const uint32_t w = e * sizeof(B) / 4 == 0 ? u.x : e * sizeof(B) / 4 == 1 ? u.y
+                     : e * sizeof(B) / 4 == 2 ? u.z : u.w;
+    return N == 4 ? w : (w >> (16 * (e & 1))) & 0xffffu;
+  }
+  // f(index, bits) for this thread's elements
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int tid = threadIdx.x;
+    for (int64_t i = tid; i < nv; i += TL_THREADS) {
+      const uint4 u = q[i];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const uint32_t b = N == 4 ? w[e] : (w[e / 2] >> (16 * (e & 1))) & 0xffffu;
-      f((int)(head + i * N + e), b);
+      for (int e = 0; e < N; ++e) f((int)(head + i * N + e), bits(u, e));
+    }
+    for (int64_t i = tid; i < head; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
+    for (int64_t i = head + nv * N + tid; i < V; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
+  }
+};
+
+// A thread's largest logit m and s = sum of 2^(c (x - m)) (against 0 where m is
+// infinite; a NaN makes s one).
+struct TLSum {
+  float m = -INFINITY, s = 0.f, ref = 0.f;
+  __device__ __forceinline__ void rise(float top, float c) {
+    if (top > m) {
+      const float r = fabsf(top) < INFINITY ? top : 0.f;
+      s = m == -INFINITY ? s : s * __builtin_amdgcn_exp2f((ref - r) * c);
+      m = top;
+      ref = r;
     }
   }
-  if (tid < head) f(tid, (uint32_t)x[tid]);
-  for (int64_t i = head + nv * N + tid; i < V; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
-}
+  __device__ __forceinline__ void add(float x, float c) {
+    s += __builtin_amdgcn_exp2f((x - ref) * c);        // (x * c may be beyond fp32)
+  }
+};
 
 template <typename E>
 __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, int64_t V,
@@ -86,35 +117,66 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
   typedef typename L::bits B;
   __shared__ uint32_t tmax[TL_THREADS];
   __shared__ uint64_t cand[TL_CAP];     // key << 32 | ~index: larger is earlier
-  __shared__ float wred[TL_WAVES];
+  __shared__ float wred[TL_WAVES], wsum[TL_WAVES];
   __shared__ int hist[256];
   __shared__ uint32_t sh[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t t = blockIdx.x;
   const B* x = (const B*)logits + t * ld;
 
-  uint32_t best = 0;
-  tl_each<E>(x, V, [&](int, uint32_t b) {
-    const uint32_t q = L::key(b);
-    best = q > best ? q : best;
-  });
+  const TLRow<E> row(x, V);
+  constexpr int N = TLRow<E>::N;
+  const float c = itemp * 1.4426950408889634f;
+  TLSum acc;
+  auto group = [&](const uint4& u) __attribute__((always_inline)) {
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = L::f(TLRow<E>::bits(u, e));
+    float top = v[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
+    acc.rise(top, c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc.add(v[e], c);
+  };
+  int64_t g = tid;
+  for (; g + 3 * TL_THREADS < row.nv; g += 4 * TL_THREADS) {
+    uint4 u[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) u[d] = row.q[g + d * TL_THREADS];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) group(u[d]);
+  }
+  for (; g < row.nv; g += TL_THREADS) group(row.q[g]);
+  auto one = [&](int64_t i) __attribute__((always_inline)) {
+    const float v = L::f((uint32_t)x[i]);
+    acc.rise(v, c);
+    acc.add(v, c);
+  };
+  for (int64_t i = tid; i < row.head; i += TL_THREADS) one(i);
+  for (int64_t i = row.head + row.nv * N + tid; i < V; i += TL_THREADS) one(i);
+  const bool some = V >= TL_THREADS || tid < V;        // threads without an element: key 0
+  const uint32_t best = some ? L::key(L::bits_of(acc.m)) : 0;
   tmax[tid] = best;
   if (tid == 0) sh[1] = 0;
+  // the row's maximum, and its sum of exponentials against it
+  float top = acc.m;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) wred[wave] = top;
   __syncthreads();
-  // k-th largest of the 1024, by its bits from the top; every wavefront for itself
-  uint32_t mine[TL_WAVES], top = 0;
-#pragma unroll
-  for (int w = 0; w < TL_WAVES; ++w) {
-    mine[w] = tmax[w * 64 + lane];
-    top = mine[w] > top ? mine[w] : top;
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t o = __shfl_xor(top, d);
-    top = o > top ? o : top;
-  }
+  for (int w = 0; w < TL_WAVES; ++w) top = fmaxf(top, wred[w]);
+  const float ref = fabsf(top) < INFINITY ? top : 0.f;
+  // (-inf: s is 0 or NaN; below an infinite maximum only NaN matters)
+  const float part = acc.m == -INFINITY || !(fabsf(top) < INFINITY)
+                         ? acc.s : acc.s * __builtin_amdgcn_exp2f((acc.ref - ref) * c);
+  const float sum = wave_sum_f(part);
+  if (lane == 0) wsum[wave] = sum;
+  // k-th largest of the 1024, by its bits from the top
   if (wave == 0) {
-    uint32_t thr = 0;
+    uint32_t mine[TL_WAVES], thr = 0;
+#pragma unroll
+    for (int w = 0; w < TL_WAVES; ++w) mine[w] = tmax[w * 64 + lane];
 #pragma unroll 1
     for (int bit = L::DIGITS * 8 - 1; bit >= 0; --bit) {
       const uint32_t c = thr | (1u << bit);
@@ -127,32 +189,22 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
   }
   __syncthreads();
   const uint32_t thr = sh[0];
-  // the row's maximum as a float (NaN and infinities: reference 0)
-  const uint32_t tb = top >> (L::DIGITS * 8 - 1) ? top & ~(1u << (L::DIGITS * 8 - 1))
-                                                 : ~top & (L::DIGITS == 4 ? 0xffffffffu : 0xffffu);
-  float m = L::f(tb) * itemp;
-  if (!(fabsf(m) < INFINITY)) m = 0.f;
-
   float s = 0.f;
-  tl_each<E>(x, V, [&](int i, uint32_t b) {
-    s += __expf(L::f(b) * itemp - m);
-    const uint32_t q = L::key(b);
-    if (q >= thr) {
-      const uint32_t at = atomicAdd(&sh[1], 1u);
-      if (at < TL_CAP) cand[at] = (uint64_t)q << 32 | (uint32_t)~i;
-    }
-  });
-  s = wave_sum_f(s);
-  if (lane == 0) wred[wave] = s;
+  for (int w = 0; w < TL_WAVES; ++w) s += wsum[w];
+  const bool nan = !(s == s);
+  if (tid == 0) lse[t] = nan || fabsf(top) < INFINITY ? ref * itemp + logf(s) : top;
+  if (best >= thr && !nan)
+    row.each([&](int i, uint32_t b) __attribute__((always_inline)) {
+      const uint32_t q = L::key(b);
+      if (q >= thr) {
+        const uint32_t at = atomicAdd(&sh[1], 1u);
+        if (at < TL_CAP) cand[at] = (uint64_t)q << 32 | (uint32_t)~i;
+      }
+    });
   __syncthreads();
-  if (tid == 0) {
-    s = 0.f;
-    for (int w = 0; w < TL_WAVES; ++w) s += wred[w];
-    lse[t] = m + logf(s);
-  }
   int n = (int)sh[1];
-  if (n > TL_CAP) {
-    // too many candidates: the k-th key digit by digit, then the elements
+  if (n > TL_CAP || nan) {
+    // too many candidates, or NaN: the k-th key digit by digit, then the elements
     // above it and the first of its equals
     uint32_t pre = 0;
     int need = k;                       // of the elements whose upper digits are pre
@@ -160,7 +212,7 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
       __syncthreads();
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
-      tl_each<E>(x, V, [&](int, uint32_t b) {
+      row.each([&](int, uint32_t b) {
         const uint32_t q = L::key(b);
         const bool in = d == L::DIGITS - 1 || (q >> (8 * d + 8)) == pre;
         const int dig = (int)((q >> (8 * d)) & 255);
@@ -186,7 +238,7 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
     __syncthreads();
     if (tid == 0) sh[1] = 0;
     __syncthreads();
-    tl_each<E>(x, V, [&](int i, uint32_t b) {
+    row.each([&](int i, uint32_t b) {
       const uint32_t q = L::key(b);
       if (q > pre) cand[atomicAdd(&sh[1], 1u)] = (uint64_t)q << 32 | (uint32_t)~i;   // below k
     });

@@ -33,7 +33,7 @@ class _LinearXent(torch.autograd.Function):
     def forward(ctx, h, weight, labels, scale, ignore_index, reduction):
         loss, state = kernels.head_xent(h, weight, labels, scale, ignore_index, reduction)
         ctx.save_for_backward(h, weight, labels, state)
-        ctx.conf = scale, ignore_index
+        ctx.conf = scale, reduction
         return loss
 
     @staticmethod
@@ -52,7 +52,7 @@ class _LinearDistill(torch.autograd.Function):
         loss, state = kernels.head_distill(h, weight, val, idx, lse, scale, temperature,
                                            reduction)
         ctx.save_for_backward(h, weight, state)
-        ctx.conf = scale, temperature
+        ctx.conf = scale, temperature, reduction
         ctx.k = val.shape[1]
         return loss
 

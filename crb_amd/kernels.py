@@ -604,13 +604,16 @@ def head_xent(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, scale: flo
     return loss, state
 
 
-def _grad_args(what, hp, Wp, state, g, need_h, need_w, lib):
+def _grad_args(what, hp, Wp, state, k, g, red, need_h, need_w, lib):
     """Output buffers (padded like their inputs), workspace and g of a gradient call."""
     _one_gpu(what, hp, state, g)
     if not (need_h or need_w):
         raise _lib.CrbqError(f"{what}: no gradient asked for")
-    if g.dtype != torch.float32 or g.dim() > 1 or (g.dim() == 1 and g.shape != hp.shape[:1]):
-        raise _lib.CrbqError(f"{what} takes an fp32 loss gradient, one number or [T]")
+    if g.dtype != torch.float32 or g.shape != (hp.shape[:1] if red == 0 else ()):
+        raise _lib.CrbqError(f"{what} takes the loss's gradient, fp32 and of its shape")
+    if (state.dtype != torch.float32 or not state.is_contiguous()
+            or state.numel() != lib.crbq_head_state_floats(hp.shape[0], k)):
+        raise _lib.CrbqError(f"{what}: not the state of this call's forward")
     dh = torch.empty_like(hp, memory_format=torch.contiguous_format) if need_h else None
     dW = torch.empty_like(Wp, memory_format=torch.contiguous_format) if need_w else None
     T, C = hp.shape
@@ -628,21 +631,25 @@ def _cut(x, C):
 
 
 def head_xent_grad(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, state: torch.Tensor,
-                   g: torch.Tensor, scale: float = 1.0, ignore_index: int = -100,
+                   g: torch.Tensor, scale: float = 1.0, reduction: str = "mean",
                    need_h: bool = True, need_w: bool = True):
-    """(dh, dW) (None where not asked for) of head_xent's loss times g: one
-    fp32 number, or [T] for reduction "none"."""
+    """(dh, dW) (None where not asked for) of head_xent's loss, called with the
+    same scale and reduction, times g (fp32, of the loss's shape)."""
     hp, Wp = _head_pair("head_xent_grad", h, W)
+    _one_gpu("head_xent_grad", h, labels)
+    if labels.dtype != torch.int64 or labels.shape != h.shape[:1]:
+        raise _lib.CrbqError("head_xent_grad takes int64 labels [T]")
+    red = _reduction("head_xent_grad", reduction)
     lib = _lib.ready(h.device)
     labels = labels.contiguous()
     with _lib.on_device(h.device):
-        dh, dW, ws, nws, g = _grad_args("head_xent_grad", hp, Wp, state, g, need_h, need_w, lib)
+        dh, dW, ws, nws, g = _grad_args("head_xent_grad", hp, Wp, state, 0, g, red, need_h,
+                                        need_w, lib)
         check(lib.crbq_head_xent_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
                                       _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0], hp.shape[1],
-                                      labels.data_ptr(), int(ignore_index), float(scale),
-                                      state.data_ptr(), g.data_ptr(), int(g.dim() == 1),
-                                      *_out_args(dh, dW), ws.data_ptr(), nws, stream_of(h)),
-              "crbq_head_xent_grad")
+                                      labels.data_ptr(), float(scale), red, state.data_ptr(),
+                                      g.data_ptr(), *_out_args(dh, dW), ws.data_ptr(), nws,
+                                      stream_of(h)), "crbq_head_xent_grad")
     return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])
 
 
@@ -686,17 +693,20 @@ def head_distill(h: torch.Tensor, W: torch.Tensor, top_val: torch.Tensor, top_id
 
 def head_distill_grad(h: torch.Tensor, W: torch.Tensor, k: int, state: torch.Tensor,
                       g: torch.Tensor, scale: float = 1.0, temperature: float = 1.0,
-                      need_h: bool = True, need_w: bool = True):
-    """(dh, dW) (None where not asked for) of head_distill's loss times g."""
+                      reduction: str = "mean", need_h: bool = True, need_w: bool = True):
+    """(dh, dW) (None where not asked for) of head_distill's loss, called with
+    k listed tokens and the same scale, temperature and reduction, times g
+    (fp32, of the loss's shape)."""
     hp, Wp = _head_pair("head_distill_grad", h, W)
+    red = _reduction("head_distill_grad", reduction)
     lib = _lib.ready(h.device)
     with _lib.on_device(h.device):
-        dh, dW, ws, nws, g = _grad_args("head_distill_grad", hp, Wp, state, g, need_h, need_w,
-                                        lib)
+        dh, dW, ws, nws, g = _grad_args("head_distill_grad", hp, Wp, state, k, g, red, need_h,
+                                        need_w, lib)
         check(lib.crbq_head_distill_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
                                          _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0],
                                          hp.shape[1], int(k), float(scale), float(temperature),
-                                         state.data_ptr(), g.data_ptr(), int(g.dim() == 1),
+                                         red, state.data_ptr(), g.data_ptr(),
                                          *_out_args(dh, dW), ws.data_ptr(), nws, stream_of(h)),
               "crbq_head_distill_grad")
     return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])

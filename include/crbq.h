@@ -376,9 +376,10 @@ int crbq_linear_packed(const uint8_t* codes, int64_t ldc, const void* lut, const
  * reduction: CRBQ_NONE: loss [T]; CRBQ_SUM, CRBQ_MEAN: loss [1], the sum
  *   over rows or the mean over the rows not left out (over none: NaN).
  * state: crbq_head_state_floats(T, k) floats (k = 0: cross entropy), what
- *   the gradients need of the forward; the caller keeps it.
- * *_grad: gradients of the same call's loss times g (g_per_row 0: *g one
- *   number; 1: g[t] per row, for CRBQ_NONE) to h (dh [T][ldd]) and W
+ *   the gradients need of the forward; the caller keeps it
+ *   (8-byte aligned).
+ * *_grad: gradients of the same call's loss (with its reduction) times g (one
+ *   number; with CRBQ_NONE one per row) to h (dh [T][ldd]) and W
  *   (dW [V][ldo]) in the inputs' dtype; either may be NULL.  The logits are
  *   computed again; sums are fp32, in a fixed order.  A left-out row of h
  *   is not read into dW.
@@ -392,10 +393,10 @@ int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t ldw, int d
                    float scale, int reduction, float* loss, float* state, void* ws,
                    size_t ws_bytes, void* stream);
 int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
-                        int64_t T, int64_t V, int64_t C, const int64_t* labels,
-                        int64_t ignore_index, float scale, const float* state, const float* g,
-                        int g_per_row, void* dh, int64_t ldd, void* dW, int64_t ldo, void* ws,
-                        size_t ws_bytes, void* stream);
+                        int64_t T, int64_t V, int64_t C, const int64_t* labels, float scale,
+                        int reduction, const float* state, const float* g, void* dh,
+                        int64_t ldd, void* dW, int64_t ldo, void* ws, size_t ws_bytes,
+                        void* stream);
 int crbq_head_distill(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
                       int64_t T, int64_t V, int64_t C, const void* top_val, int val_dtype,
                       int64_t ldv, const int32_t* top_idx, int64_t ldi, int k,
@@ -403,9 +404,9 @@ int crbq_head_distill(const void* h, int64_t ldh, const void* W, int64_t ldw, in
                       float* loss, float* state, void* ws, size_t ws_bytes, void* stream);
 int crbq_head_distill_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
                            int64_t T, int64_t V, int64_t C, int k, float scale,
-                           float temperature, const float* state, const float* g, int g_per_row,
-                           void* dh, int64_t ldd, void* dW, int64_t ldo, void* ws,
-                           size_t ws_bytes, void* stream);
+                           float temperature, int reduction, const float* state,
+                           const float* g, void* dh, int64_t ldd, void* dW, int64_t ldo,
+                           void* ws, size_t ws_bytes, void* stream);
 /* The k largest of each row of logits [T][V] (row stride ld, any dtype),
  * descending, ties to the lowest index, NaN above everything: val [T][k]
  * (the logits' dtype), idx [T][k], and lse[t] = log sum exp of the row

@@ -561,9 +561,14 @@ def test_refusals():
             f()
             pytest.fail(f"call {i} was not refused")
     _, state = kernels.head_xent(h, W, y)
-    for g in (torch.ones(3, device=DEV), torch.ones((), device=DEV).double()):
+    for g in (torch.ones(4, device=DEV), torch.ones((), device=DEV).double()):
         with pytest.raises(CrbqError):
             kernels.head_xent_grad(h, W, y, state, g)
+    one = torch.ones((), device=DEV)
+    for kw in (dict(need_h=False, need_w=False), dict(reduction="none"), dict(reduction="x")):
+        with pytest.raises(CrbqError):
+            kernels.head_xent_grad(h, W, y, state, one, **kw)
     with pytest.raises(CrbqError):
-        kernels.head_xent_grad(h, W, y, state, torch.ones((), device=DEV), need_h=False,
-                               need_w=False)
+        kernels.head_xent_grad(h, W, y, state[1:], one)
+    with pytest.raises(CrbqError):
+        kernels.head_distill_grad(h, W, 3, state, one)

@@ -22,9 +22,8 @@ def xent(**kw):
 
 
 def xent_grad(**kw):
-    a = dict(h=P[0], ldh=64, W=P[1], ldw=64, dtype=1, T=4, V=100, C=64, labels=P[2], ignore=-100,
-             scale=1.0, state=P[4], g=P[3], rows=0, dh=P[5], ldd=64, dW=P[6], ldo=64, ws=None,
-             nws=0, s=None)
+    a = dict(h=P[0], ldh=64, W=P[1], ldw=64, dtype=1, T=4, V=100, C=64, labels=P[2], scale=1.0,
+             red=1, state=P[4], g=P[3], dh=P[5], ldd=64, dW=P[6], ldo=64, ws=None, nws=0, s=None)
     a.update(kw)
     return lib().crbq_head_xent_grad(*a.values())
 
@@ -39,7 +38,7 @@ def distill(**kw):
 
 def distill_grad(**kw):
     a = dict(h=P[0], ldh=64, W=P[1], ldw=64, dtype=1, T=4, V=100, C=64, k=8, scale=1.0, temp=1.0,
-             state=P[4], g=P[3], rows=0, dh=P[5], ldd=64, dW=P[6], ldo=64, ws=None, nws=0, s=None)
+             red=0, state=P[4], g=P[3], dh=P[5], ldd=64, dW=P[6], ldo=64, ws=None, nws=0, s=None)
     a.update(kw)
     return lib().crbq_head_distill_grad(*a.values())
 
@@ -69,7 +68,7 @@ def test_other_refusals():
         assert xent(**bad) == ARG, bad
     for call in (xent_grad, distill_grad):
         for bad in (dict(state=None), dict(g=None), dict(dh=None, dW=None), dict(dh=ODD),
-                    dict(dW=ODD), dict(ldd=60), dict(ldo=8)):
+                    dict(dW=ODD), dict(ldd=60), dict(ldo=8), dict(state=ODD), dict(red=3)):
             assert call(**bad) == ARG, bad
         assert call(dh=None) == WS and call(dW=None) == WS
     assert xent_grad(labels=None) == ARG
