@@ -638,14 +638,18 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   g_wait_vm<0>();
 }
 
-// 64 words (lane l: word l of p) and 64 rows of 16 bytes (lane l: p + l * ld) into
-// the wavefront's own LDS; what lies behind nbytes reads as zeros.
-__device__ __forceinline__ void g_load_lds_words(const void* dst, const void* p, int64_t nbytes,
-                                                 int lane) {
+__device__ __forceinline__ void g_load_lds_word(const void* dst, i4_t rs, unsigned voff) {
   const unsigned d = __builtin_amdgcn_readfirstlane(
       (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)dst);
-  const i4_t rs = g_rsrc((const uint16_t*)p, nbytes > 0 ? (nbytes < 256 ? nbytes : 256) : 0);
-  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(lane * 4), "s"(rs), "{m0}"(d));
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(d));
+}
+
+// 64 words (lane l: word l of p) into the wavefront's own LDS; what lies behind
+// nbytes reads as zeros.
+__device__ __forceinline__ void g_load_lds_words(const void* dst, const void* p, int64_t nbytes,
+                                                 int lane) {
+  g_load_lds_word(dst, g_rsrc((const uint16_t*)p, nbytes > 0 ? (nbytes < 256 ? nbytes : 256) : 0),
+                  lane * 4);
 }
 
 // 16 rows (n) of a wavefront's 16-bit output of a 256 x 256 tile (128 elements each, m

@@ -77,11 +77,18 @@ __device__ __forceinline__ float log_add(float a, float b) {
 // Where the listed tokens of the rows are (forward).
 struct Listed {
   const int64_t* labels;   // cross entropy: one per row
-  const uint32_t* mask;    // distillation: a bit per (row, token), ldm words a row
-  const int32_t* sidx;     //   and each row's k tokens, ascending, PAD_IDX behind them
-  int64_t ldm;
+  const uint32_t* mask;    // distillation: a bit per (row, token), 8 words a tile of 256,
+  const int32_t* base;     //   and the row's listed tokens before each tile: a token's slot in
+  int64_t ntile;           //   the row's ascending list is that plus the bits before its own
   int k;
 };
+// the bits of words before word w
+__device__ __forceinline__ int bits_before(const uint32_t (&w)[8], int n) {
+  int c = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) c += q < n ? __popc(w[q]) : 0;
+  return c;
+}
 
 // ---------------------------------------------------------------------------
 // forward product: partial (max, sum) of every (row, tile row of wavefronts)
@@ -98,30 +105,19 @@ struct FwdArgs {
   float* zt;
 };
 
-// The slot of token v in row t's ascending list.
-__device__ __forceinline__ int64_t list_slot(const Listed& ls, int64_t t, int v) {
-  const int32_t* s = ls.sidx + t * ls.k;
-  int lo = 0, hi = ls.k - 1;
-  while (lo < hi) {
-    const int md = (lo + hi) >> 1;
-    if (s[md] < v) lo = md + 1;
-    else hi = md;
-  }
-  return t * ls.k + lo;
-}
-
 // Column t (n) of a wavefront's tile, MI times 16 tokens, the i-th 16 of them
 // from v0 + off(i) on: listed tokens and what lies behind the vocabulary
 // become -inf (the listed ones' z is written), then the maximum and the sum
-// of exponentials.  lab: the label's place behind v0; words: each i's 16 mask bits.
+// of exponentials.  lab: the label's place behind v0; words: each i's 16 mask
+// bits; before(q): the slot of the first token of words[q].
 // In units of log 2: exp z = 2^(acc * scale2), so an exponential is one
 // multiply-add and one v_exp; the listed tokens and the end are looked for
 // only where a wavefront has any.  Bound by the v_exp (16 cycles a wavefront)
 // and the 2 to 3 vector operations beside each.
-template <int MI, int NJ, bool XENT, int j, typename Off>
+template <int MI, int NJ, bool XENT, int j, typename Off, typename Before>
 __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t v0, Off off,
                                            int lab, const uint32_t (&words)[(MI + 1) / 2],
-                                           f4_t (&acc)[MI][NJ], float2* out) {
+                                           Before before, f4_t (&acc)[MI][NJ], float2* out) {
   const int lane = g_lane(), g4 = (lane >> 4) * 4;
   const bool ok = t < p.T;
   bool any;
@@ -135,6 +131,11 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   }
   const float fin = p.scale < 0.f ? INFINITY : -INFINITY;        // scale * fin = -inf
   if (__any(any)) {
+    int slot[(MI + 1) / 2] = {};
+    if (!XENT) {
+#pragma unroll
+      for (int q = 0; q < (MI + 1) / 2; ++q) slot[q] = before(q);
+    }
     g_each<MI>([&](auto ii) __attribute__((always_inline)) {
       constexpr int i = decltype(ii)::value;
       const int o = off(i) + g4;
@@ -144,7 +145,9 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
         g_each<4>([&](auto rr) __attribute__((always_inline)) {
           constexpr int r = decltype(rr)::value;
           if (XENT ? o + r == lab : (nib >> r) & 1u) {
-            p.zt[XENT ? t : list_slot(p.ls, t, (int)(v0 + o + r))] = acc[i][j][r] * p.scale;
+            const int bit = 16 * (i & 1) + g4 + r;     // of words[i / 2]
+            p.zt[XENT ? t : t * p.ls.k + slot[i / 2] + __popc(words[i / 2] & ((1u << bit) - 1))] =
+                acc[i][j][r] * p.scale;
             acc[i][j][r] = fin;
           }
         });
@@ -203,16 +206,27 @@ __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
     const int64_t t = t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15);
     const bool ok = t < p.T;
     int lab = -1;                                      // the label's place among the wavefront's
-    uint32_t words[G::WM / 32] = {};
+    uint32_t words[G::WM / 32] = {}, all[8] = {};
     if (XENT) {
       const int64_t y = ok ? p.ls.labels[t] : -1;
       lab = y >= vw && y < vw + G::WM ? (int)(y - vw) : -1;
     } else if (ok) {
+      const uint4* w = (const uint4*)(p.ls.mask + (t * p.ls.ntile + tm) * 8);
+      const uint4 a = w[0], b = w[1];
+      all[0] = a.x; all[1] = a.y; all[2] = a.z; all[3] = a.w;
+      all[4] = b.x; all[5] = b.y; all[6] = b.z; all[7] = b.w;
 #pragma unroll
-      for (int w = 0; w < G::WM / 32; ++w) words[w] = p.ls.mask[t * p.ls.ldm + (vw >> 5) + w];
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int e = 0; e < G::WM / 32; ++e)
+          if (q == wr * (G::WM / 32) + e) words[e] = all[q];
     }
-    fwd_column<G::MI, G::NJ, XENT, j>(p, t, vw, [](int i) { return 16 * i; }, lab, words, acc,
-                                      p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
+    auto before = [&](int q) __attribute__((always_inline)) {
+      return ok ? p.ls.base[t * p.ls.ntile + tm] + bits_before(all, wr * (G::WM / 32) + q) : 0;
+    };
+    fwd_column<G::MI, G::NJ, XENT, j>(
+        p, t, vw, [](int i) { return 16 * i; }, lab, words, before, acc,
+        p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
   });
 }
 
@@ -263,9 +277,13 @@ struct FwdJob {
       } else {
         const int64_t rows = left < 32 ? left : 32;
         g_load_lds(priv + 1024 * b,
-                   g_rsrc((const uint16_t*)(p.ls.mask + t * p.ls.ldm + (v0 >> 5)),
-                          rows > 0 ? ((rows - 1) * p.ls.ldm + 8) * 4 : 0),
-                   (unsigned)((lane >> 1) * p.ls.ldm * 4 + (lane & 1) * 16));
+                   g_rsrc((const uint16_t*)(p.ls.mask + (t * p.ls.ntile + tm) * 8),
+                          rows > 0 ? ((rows - 1) * p.ls.ntile + 1) * 32 : 0),
+                   (unsigned)((lane >> 1) * p.ls.ntile * 32 + (lane & 1) * 16));
+        g_load_lds_word(priv + 2048 + 256 * b,
+                        g_rsrc((const uint16_t*)(p.ls.base + t * p.ls.ntile + tm),
+                               rows > 0 ? ((rows - 1) * p.ls.ntile + 1) * 4 : 0),
+                        (unsigned)(lane * p.ls.ntile * 4));      // (lanes behind the 32 rows: 0)
       }
     }
   }
@@ -291,9 +309,15 @@ struct FwdJob {
 #pragma unroll
         for (int q = 0; q < 4; ++q) words[q] = w[2 * q];
       }
+      auto before = [&](int q) __attribute__((always_inline)) {
+        const uint32_t* w = (const uint32_t*)(priv + 1024 * (j >> 1)) + row * 8;
+        int c = ((const int*)(priv + 2048 + 256 * (j >> 1)))[row];
+        for (int e = 0; e < 2 * q + wr; ++e) c += __popc(w[e]);
+        return c;
+      };
       fwd_column<8, 4, XENT, j>(
           p, t, v0, [&](int i) { return 64 * (i >> 1) + 32 * wr + 16 * (i & 1); }, lab, words,
-          acc.v, p.part + t * p.npart + (int64_t)tm * 2 + wr);
+          before, acc.v, p.part + t * p.npart + (int64_t)tm * 2 + wr);
     });
   }
 };
@@ -461,13 +485,14 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
                                              const int32_t* __restrict__ idx, int64_t ldi,
                                              const float* __restrict__ tlse, float itemp,
                                              int64_t V, int k, State st, uint32_t* mask,
-                                             int64_t ldm) {
+                                             int32_t* base, int64_t ntile) {
   __shared__ __attribute__((aligned(16))) int ix[LIST_MAX];
   __shared__ __attribute__((aligned(16))) float pr[LIST_MAX];
+  __shared__ int srt[LIST_MAX];
   const int lane = threadIdx.x;
   const int64_t t = blockIdx.x;
-  uint4* words = (uint4*)(mask + t * ldm);             // ldm is a multiple of 8
-  for (int64_t i = lane; i < ldm / 4; i += 64) words[i] = make_uint4(0u, 0u, 0u, 0u);
+  uint32_t* words = mask + t * ntile * 8;
+  for (int64_t i = lane; i < ntile * 2; i += 64) ((uint4*)words)[i] = make_uint4(0u, 0u, 0u, 0u);
   float m = -INFINITY;
   const int k4 = (k + 3) & ~3;
   if (lane < k4 - k) ix[k + lane] = -1;                // read by fours
@@ -487,6 +512,8 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
     s += pr[i];
   }
   s = wave_sum_f(s);
+  // (the cleared words have arrived before their bits are set)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   const float norm = tlse ? 1.f : 1.f / s;
   float ent = 0.f;
@@ -524,6 +551,7 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
   for (int q = 0; q < LIST_MAX / 64; ++q)
     if (lane + 64 * q < k) {
       ix[lane + 64 * q] = mine[q];
+      srt[lane + 64 * q] = PAD_IDX;
       st.sidx[t * k + lane + 64 * q] = PAD_IDX;
       st.p[t * k + lane + 64 * q] = 0.f;
       st.zt[t * k + lane + 64 * q] = 0.f;
@@ -541,8 +569,20 @@ __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t
       }
       st.sidx[t * k + rank] = mine[q];
       st.p[t * k + rank] = prob[q] * norm;
-      atomicOr(mask + t * ldm + (mine[q] >> 5), 1u << (mine[q] & 31));
+      atomicOr(words + (mine[q] >> 5), 1u << (mine[q] & 31));
+      srt[rank] = mine[q];
     }
+  __syncthreads();
+  // listed tokens before each tile of 256
+  for (int64_t i = lane; i < ntile; i += 64) {
+    int lo = 0, hi = k;
+    while (lo < hi) {
+      const int md = (lo + hi) >> 1;
+      if (srt[md] < (int)(i * 256)) lo = md + 1;
+      else hi = md;
+    }
+    base[t * ntile + i] = lo;
+  }
   if (lane == 0) {
     st.ent[t] = ent;
     st.pt[t] = tlse && s < 1.f ? 1.f - s : 0.f;
@@ -990,7 +1030,6 @@ static int64_t n_part(int64_t T, int64_t V) {
   static const int wgm[3] = {ZS::WGM, ZM::WGM, Big::WGM};
   return cdiv(V, 256) * wgm[token_tile(T)];
 }
-static int64_t mask_words(int64_t V) { return cdiv(V, 256) * 8; }
 
 // Vocabulary of a backward piece: dz of a piece in about 128 MB (it is read
 // back by two products: within the 256 MB of the last-level cache), at
@@ -1025,13 +1064,15 @@ struct FwdWs {
   float* rows;
   uint8_t* live;
   uint32_t* mask;
+  int32_t* base;
   size_t bytes;
   FwdWs(void* ws, size_t cap, int64_t T, int64_t V, int64_t k, bool& ok) {
     WsCarver w(ws, cap);
     part = w.take<float2>((size_t)(T * n_part(T, V)));
     rows = w.take<float>((size_t)T);
     live = w.take<uint8_t>((size_t)T);
-    mask = k ? w.take<uint32_t>((size_t)(T * mask_words(V))) : nullptr;
+    mask = k ? w.take<uint32_t>((size_t)(T * cdiv(V, 256)) * 8) : nullptr;
+    base = k ? w.take<int32_t>((size_t)(T * cdiv(V, 256))) : nullptr;
     bytes = w.off;
     ok = w.ok();
   }
@@ -1275,19 +1316,19 @@ extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int6
   if (!ok) return CRBQ_ERR_WORKSPACE;
   const State st(state, T, k);
   hipStream_t s = (hipStream_t)stream;
-  const int64_t ldm = mask_words(V);
+  const int64_t ntile = cdiv(V, 256);
   const float it = 1.f / temperature;
   if (val_dtype == CRBQ_F32)
     k_list<float><<<(unsigned)T, 64, 0, s>>>((const float*)top_val, ldv, top_idx, ldi, top_lse, it,
-                                             V, k, st, w.mask, ldm);
+                                             V, k, st, w.mask, w.base, ntile);
   else if (val_dtype == CRBQ_F16)
     k_list<_Float16><<<(unsigned)T, 64, 0, s>>>((const _Float16*)top_val, ldv, top_idx, ldi,
-                                                top_lse, it, V, k, st, w.mask, ldm);
+                                                top_lse, it, V, k, st, w.mask, w.base, ntile);
   else
     k_list<__bf16><<<(unsigned)T, 64, 0, s>>>((const __bf16*)top_val, ldv, top_idx, ldi, top_lse,
-                                              it, V, k, st, w.mask, ldm);
+                                              it, V, k, st, w.mask, w.base, ntile);
   CRBQ_LAUNCH_CHECK();
-  const Listed ls{nullptr, w.mask, st.sidx, ldm, k};
+  const Listed ls{nullptr, w.mask, w.base, ntile, k};
   return dtype == CRBQ_F16 ? head_fwd<h8_t, false>(h, ldh, W, ldw, T, V, C, scale * it, ls, 0,
                                                    reduction, loss, st, w, s)
                            : head_fwd<b8_t, false>(h, ldh, W, ldw, T, V, C, scale * it, ls, 0,

@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as fwad
 
 from . import kernels
 from ._lib import CrbqError
@@ -28,42 +29,31 @@ class TopLogits(NamedTuple):
     lse: Optional[torch.Tensor]        # fp32 [...]: log sum exp of logits / temperature
 
 
-class _LinearXent(torch.autograd.Function):
+class _Loss(torch.autograd.Function):
+    """One of the losses; call, top and ignore_index as kernels takes them."""
+
     @staticmethod
-    def forward(ctx, h, weight, labels, scale, ignore_index, reduction):
-        loss, state = kernels.head_xent(h, weight, labels, scale, ignore_index, reduction)
-        ctx.save_for_backward(h, weight, labels, state)
-        ctx.conf = scale, reduction
+    def forward(ctx, h, weight, call, top, ignore_index):
+        loss, state = call.forward(top, ignore_index)
+        ctx.save_for_backward(h, weight, call.labels, state)
+        ctx.call = call
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        h, weight, labels, state = ctx.saved_tensors
-        dh, dW = kernels.head_xent_grad(h, weight, labels, state, g, *ctx.conf,
-                                        need_h=ctx.needs_input_grad[0],
-                                        need_w=ctx.needs_input_grad[1])
-        return dh, dW, None, None, None, None
+        call, state = ctx.call, ctx.saved_tensors[3]   # (and the check that none was changed)
+        dh, dW = call.grad(state, g.contiguous(), ctx.needs_input_grad[0],
+                           ctx.needs_input_grad[1])
+        return dh, dW, None, None, None
 
 
-class _LinearDistill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, weight, val, idx, lse, scale, temperature, reduction):
-        loss, state = kernels.head_distill(h, weight, val, idx, lse, scale, temperature,
-                                           reduction)
-        ctx.save_for_backward(h, weight, state)
-        ctx.conf = scale, temperature, reduction
-        ctx.k = val.shape[1]
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        h, weight, state = ctx.saved_tensors
-        dh, dW = kernels.head_distill_grad(h, weight, ctx.k, state, g, *ctx.conf,
-                                           need_h=ctx.needs_input_grad[0],
-                                           need_w=ctx.needs_input_grad[1])
-        return dh, dW, None, None, None, None, None, None
+def _loss(h, weight, call, top=None, ignore_index=-100):
+    # (a forward-mode tangent is refused by the Function, not dropped)
+    if (torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
+            or fwad._current_level >= 0):
+        return _Loss.apply(h, weight, call, top, ignore_index)
+    return call.forward(top, ignore_index)[0]
 
 
 def _rows(x: torch.Tensor, lead, what: str, tail: int) -> torch.Tensor:
@@ -71,7 +61,7 @@ def _rows(x: torch.Tensor, lead, what: str, tail: int) -> torch.Tensor:
     if x.shape[:x.dim() - tail] != lead:
         raise CrbqError(f"{what} of shape {tuple(x.shape)} do not fit hidden states of "
                         f"{tuple(lead)} tokens")
-    return x.reshape(-1, *x.shape[x.dim() - tail:])
+    return x if len(lead) == 1 else x.reshape(-1, *x.shape[x.dim() - tail:])
 
 
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -83,9 +73,11 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     no token is NaN) and of the gradients; a label outside the vocabulary
     makes loss and gradients NaN.  reduction "mean", "sum" or "none"."""
     lead = h.shape[:-1]
-    loss = _LinearXent.apply(h.reshape(-1, h.shape[-1]), weight, _rows(labels, lead, "labels", 0),
-                             float(scale), int(ignore_index), reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+    x = h if len(lead) == 1 else h.reshape(-1, h.shape[-1])
+    call = kernels.xent_call(x, weight, _rows(labels, lead, "labels", 0), scale, reduction,
+                             "linear_cross_entropy")
+    loss = _loss(x, weight, call, None, int(ignore_index))
+    return loss if reduction != "none" or len(lead) == 1 else loss.reshape(lead)
 
 
 def linear_distill(h: torch.Tensor, weight: torch.Tensor, top, temperature: float = 1.0,
@@ -100,18 +92,22 @@ def linear_distill(h: torch.Tensor, weight: torch.Tensor, top, temperature: floa
     loss has no factor temperature ** 2."""
     val, idx, lse = top
     lead = h.shape[:-1]
-    loss = _LinearDistill.apply(
-        h.reshape(-1, h.shape[-1]), weight, _rows(val.detach(), lead, "teacher logits", 1),
-        _rows(idx, lead, "teacher tokens", 1),
-        None if lse is None else _rows(lse.detach(), lead, "teacher log-sum-exps", 0),
-        float(scale), float(temperature), reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+    x = h if len(lead) == 1 else h.reshape(-1, h.shape[-1])
+    top = kernels.top_args(x, _rows(val, lead, "teacher logits", 1),
+                           _rows(idx, lead, "teacher tokens", 1),
+                           None if lse is None else _rows(lse, lead, "teacher log-sum-exps", 0),
+                           "linear_distill")
+    call = kernels.distill_call(x, weight, top[0].shape[1], scale, temperature, reduction,
+                                "linear_distill")
+    loss = _loss(x, weight, call, top)
+    return loss if reduction != "none" or len(lead) == 1 else loss.reshape(lead)
 
 
-@torch.no_grad()
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest of logits [..., V] (ties to the lowest index, NaN above
     everything) and the log-sum-exp of logits / temperature."""
     lead = logits.shape[:-1]
+    if len(lead) == 1:
+        return TopLogits(*kernels.top_logits(logits, k, temperature))
     val, idx, lse = kernels.top_logits(logits.reshape(-1, logits.shape[-1]), k, temperature)
     return TopLogits(val.reshape(*lead, k), idx.reshape(*lead, k), lse.reshape(lead))

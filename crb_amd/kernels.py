@@ -7,6 +7,7 @@ torch's current stream and raises CrbqError on a non-zero status.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 from typing import NamedTuple
 
@@ -536,30 +537,38 @@ def linear_packed(codes: torch.Tensor, lut: torch.Tensor, sal: torch.Tensor, C: 
 
 
 # -- losses of the output head -------------------------------------------------
-def _one_gpu(what, *ts):
-    dev = ts[0].get_device()                     # -1 on the CPU
-    if dev < 0 or any(t is not None and t.get_device() != dev for t in ts):
+# One token's call is host time: checks without generators, sizes asked of the
+# library once per shape, few allocations.
+def _one_gpu(what, a, *ts):
+    dev = a.get_device()                         # -1 on the CPU
+    ok = dev >= 0
+    for t in ts:
+        ok = ok and (t is None or t.get_device() == dev)
+    if not ok:
         raise _lib.CrbqError(f"{what}: its tensors must live on the GPU, on one device")
 
 
 def _head_matrix(x: torch.Tensor) -> torch.Tensor:
     """x [n, C] as the head kernels read it: rows of a multiple of 8 elements
     (zeros behind the last channel) that start at multiples of 16 bytes."""
-    C = x.shape[1]
+    n, C = x.shape
     if C % 8:
-        y = torch.zeros((x.shape[0], (C + 7) // 8 * 8), dtype=x.dtype, device=x.device)
+        y = torch.empty((n, (C + 7) // 8 * 8), dtype=x.dtype, device=x.device)
         y[:, :C] = x
+        y[:, C:] = 0
         return y
-    if x.shape[0] == 1 and x.stride(1) == 1 and x.data_ptr() % 16 == 0:
-        return x.as_strided((1, C), (C, 1))      # the stride of a single row says nothing
-    if x.stride(1) != 1 or x.stride(0) < C or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    ld, one = x.stride()
+    if one == 1 and x.data_ptr() % 16 == 0:
+        if ld >= C and ld % 8 == 0:
+            return x
+        if n == 1:
+            return x.as_strided((1, C), (C, 1))  # the stride of a single row says nothing
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _head_pair(what, h, W):
     _one_gpu(what, h, W)
-    if h.dtype not in (torch.float16, torch.bfloat16) or W.dtype != h.dtype:
+    if W.dtype != h.dtype or h.dtype not in (torch.float16, torch.bfloat16):
         raise _lib.CrbqError(f"{what} takes hidden states and a weight that are both fp16 or both "
                              f"bf16, not {h.dtype} and {W.dtype}")
     if h.dim() != 2 or W.dim() != 2 or h.shape[1] != W.shape[1] or 0 in h.shape or 0 in W.shape:
@@ -569,65 +578,147 @@ def _head_pair(what, h, W):
 
 
 def _reduction(what, reduction):
-    if reduction not in _lib.REDUCTIONS:
+    red = _lib.REDUCTIONS.get(reduction)
+    if red is None:
         raise _lib.CrbqError(f"{what}: reduction {reduction!r} is none of "
                              f"{sorted(_lib.REDUCTIONS)}")
-    return _lib.REDUCTIONS[reduction]
+    return red
 
 
-def _head_buffers(lib, h, W, k, red, dev):
-    T, C = h.shape
-    nws = int(lib.crbq_head_workspace_size(T, W.shape[0], C, k, 0))
-    state = torch.empty(int(lib.crbq_head_state_floats(T, k)), dtype=torch.float32, device=dev)
-    loss = torch.empty((T,) if red == 0 else (), dtype=torch.float32, device=dev)
-    return loss, state, _ws(nws, dev), nws
+def _labels(what, h, labels):
+    _one_gpu(what, h, labels)
+    if labels.dtype != torch.int64 or labels.shape != h.shape[:1]:
+        raise _lib.CrbqError(f"{what} takes int64 labels [T]")
+    return labels.contiguous()
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_sizes(T, V, C, k):
+    """(floats of the state, bytes of the forward's and of the gradients' workspace)"""
+    lib = _lib.load()
+    return (int(lib.crbq_head_state_floats(T, k)), int(lib.crbq_head_workspace_size(T, V, C, k, 0)),
+            int(lib.crbq_head_workspace_size(T, V, C, k, 1)))
+
+
+class _HeadCall:
+    """A validated call of one of the losses: its operands as the kernels read
+    them, what its gradients take over, and its launches."""
+
+    __slots__ = ("h", "W", "C", "labels", "k", "scale", "temperature", "red", "lib", "dt")
+
+    def __init__(self, h, W, C, labels, k, scale, temperature, red):
+        self.h, self.W, self.C = h, W, C         # C: the channels that are not padding
+        self.labels, self.k = labels, k
+        self.scale, self.temperature, self.red = scale, temperature, red
+        self.lib = _lib.ready(h.device)
+        self.dt = _lib.DTYPES[h.dtype]
+
+    def forward(self, top=None, ignore_index=-100):
+        """(loss, state); top: (values, tokens, lse or None) of a distillation"""
+        h, W = self.h, self.W
+        T, C = h.shape
+        V, dev = W.shape[0], h.device
+        floats, nws, _ = _head_sizes(T, V, C, self.k)
+        with _lib.on_device(dev):
+            state = torch.empty(floats, dtype=torch.float32, device=dev)
+            loss = torch.empty((T,) if self.red == 0 else (), dtype=torch.float32, device=dev)
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+            if top is None:
+                st = self.lib.crbq_head_xent(h.data_ptr(), h.stride(0), W.data_ptr(), W.stride(0),
+                                             self.dt, T, V, C, self.labels.data_ptr(),
+                                             ignore_index, self.scale, self.red, loss.data_ptr(),
+                                             state.data_ptr(), ws.data_ptr(), nws, stream_of(h))
+            else:
+                val, idx, lse = top
+                k = self.k
+                st = self.lib.crbq_head_distill(h.data_ptr(), h.stride(0), W.data_ptr(),
+                                                W.stride(0), self.dt, T, V, C, val.data_ptr(),
+                                                _lib.DTYPES[val.dtype], max(val.stride(0), k),
+                                                idx.data_ptr(), max(idx.stride(0), k), k, ptr(lse),
+                                                self.scale, self.temperature, self.red,
+                                                loss.data_ptr(), state.data_ptr(), ws.data_ptr(),
+                                                nws, stream_of(h))
+        check(st, "crbq_head_xent" if top is None else "crbq_head_distill")
+        return loss, state
+
+    def grad(self, state, g, need_h=True, need_w=True):
+        """(dh, dW), None where not asked for"""
+        h, W = self.h, self.W
+        T, C = h.shape
+        V, dev = W.shape[0], h.device
+        nws = _head_sizes(T, V, C, self.k)[2]
+        with _lib.on_device(dev):
+            dh = torch.empty((T, C), dtype=h.dtype, device=dev) if need_h else None
+            dW = torch.empty((V, C), dtype=h.dtype, device=dev) if need_w else None
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+            tail = (self.red, state.data_ptr(), g.data_ptr(), ptr(dh), C, ptr(dW), C,
+                    ws.data_ptr(), nws, stream_of(h))
+            args = (h.data_ptr(), h.stride(0), W.data_ptr(), W.stride(0), self.dt, T, V, C)
+            if self.k:
+                st = self.lib.crbq_head_distill_grad(*args, self.k, self.scale, self.temperature,
+                                                     *tail)
+            else:
+                st = self.lib.crbq_head_xent_grad(*args, self.labels.data_ptr(), self.scale, *tail)
+            check(st, "crbq_head_distill_grad" if self.k else "crbq_head_xent_grad")
+            if self.C != C:
+                dh = dh[:, :self.C].contiguous() if need_h else None
+                dW = dW[:, :self.C].contiguous() if need_w else None
+        return dh, dW
+
+    def check_grad(self, what, state, g, need_h, need_w):
+        _one_gpu(what, self.h, state, g)
+        if not (need_h or need_w):
+            raise _lib.CrbqError(f"{what}: no gradient asked for")
+        if g.dtype != torch.float32 or g.shape != (self.h.shape[:1] if self.red == 0 else ()):
+            raise _lib.CrbqError(f"{what} takes the loss's gradient, fp32 and of its shape")
+        if (state.dtype != torch.float32 or not state.is_contiguous() or state.data_ptr() % 8
+                or state.numel() != _head_sizes(self.h.shape[0], self.W.shape[0], self.h.shape[1],
+                                                self.k)[0]):
+            raise _lib.CrbqError(f"{what}: not the state of this call's forward")
+
+
+def xent_call(h, W, labels, scale, reduction, what="head_xent") -> _HeadCall:
+    hp, Wp = _head_pair(what, h, W)
+    return _HeadCall(hp, Wp, h.shape[1], _labels(what, h, labels), 0, float(scale), 1.0,
+                     _reduction(what, reduction))
+
+
+def distill_call(h, W, k, scale, temperature, reduction, what="head_distill") -> _HeadCall:
+    hp, Wp = _head_pair(what, h, W)
+    if not 1 <= k <= _lib.HEAD_MAX_K:
+        raise _lib.CrbqError(f"{what} takes 1 to {_lib.HEAD_MAX_K} listed tokens, not {k}")
+    if not temperature > 0:
+        raise _lib.CrbqError(f"{what} takes a temperature above 0")
+    return _HeadCall(hp, Wp, h.shape[1], None, k, float(scale), float(temperature),
+                     _reduction(what, reduction))
+
+
+def top_args(h, val, idx, lse, what="head_distill"):
+    """The teacher's (values, tokens, lse or None) of hidden states h [T, C], checked."""
+    _one_gpu(what, h, val, idx, lse)
+    T = h.shape[0]
+    if val.dtype not in _lib.DTYPES or idx.dtype != torch.int32:
+        raise _lib.CrbqError(f"{what} takes floating teacher logits and int32 tokens")
+    if val.dim() != 2 or val.shape != idx.shape or val.shape[0] != T:
+        raise _lib.CrbqError(f"{what} takes teacher logits and tokens [T, k], not "
+                             f"{tuple(val.shape)} and {tuple(idx.shape)}")
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (T,):
+            raise _lib.CrbqError(f"{what} takes an fp32 teacher log-sum-exp [T]")
+        lse = lse.contiguous()
+    k = val.shape[1]
+    if val.stride(1) != 1 or val.stride(0) < k:
+        val = val.contiguous()
+    if idx.stride(1) != 1 or idx.stride(0) < k:
+        idx = idx.contiguous()
+    return val, idx, lse
 
 
 def head_xent(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, scale: float = 1.0,
               ignore_index: int = -100, reduction: str = "mean"):
     """Cross entropy of the logits scale * h W^T (never kept) against labels
     [T] int64.  Returns (loss fp32 [T] or scalar, state for head_xent_grad)."""
-    hp, Wp = _head_pair("head_xent", h, W)
-    _one_gpu("head_xent", h, labels)
-    if labels.dtype != torch.int64 or labels.shape != h.shape[:1]:
-        raise _lib.CrbqError("head_xent takes int64 labels [T]")
-    labels = labels.contiguous()
-    red = _reduction("head_xent", reduction)
-    lib = _lib.ready(h.device)
-    with _lib.on_device(h.device):
-        loss, state, ws, nws = _head_buffers(lib, hp, Wp, 0, red, h.device)
-        check(lib.crbq_head_xent(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
-                                 _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0], hp.shape[1],
-                                 labels.data_ptr(), int(ignore_index), float(scale), red,
-                                 loss.data_ptr(), state.data_ptr(), ws.data_ptr(), nws,
-                                 stream_of(h)), "crbq_head_xent")
-    return loss, state
-
-
-def _grad_args(what, hp, Wp, state, k, g, red, need_h, need_w, lib):
-    """Output buffers (padded like their inputs), workspace and g of a gradient call."""
-    _one_gpu(what, hp, state, g)
-    if not (need_h or need_w):
-        raise _lib.CrbqError(f"{what}: no gradient asked for")
-    if g.dtype != torch.float32 or g.shape != (hp.shape[:1] if red == 0 else ()):
-        raise _lib.CrbqError(f"{what} takes the loss's gradient, fp32 and of its shape")
-    if (state.dtype != torch.float32 or not state.is_contiguous()
-            or state.numel() != lib.crbq_head_state_floats(hp.shape[0], k)):
-        raise _lib.CrbqError(f"{what}: not the state of this call's forward")
-    dh = torch.empty_like(hp, memory_format=torch.contiguous_format) if need_h else None
-    dW = torch.empty_like(Wp, memory_format=torch.contiguous_format) if need_w else None
-    T, C = hp.shape
-    nws = int(lib.crbq_head_workspace_size(T, Wp.shape[0], C, 0, 1))
-    return dh, dW, _ws(nws, hp.device), nws, g.contiguous()
-
-
-def _out_args(dh, dW):
-    return (ptr(dh), dh.stride(0) if dh is not None else 0, ptr(dW),
-            dW.stride(0) if dW is not None else 0)
-
-
-def _cut(x, C):
-    return x if x is None or x.shape[1] == C else x[:, :C].contiguous()
+    return xent_call(h, W, labels, scale, reduction).forward(None, int(ignore_index))
 
 
 def head_xent_grad(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, state: torch.Tensor,
@@ -635,22 +726,9 @@ def head_xent_grad(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, state
                    need_h: bool = True, need_w: bool = True):
     """(dh, dW) (None where not asked for) of head_xent's loss, called with the
     same scale and reduction, times g (fp32, of the loss's shape)."""
-    hp, Wp = _head_pair("head_xent_grad", h, W)
-    _one_gpu("head_xent_grad", h, labels)
-    if labels.dtype != torch.int64 or labels.shape != h.shape[:1]:
-        raise _lib.CrbqError("head_xent_grad takes int64 labels [T]")
-    red = _reduction("head_xent_grad", reduction)
-    lib = _lib.ready(h.device)
-    labels = labels.contiguous()
-    with _lib.on_device(h.device):
-        dh, dW, ws, nws, g = _grad_args("head_xent_grad", hp, Wp, state, 0, g, red, need_h,
-                                        need_w, lib)
-        check(lib.crbq_head_xent_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
-                                      _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0], hp.shape[1],
-                                      labels.data_ptr(), float(scale), red, state.data_ptr(),
-                                      g.data_ptr(), *_out_args(dh, dW), ws.data_ptr(), nws,
-                                      stream_of(h)), "crbq_head_xent_grad")
-    return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])
+    call = xent_call(h, W, labels, scale, reduction, "head_xent_grad")
+    call.check_grad("head_xent_grad", state, g, need_h, need_w)
+    return call.grad(state, g.contiguous(), need_h, need_w)
 
 
 def head_distill(h: torch.Tensor, W: torch.Tensor, top_val: torch.Tensor, top_idx: torch.Tensor,
@@ -659,36 +737,8 @@ def head_distill(h: torch.Tensor, W: torch.Tensor, top_val: torch.Tensor, top_id
     """KL from a teacher's listed logits (top_val, top_idx int32 [T, k],
     top_lse fp32 [T] or None) to softmax(scale / temperature * h W^T).
     Returns (loss fp32 [T] or scalar, state for head_distill_grad)."""
-    hp, Wp = _head_pair("head_distill", h, W)
-    _one_gpu("head_distill", h, top_val, top_idx, top_lse)
-    T = h.shape[0]
-    if top_val.dtype not in _lib.DTYPES or top_idx.dtype != torch.int32:
-        raise _lib.CrbqError("head_distill takes floating teacher logits and int32 tokens")
-    if top_val.dim() != 2 or top_val.shape != top_idx.shape or top_val.shape[0] != T or not (
-            1 <= top_val.shape[1] <= _lib.HEAD_MAX_K):
-        raise _lib.CrbqError(f"head_distill takes teacher logits and tokens [T, k], k up to "
-                             f"{_lib.HEAD_MAX_K}, not {tuple(top_val.shape)} and "
-                             f"{tuple(top_idx.shape)}")
-    if top_lse is not None and (top_lse.dtype != torch.float32 or top_lse.shape != (T,)):
-        raise _lib.CrbqError("head_distill takes an fp32 teacher log-sum-exp [T]")
-    if not temperature > 0:
-        raise _lib.CrbqError("head_distill takes a temperature above 0")
-    k = top_val.shape[1]
-    val = top_val if top_val.stride(1) == 1 and top_val.stride(0) >= k else top_val.contiguous()
-    idx = top_idx if top_idx.stride(1) == 1 and top_idx.stride(0) >= k else top_idx.contiguous()
-    tlse = top_lse.contiguous() if top_lse is not None else None
-    red = _reduction("head_distill", reduction)
-    lib = _lib.ready(h.device)
-    with _lib.on_device(h.device):
-        loss, state, ws, nws = _head_buffers(lib, hp, Wp, k, red, h.device)
-        check(lib.crbq_head_distill(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
-                                    _lib.DTYPES[h.dtype], T, Wp.shape[0], hp.shape[1],
-                                    val.data_ptr(), _lib.DTYPES[val.dtype], max(val.stride(0), k),
-                                    idx.data_ptr(), max(idx.stride(0), k), k, ptr(tlse),
-                                    float(scale), float(temperature), red, loss.data_ptr(),
-                                    state.data_ptr(), ws.data_ptr(), nws, stream_of(h)),
-              "crbq_head_distill")
-    return loss, state
+    top = top_args(h, top_val, top_idx, top_lse)
+    return distill_call(h, W, top[0].shape[1], scale, temperature, reduction).forward(top)
 
 
 def head_distill_grad(h: torch.Tensor, W: torch.Tensor, k: int, state: torch.Tensor,
@@ -697,19 +747,9 @@ def head_distill_grad(h: torch.Tensor, W: torch.Tensor, k: int, state: torch.Ten
     """(dh, dW) (None where not asked for) of head_distill's loss, called with
     k listed tokens and the same scale, temperature and reduction, times g
     (fp32, of the loss's shape)."""
-    hp, Wp = _head_pair("head_distill_grad", h, W)
-    red = _reduction("head_distill_grad", reduction)
-    lib = _lib.ready(h.device)
-    with _lib.on_device(h.device):
-        dh, dW, ws, nws, g = _grad_args("head_distill_grad", hp, Wp, state, k, g, red, need_h,
-                                        need_w, lib)
-        check(lib.crbq_head_distill_grad(hp.data_ptr(), hp.stride(0), Wp.data_ptr(), Wp.stride(0),
-                                         _lib.DTYPES[h.dtype], hp.shape[0], Wp.shape[0],
-                                         hp.shape[1], int(k), float(scale), float(temperature),
-                                         red, state.data_ptr(), g.data_ptr(),
-                                         *_out_args(dh, dW), ws.data_ptr(), nws, stream_of(h)),
-              "crbq_head_distill_grad")
-    return _cut(dh, h.shape[1]), _cut(dW, W.shape[1])
+    call = distill_call(h, W, int(k), scale, temperature, reduction, "head_distill_grad")
+    call.check_grad("head_distill_grad", state, g, need_h, need_w)
+    return call.grad(state, g.contiguous(), need_h, need_w)
 
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
@@ -717,7 +757,8 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     lowest index: (val [T, k], idx int32 [T, k], lse fp32 [T] of the row
     divided by temperature)."""
     _one_gpu("top_logits", logits)
-    if logits.dtype not in _lib.DTYPES:
+    dt = _lib.DTYPES.get(logits.dtype)
+    if dt is None:
         raise _lib.CrbqError(f"top_logits takes fp32, fp16 or bf16 logits, not {logits.dtype}")
     if logits.dim() != 2 or 0 in logits.shape:
         raise _lib.CrbqError(f"top_logits takes logits [T, V], not {tuple(logits.shape)}")
@@ -727,13 +768,16 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
         raise _lib.CrbqError(f"top_logits: k = {k} is not within 1..{min(V, _lib.HEAD_MAX_K)}")
     if not temperature > 0:
         raise _lib.CrbqError("top_logits takes a temperature above 0")
-    x = logits if logits.stride(1) == 1 and (T == 1 or logits.stride(0) >= V) else logits.contiguous()
-    lib = _lib.ready(x.device)
-    with _lib.on_device(x.device):
-        val = torch.empty((T, k), dtype=x.dtype, device=x.device)
-        idx = torch.empty((T, k), dtype=torch.int32, device=x.device)
-        lse = torch.empty(T, dtype=torch.float32, device=x.device)
-        check(lib.crbq_top_logits(x.data_ptr(), _lib.DTYPES[x.dtype], T, V, max(x.stride(0), V), k,
+    x = logits
+    if x.stride(1) != 1 or (T > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    dev = x.device
+    lib = _lib.ready(dev)
+    with _lib.on_device(dev):
+        val = torch.empty((T, k), dtype=x.dtype, device=dev)
+        idx = torch.empty((T, k), dtype=torch.int32, device=dev)
+        lse = torch.empty(T, dtype=torch.float32, device=dev)
+        check(lib.crbq_top_logits(x.data_ptr(), dt, T, V, max(x.stride(0), V), k,
                                   float(temperature), val.data_ptr(), idx.data_ptr(),
                                   lse.data_ptr(), stream_of(x)), "crbq_top_logits")
     return val, idx, lse
