@@ -2,15 +2,17 @@
 // index) and the row's log-sum-exp: what a teacher leaves behind for
 // distillation instead of its logits.
 //
-// One workgroup of 1024 threads a row.  One pass over the row takes each
+// One workgroup a row (1024 threads, or fewer).  One pass over the row takes each
 // thread's largest logit and its sum of exponentials against that (rescaled
 // the few times the largest one rises): 8.5 vector instructions' time an
 // element, below the time its bytes take.  The k-th largest of
-// the 1024 maxima is a lower bound of the row's k-th largest logit that only about
+// the threads' maxima is a lower bound of the row's k-th largest logit that only about
 // k elements reach (with k of 1024 threads hit, -1024 log(1 - k / 1024)
-// elements: 137 for k = 128); the threads whose maximum reaches it read their
-// elements again and collect those that do, which are then ranked by
-// counting.  Rows whose ties leave more candidates than the list holds (a
+// elements: 137 for k = 128).  Each thread keeps the largest logit of each of
+// its 16-byte groups (every 16th of them where it has more than 16) and reads
+// those groups again that reach the bound: about k of them, where all groups of all threads
+// whose maximum reaches it cost as much as the row over again (2047 rows of 128256: 85
+// us of 200).  What they hold above the bound is ranked by counting.  Rows whose ties leave more candidates than the list holds (a
 // constant row, a row masked to one value) and rows with a NaN are selected
 // exactly, by digits of the key.
 // Logits are compared as whole numbers in the order of the values (-0 as
@@ -19,10 +21,8 @@
 
 namespace crbq {
 
-constexpr int TL_THREADS = 1024;
-constexpr int TL_WAVES = TL_THREADS / 64;
-constexpr int TL_CAP = 2048;            // candidates
-constexpr int TL_SCALAR = 8192;         // rows up to this: one element a thread and step
+constexpr int TL_SCALAR = 2560;         // rows up to this: one element a thread and step
+constexpr int TL_GROUPS = 16;           // group maxima a thread keeps
 
 template <typename E> struct TL;
 template <> struct TL<float> {
@@ -59,7 +59,7 @@ template <> struct TL<__bf16> : TL16<0x7f80> {
 
 // A row as the threads share it: 16-byte groups from the first 16-byte boundary
 // on (long rows), elements one by one before and behind.
-template <typename E>
+template <typename E, int NT>
 struct TLRow {
   typedef typename TL<E>::bits B;
   static constexpr int N = 16 / sizeof(B);
@@ -81,13 +81,13 @@ struct TLRow {
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
     const int tid = threadIdx.x;
-    for (int64_t i = tid; i < nv; i += TL_THREADS) {
+    for (int64_t i = tid; i < nv; i += NT) {
       const uint4 u = q[i];
 #pragma unroll
       for (int e = 0; e < N; ++e) f((int)(head + i * N + e), bits(u, e));
     }
-    for (int64_t i = tid; i < head; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
-    for (int64_t i = head + nv * N + tid; i < V; i += TL_THREADS) f((int)i, (uint32_t)x[i]);
+    for (int64_t i = tid; i < head; i += NT) f((int)i, (uint32_t)x[i]);
+    for (int64_t i = head + nv * N + tid; i < V; i += NT) f((int)i, (uint32_t)x[i]);
   }
 };
 
@@ -108,14 +108,17 @@ struct TLSum {
   }
 };
 
-template <typename E>
-__global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, int64_t V,
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void k_top_logits(const void* logits, int64_t V,
                                                            int64_t ld, int k, float itemp,
                                                            void* val, int32_t* __restrict__ idx,
                                                            float* __restrict__ lse) {
+  constexpr int TL_WAVES = NT / 64;
+  constexpr int TL_LOG = NT == 1024 ? 4 : NT == 512 ? 3 : 2;     // log2 of the wavefronts
+  constexpr int TL_CAP = NT == 256 ? 1024 : 2048;                // candidates
   typedef TL<E> L;
   typedef typename L::bits B;
-  __shared__ uint32_t tmax[TL_THREADS];
+  __shared__ uint32_t tmax[NT];
   __shared__ uint64_t cand[TL_CAP];     // key << 32 | ~index: larger is earlier
   __shared__ float wred[TL_WAVES], wsum[TL_WAVES];
   __shared__ int hist[256];
@@ -124,38 +127,47 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
   const int64_t t = blockIdx.x;
   const B* x = (const B*)logits + t * ld;
 
-  const TLRow<E> row(x, V);
-  constexpr int N = TLRow<E>::N;
+  const TLRow<E, NT> row(x, V);
+  constexpr int N = TLRow<E, NT>::N;
   const float c = itemp * 1.4426950408889634f;
   TLSum acc;
   auto group = [&](const uint4& u) __attribute__((always_inline)) {
     float v[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = L::f(TLRow<E>::bits(u, e));
+    for (int e = 0; e < N; ++e) v[e] = L::f(TLRow<E, NT>::bits(u, e));
     float top = v[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
     acc.rise(top, c);
 #pragma unroll
     for (int e = 0; e < N; ++e) acc.add(v[e], c);
+    return top;
   };
-  int64_t g = tid;
-  for (; g + 3 * TL_THREADS < row.nv; g += 4 * TL_THREADS) {
-    uint4 u[4];
+  float gm[TL_GROUPS];                                 // maximum of groups i, i + 16, ...
 #pragma unroll
-    for (int d = 0; d < 4; ++d) u[d] = row.q[g + d * TL_THREADS];
+  for (int i = 0; i < TL_GROUPS; ++i) gm[i] = -INFINITY;
+  for (int64_t g0 = tid; g0 - tid < row.nv; g0 += (int64_t)TL_GROUPS * NT) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d) group(u[d]);
+    for (int i0 = 0; i0 < TL_GROUPS; i0 += 4) {
+      const int64_t g = g0 + (int64_t)i0 * NT;
+      if (g - tid >= row.nv) break;
+      uint4 u[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        u[d] = row.q[g + d * NT < row.nv ? g + d * NT : row.nv - 1];
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (g + d * NT < row.nv) gm[i0 + d] = fmaxf(gm[i0 + d], group(u[d]));
+    }
   }
-  for (; g < row.nv; g += TL_THREADS) group(row.q[g]);
   auto one = [&](int64_t i) __attribute__((always_inline)) {
     const float v = L::f((uint32_t)x[i]);
     acc.rise(v, c);
     acc.add(v, c);
   };
-  for (int64_t i = tid; i < row.head; i += TL_THREADS) one(i);
-  for (int64_t i = row.head + row.nv * N + tid; i < V; i += TL_THREADS) one(i);
-  const bool some = V >= TL_THREADS || tid < V;        // threads without an element: key 0
+  for (int64_t i = tid; i < row.head; i += NT) one(i);
+  for (int64_t i = row.head + row.nv * N + tid; i < V; i += NT) one(i);
+  const bool some = V >= NT || tid < V;        // threads without an element: key 0
   const uint32_t best = some ? L::key(L::bits_of(acc.m)) : 0;
   tmax[tid] = best;
   if (tid == 0) sh[1] = 0;
@@ -172,35 +184,70 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
                          ? acc.s : acc.s * __builtin_amdgcn_exp2f((acc.ref - ref) * c);
   const float sum = wave_sum_f(part);
   if (lane == 0) wsum[wave] = sum;
-  // k-th largest of the 1024, by its bits from the top
-  if (wave == 0) {
-    uint32_t mine[TL_WAVES], thr = 0;
+  // the k-th largest of the maxima, TL_LOG bits at a time from the top:
+  // wavefront w counts the maxima that reach w as the next bits (one wavefront
+  // bit by bit waits for a count as often as there are bits)
+  uint32_t mine[TL_WAVES], thr = 0;
 #pragma unroll
-    for (int w = 0; w < TL_WAVES; ++w) mine[w] = tmax[w * 64 + lane];
+  for (int w = 0; w < TL_WAVES; ++w) mine[w] = tmax[w * 64 + lane];
+  constexpr int STEPS = (L::DIGITS * 8 + TL_LOG - 1) / TL_LOG;
 #pragma unroll 1
-    for (int bit = L::DIGITS * 8 - 1; bit >= 0; --bit) {
-      const uint32_t c = thr | (1u << bit);
-      int n = 0;
+  for (int d = STEPS - 1; d >= 0; --d) {
+    // (the top step may have bits that no key has)
+    const uint64_t want = thr | (uint64_t)wave << (TL_LOG * d);
+    int n = 0;
 #pragma unroll
-      for (int w = 0; w < TL_WAVES; ++w) n += __popcll(__ballot(mine[w] >= c));
-      if (n >= k) thr = c;
-    }
-    if (lane == 0) sh[0] = thr;
+    for (int w = 0; w < TL_WAVES; ++w) n += __popcll(__ballot(mine[w] >= want));
+    int* cnt = hist + (d & 1) * TL_WAVES;
+    if (lane == 0) cnt[wave] = n;
+    __syncthreads();
+    const uint64_t ok = __ballot(lane < TL_WAVES && cnt[lane & (TL_WAVES - 1)] >= k);
+    thr |= (uint32_t)(63 - __clzll((long long)(ok | 1))) << (TL_LOG * d);
   }
-  __syncthreads();
-  const uint32_t thr = sh[0];
   float s = 0.f;
   for (int w = 0; w < TL_WAVES; ++w) s += wsum[w];
   const bool nan = !(s == s);
   if (tid == 0) lse[t] = nan || fabsf(top) < INFINITY ? ref * itemp + logf(s) : top;
-  if (best >= thr && !nan)
-    row.each([&](int i, uint32_t b) __attribute__((always_inline)) {
-      const uint32_t q = L::key(b);
-      if (q >= thr) {
-        const uint32_t at = atomicAdd(&sh[1], 1u);
-        if (at < TL_CAP) cand[at] = (uint64_t)q << 32 | (uint32_t)~i;
+  // candidates among n elements from i0 on
+  auto take = [&](const uint32_t (&key)[N], int i0, int n) __attribute__((always_inline)) {
+    uint32_t hit = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) hit |= (uint32_t)(e < n && key[e] >= thr) << e;
+    if (!hit) return;
+    uint32_t at = atomicAdd(&sh[1], (uint32_t)__popc(hit));
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if ((hit >> e) & 1) {
+        if (at < TL_CAP) cand[at] = (uint64_t)key[e] << 32 | (uint32_t)~(i0 + e);
+        ++at;
       }
-    });
+  };
+  auto take_one = [&](int64_t i) __attribute__((always_inline)) {
+    uint32_t key[N] = {};
+    key[0] = L::key((uint32_t)x[i]);
+    take(key, (int)i, 1);
+  };
+  if (best >= thr && !nan) {
+    uint32_t todo = 0;
+#pragma unroll
+    for (int i = 0; i < TL_GROUPS; ++i)
+      todo |= (uint32_t)(row.nv > tid && L::key(L::bits_of(gm[i])) >= thr) << i;
+    // (a lane's next group whatever the others': their loads run at one time)
+    while (todo) {
+      const int i = __ffs((int)todo) - 1;
+      todo &= todo - 1;
+      for (int64_t g = tid + (int64_t)i * NT; g < row.nv;
+           g += (int64_t)TL_GROUPS * NT) {
+        const uint4 u = row.q[g];
+        uint32_t key[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) key[e] = L::key(TLRow<E, NT>::bits(u, e));
+        take(key, (int)(row.head + g * N), N);
+      }
+    }
+    for (int64_t i = tid; i < row.head; i += NT) take_one(i);
+    for (int64_t i = row.head + row.nv * N + tid; i < V; i += NT) take_one(i);
+  }
   __syncthreads();
   int n = (int)sh[1];
   if (n > TL_CAP || nan) {
@@ -244,7 +291,7 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
     });
     __syncthreads();
     int have = (int)sh[1];              // k - need
-    for (int64_t i0 = 0; i0 < V && have < k; i0 += TL_THREADS) {
+    for (int64_t i0 = 0; i0 < V && have < k; i0 += NT) {
       const int64_t i = i0 + tid;
       const bool eq = i < V && L::key((uint32_t)x[i]) == pre;
       const uint64_t bits = __ballot(eq);
@@ -262,16 +309,33 @@ __global__ __launch_bounds__(TL_THREADS) void k_top_logits(const void* logits, i
     __syncthreads();
     n = k;
   }
-  for (int c = tid; c < n; c += TL_THREADS) {
+  for (int c = tid; c < n; c += NT) {
     const uint64_t q = cand[c];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand[j] > q;
+    int rank = 0, j = 0;
+    for (; j + 4 <= n; j += 4)
+      rank += (cand[j] > q) + (cand[j + 1] > q) + (cand[j + 2] > q) + (cand[j + 3] > q);
+    for (; j < n; ++j) rank += cand[j] > q;
     if (rank < k) {
       const int i = ~(int)(uint32_t)q;
       idx[t * k + rank] = i;
       ((B*)val)[t * k + rank] = x[i];
     }
   }
+}
+
+// Up to a row a CU: workgroups of 1024, for the row's latency.  More rows:
+// small workgroups, since after its pass over the row a workgroup mostly
+// waits, so that what counts is the rows at work on a CU (2, 4 or 8).  256 maxima
+// bound the k-th logit well for k up to 128 (177 candidates).
+template <typename E>
+static void top_logits(const void* logits, int64_t T, int64_t V, int64_t ld, int k, float it,
+                       void* val, int32_t* idx, float* lse, hipStream_t s) {
+  if (T <= 256)
+    k_top_logits<E, 1024><<<(unsigned)T, 1024, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
+  else if (k > 128)
+    k_top_logits<E, 512><<<(unsigned)T, 512, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
+  else
+    k_top_logits<E, 256><<<(unsigned)T, 256, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
 }
 
 }  // namespace crbq
@@ -288,15 +352,9 @@ extern "C" int crbq_top_logits(const void* logits, int dtype, int64_t T, int64_t
   hipStream_t s = (hipStream_t)stream;
   const float it = 1.f / temperature;
   switch (dtype) {
-    case CRBQ_F32:
-      k_top_logits<float><<<(unsigned)T, TL_THREADS, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
-      break;
-    case CRBQ_F16:
-      k_top_logits<_Float16><<<(unsigned)T, TL_THREADS, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
-      break;
-    case CRBQ_BF16:
-      k_top_logits<__bf16><<<(unsigned)T, TL_THREADS, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
-      break;
+    case CRBQ_F32: top_logits<float>(logits, T, V, ld, k, it, val, idx, lse, s); break;
+    case CRBQ_F16: top_logits<_Float16>(logits, T, V, ld, k, it, val, idx, lse, s); break;
+    case CRBQ_BF16: top_logits<__bf16>(logits, T, V, ld, k, it, val, idx, lse, s); break;
     default: return CRBQ_ERR_ARG;
   }
   CRBQ_LAUNCH_CHECK();
