@@ -325,14 +325,17 @@ __global__ __launch_bounds__(NT) void k_top_logits(const void* logits, int64_t V
 
 // Up to a row a CU: workgroups of 1024, for the row's latency.  More rows:
 // small workgroups, since after its pass over the row a workgroup mostly
-// waits, so that what counts is the rows at work on a CU (2, 4 or 8).  256 maxima
-// bound the k-th logit well for k up to 128 (177 candidates).
+// waits, so that what counts is the rows at work on a CU (2, 4 or 8): 4096 rows of
+// 8000, 256 threads 33 us, 512 70, 1024 120.  256 maxima bound the k-th logit well
+// for k up to 128 (177 candidates), and a thread's groups are read again one
+// by one while it has few: 2047 rows of 128256, 256 threads 152 us, 512 123; of
+// 50272, 66 and 73.
 template <typename E>
 static void top_logits(const void* logits, int64_t T, int64_t V, int64_t ld, int k, float it,
                        void* val, int32_t* idx, float* lse, hipStream_t s) {
   if (T <= 256)
     k_top_logits<E, 1024><<<(unsigned)T, 1024, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
-  else if (k > 128)
+  else if (k > 128 || V > 65536)
     k_top_logits<E, 512><<<(unsigned)T, 512, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
   else
     k_top_logits<E, 256><<<(unsigned)T, 256, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
