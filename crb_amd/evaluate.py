@@ -16,7 +16,10 @@ Differences in mechanism, not in result: everything stays on the model's
 device (the reference moves layers between host and device), and windows
 run through a layer in chunks of ``chunk`` (chunk=1 is the reference's
 per-window order).  Works on dense models and on models whose linears were
-replaced by PackedLinear.
+replaced by PackedLinear.  With fused=True the head and the cross entropy are
+one product (head.linear_cross_entropy) that keeps no logits: the loss of the
+fp32 logits, where the default, as the reference, rounds logits and each
+window's loss to the model's type.
 """
 from __future__ import annotations
 
@@ -24,6 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .head import linear_cross_entropy
 from .stack import _Catch, _first, _fit_batch, decoder_layers
 
 
@@ -93,10 +97,35 @@ def layer0_inputs(model: nn.Module, windows: torch.Tensor, chunk: int):
 
 
 @torch.no_grad()
+def final_hidden(model: nn.Module, windows: torch.Tensor, chunk: int = 8) -> torch.Tensor:
+    """Outputs [nsamples, seqlen, hidden] of the last decoder layer for token
+    windows [nsamples, seqlen], one layer at a time."""
+    inps, kw, kw_batch = layer0_inputs(model, windows, chunk)
+    outs = torch.empty_like(inps)
+    for layer in decoder_layers(model):
+        for j in range(0, windows.shape[0], chunk):
+            x = inps[j:j + chunk]
+            outs[j:j + x.shape[0]] = _first(layer(x, **_fit_batch(kw, x.shape[0], kw_batch)))
+        inps, outs = outs, inps
+    return inps
+
+
+def split_head(model: nn.Module):
+    """(the modules before the output head, the head, logit divisor); the head
+    as head.linear_cross_entropy takes it: an nn.Linear without bias."""
+    mods, scale = _head(model)
+    if not isinstance(mods[-1], nn.Linear) or mods[-1].bias is not None:
+        raise NotImplementedError(f"the output head of {type(model).__name__} is no nn.Linear "
+                                  "without bias")
+    return mods[:-1], mods[-1], scale
+
+
+@torch.no_grad()
 def eval_ppl(model: nn.Module, input_ids: torch.Tensor, seqlen: int, chunk: int = 8,
-             return_nlls: bool = False):
+             return_nlls: bool = False, fused: bool = False):
     """Perplexity of ``model`` on the token stream ``input_ids`` ([1, T] as
-    the reference's testenc.input_ids, or [T]) in windows of ``seqlen``."""
+    the reference's testenc.input_ids, or [T]) in windows of ``seqlen``;
+    fused: without logits (16-bit models on the GPU)."""
     if seqlen < 2:
         raise ValueError("seqlen must be at least 2")
     ids = input_ids.reshape(1, -1)
@@ -106,19 +135,22 @@ def eval_ppl(model: nn.Module, input_ids: torch.Tensor, seqlen: int, chunk: int 
     chunk = max(1, int(chunk))
     dev = next(model.parameters()).device
     windows = ids[:, :nsamples * seqlen].reshape(nsamples, seqlen).to(dev)
-    inps, kw, kw_batch = layer0_inputs(model, windows, chunk)
-    outs = torch.empty_like(inps)
-    for layer in decoder_layers(model):
-        for j in range(0, nsamples, chunk):
-            x = inps[j:j + chunk]
-            outs[j:j + x.shape[0]] = _first(layer(x, **_fit_batch(kw, x.shape[0], kw_batch)))
-        inps, outs = outs, inps
     mods, scale = _head(model)
+    if fused:
+        mods, head, _ = split_head(model)
+        # every token's label is the next one; the last of a window has none
+        labels = F.pad(windows[:, 1:].long(), (0, 1), value=-100)
+    inps = final_hidden(model, windows, chunk)
     nlls = []
     for j in range(0, nsamples, chunk):
         h = inps[j:j + chunk]
         for m in mods:
             h = m(h)
+        if fused:
+            rows = linear_cross_entropy(h, head.weight, labels[j:j + chunk], scale=1.0 / scale,
+                                        reduction="none")
+            nlls.extend(rows.sum(1) / (seqlen - 1) * seqlen)
+            continue
         logits = h / scale if scale != 1.0 else h
         for k in range(h.shape[0]):
             shift_logits = logits[k:k + 1, :-1, :].contiguous()

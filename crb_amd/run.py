@@ -25,7 +25,9 @@ blocksize, partition), with the minlayer / maxlayer / quant_only / invert
 filter of run.py:332-336.  Extensions: --refine_iters (CRB sign-refinement
 rounds; the reference has one), --layers (decoder layers to build), --pack
 (3-bit packed storage), --eval_tokens (perplexity on held-out synthetic
-windows, eval_ppl_utils.py:538-637).
+windows, eval_ppl_utils.py:538-637), --fused_eval (that without keeping
+logits), --recover_steps N (the final norm and the head tuned against the dense
+model's --recover_topk top logits, crb_amd/recover.py).
 """
 from __future__ import annotations
 
@@ -88,6 +90,10 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--pack", action="store_true")
     p.add_argument("--token_file", type=str, default=None)
     p.add_argument("--eval_tokens", type=int, default=0)
+    p.add_argument("--fused_eval", action="store_true")
+    p.add_argument("--recover_steps", type=int, default=0)
+    p.add_argument("--recover_topk", type=int, default=64)
+    p.add_argument("--recover_lr", type=float, default=1e-4)
     return p
 
 
@@ -165,6 +171,9 @@ def main(argv=None) -> dict:
     model = build_model(key, args.layers, dev, args.seed)
     seqlen = args.seqlen or model.seqlen
     samples = calibration(args, model.config.vocab_size, seqlen).to(dev)
+    if args.recover_steps:
+        from .recover import recover_head, teacher_top
+        top = teacher_top(model, samples, args.recover_topk, chunk=args.chunk)
     tick = time.time()
     sq = StackQuantizer(model, **stack_kwargs(args))
     stats = sq.run(samples, verbose=True)
@@ -174,11 +183,16 @@ def main(argv=None) -> dict:
     out = {"model": args.model, "method": args.low_quant_method, "layers": len(stats),
            "quantization_time_s": qtime,
            "errors": [st.errors for st in stats]}
+    if args.recover_steps:
+        out["recover_losses"] = recover_head(model, samples, top, args.recover_steps,
+                                             args.recover_lr, chunk=args.chunk)
+        print("recovery: KL", out["recover_losses"][0], "->", out["recover_losses"][-1])
     if args.eval_tokens:
         from .evaluate import eval_ppl
         g = torch.Generator().manual_seed(args.seed + 1)
         ids = torch.randint(0, model.config.vocab_size, (1, args.eval_tokens), generator=g)
-        out["ppl"] = eval_ppl(model, ids.to(dev), seqlen, chunk=args.chunk)
+        out["ppl"] = eval_ppl(model, ids.to(dev), seqlen, chunk=args.chunk,
+                              fused=args.fused_eval)
         print("ppl", out["ppl"])
     print(json.dumps({k: v for k, v in out.items() if k != "errors"}))
     return out
