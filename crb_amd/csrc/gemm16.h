@@ -62,8 +62,8 @@ struct GOperand {
   int64_t kstep;           // elements from one 64 k to the next: 64 (KC), 64 ld (K-strided)
   int64_t rows;            // rows (outputs) from row0 to the end; K-strided: even
   int64_t K;               // k's that exist; KC: a multiple of 8
-  const uint64_t* live;    // K-strided only, may be null: bit k % 64 of word k / 64 clear =
-                           // row k reads as zeros, whatever it holds
+  const uint64_t* live;    // K-strided A, may be null: bit k % 64 of word k / 64 clear = row k
+                           // is not read but zeros (of a K-strided B too)
 };
 
 __device__ __forceinline__ i4_t g_rsrc(const uint16_t* base, int64_t nrec) {
@@ -518,8 +518,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   auto loadB = [&](auto uu, const Stage& s, int buf) __attribute__((always_inline)) {
     constexpr int u = decltype(uu)::value;
     char* d = mine + buf * G_STAGE + (4 + u) * G_UNIT;
-    // (a blocked K-strided B may hold anything behind A's last k)
-    const bool in = LB == G_KC_BLOCKED || (BKC ? UB.kc8 : UB.row) < s.k;
+    const bool in = BKC ? LB == G_KC_BLOCKED || UB.kc8 < s.k
+                        : !Job::MASKED || ((s.live >> UB.row) & 1);
     g_load_lds(d, s.rb, (in ? UB.voff : OUT) + (unsigned)(u * ub));
   };
   // A fragment (h, e) of unit u; B fragment (h, j)

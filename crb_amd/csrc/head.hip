@@ -27,8 +27,11 @@
 // that writes the piece's dz (16 bits, the operand of the two products that
 // follow), then dh += dz W (fp32 sums) and dW = dz^T h.  dz is rounded to the inputs'
 // type as the gradients themselves are: its error (at most 2^-8 or 2^-11 of it, independent
-// from element to element) is that of the final rounding again.  It is scaled by a
-// power of two (fp16) and by the largest row coefficient so that it stays in range.
+// from element to element) is that of the final rounding again.  Up to 64
+// tokens, where few elements of dz may make up a gradient and the products
+// wait for memory anyway, a second 16-bit part holds what the rounding left
+// (relative 2^-16).  dz is scaled by a power of two (fp16) and by the
+// largest row coefficient so that it stays in range.
 #include "gemm16.h"
 
 namespace crbq {
@@ -335,13 +338,16 @@ __global__ __launch_bounds__(G_THREADS) void k_head_fwd_p(const FwdArgs) {
 // distillation: p_T, the sum of p log p over the listed entries, m, and of the
 // lists' distinct tokens z [T][k], p [T][k] and, ascending, the tokens
 // themselves (int32) [T][k].  live is written with a sum or mean only.
+__host__ __device__ __forceinline__ int64_t live_words(int64_t T) {
+  return T <= 64 ? 2 : (T + 63) / 64;
+}
 struct State {
   uint64_t* live;
   float *inv, *a, *lse, *rowb, *ratio, *pt, *ent, *mass, *zt, *p;
   int32_t* sidx;
   __host__ __device__ State(float* b, int64_t T, int64_t k) {
     live = (uint64_t*)b;
-    inv = b + (T + 63) / 64 * 2;
+    inv = b + live_words(T) * 2;
     a = inv + 2;
     lse = a + T;
     rowb = lse + T;
@@ -354,7 +360,7 @@ struct State {
     sidx = (int32_t*)(p + T * k);
   }
   static int64_t floats(int64_t T, int64_t k) {
-    return (T + 63) / 64 * 2 + 2 + (k ? (3 * k + 7) * T : 5 * T);
+    return live_words(T) * 2 + 2 + (k ? (3 * k + 7) * T : 5 * T);
   }
 };
 
@@ -454,7 +460,10 @@ __global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ 
     const uint64_t bits = __ballot(on);
     if (t < T) s += rows[t];
     c += on ? 1.f : 0.f;
-    if ((threadIdx.x & 63) == 0) st.live[t0 / 64] = bits;
+    if ((threadIdx.x & 63) == 0) {
+      st.live[t0 / 64] = bits;
+      if (T <= 64) st.live[1] = bits;                  // of the second parts
+    }
   }
   s = wave_sum_f(s);
   c = wave_sum_f(c);
@@ -628,7 +637,10 @@ __global__ __launch_bounds__(64) void k_grad_rows(State st, int64_t T,
     rowb[t] = r == 0.f ? 0.f : st.rowb[t] * w;
   }
   const uint64_t bits = __ballot(!(r == 0.f));
-  if (threadIdx.x == 0) live[blockIdx.x] = bits;
+  if (threadIdx.x == 0) {
+    live[blockIdx.x] = bits;
+    if (T <= 64) live[1] = bits;                       // of the second parts
+  }
 }
 
 // What undoes the scaling of dz: f0 f1 mul (the loss's gradient or the largest
@@ -660,33 +672,49 @@ struct DzArgs {
 // piece (row by row, dW's loads went 64 KB from row to row: 0.53 of the time
 // with busy MFMAs against 0.72 of dh's).  The columns of whole tiles are
 // written, zeros behind nv; the rows behind T are not, and dh's tiles, which
-// read them, do not keep what comes of them.
+// read them, do not keep what comes of them.  Up to 64 tokens, rows 64 on hold the
+// second parts.
 __host__ __device__ __forceinline__ int64_t dz_cols(int64_t nv) { return (nv + 255) / 256 * 256; }
-__host__ __device__ __forceinline__ int64_t dz_rows(int64_t T) { return (T + 255) / 256 * 256; }
+__host__ __device__ __forceinline__ int64_t dz_rows(int64_t T) {
+  return T <= 64 ? 128 : (T + 255) / 256 * 256;
+}
 __device__ __forceinline__ uint16_t* dz_at(uint16_t* dz, int64_t zstep, int64_t t, int64_t v) {
   return dz + v / G_K * zstep + t * G_K + v % G_K;
 }
 
 // 4 consecutive tokens of a row, `left` of them within the vocabulary, the
-// label lab tokens on from the first
-template <typename T8>
+// label lab tokens on from the first; rest: what the rounding leaves (TWO)
+template <typename T8, bool TWO = false>
 __device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2, float b,
-                                         int64_t left, int lab) {
-  uint16_t o[4];
+                                         int64_t left, int lab, uint2* rest = nullptr) {
+  typedef typename Half<T8>::t H;
+  uint16_t o[4], l[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    o[r] = to16<T8>(b * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], scale2, -a2)));
+  for (int r = 0; r < 4; ++r) {
+    const float x = b * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[r], scale2, -a2));
+    o[r] = to16<T8>(x);
+    if (TWO) l[r] = to16<T8>(x - (float)__builtin_bit_cast(H, o[r]));
+  }
   if ((unsigned)lab < 4u) {
     const uint16_t y = to16<T8>(-b);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (r == lab) o[r] = y;
+      if (r == lab) {
+        o[r] = y;
+        if (TWO) l[r] = to16<T8>(-b - (float)__builtin_bit_cast(H, y));
+      }
   }
   if (left < 4) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (r >= left) o[r] = 0;
+      if (r >= left) {
+        o[r] = 0;
+        if (TWO) l[r] = 0;
+      }
   }
+  if (TWO)
+    *rest = b == 0.f ? make_uint2(0u, 0u)
+                     : make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
   const uint2 u = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
   return b == 0.f ? make_uint2(0u, 0u) : u;
 }
@@ -715,8 +743,10 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
     for (int i = 0; i < G::MI; ++i) {
       const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below dz_cols
       const int64_t o = y - v;
-      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8>(acc[i][j], scale2, a2, b, p.nv - v,
-                                                        o >= 0 && o < 4 ? (int)o : -1);
+      uint2 rest;
+      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8, true>(
+          acc[i][j], scale2, a2, b, p.nv - v, o >= 0 && o < 4 ? (int)o : -1, &rest);
+      *(uint2*)dz_at(p.dz, p.zstep, 64 + t, v) = rest;
     }
   }
 }
@@ -817,7 +847,12 @@ __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
   const int64_t v = st.sidx[e];
   if (v == PAD_IDX || v < vbeg || v >= vbeg + nv) return;
   const float r = ratio[t], d = st.mass[t] * expf(st.zt[e] - st.lse[t]) - st.p[e];
-  *dz_at(dz, zstep, t, v - vbeg) = r == 0.f ? (uint16_t)0 : to16<T8>(r * d);
+  const float x = r == 0.f ? 0.f : r * d;
+  const uint16_t o = to16<T8>(x);
+  *dz_at(dz, zstep, t, v - vbeg) = o;
+  if (T <= 64)
+    *dz_at(dz, zstep, 64 + t, v - vbeg) =
+        to16<T8>(x - (float)__builtin_bit_cast(typename Half<T8>::t, o));
 }
 
 // dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the
@@ -849,10 +884,11 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
   int tm, tn;
   const int lin = g_xcd(blockIdx.x, gridDim.x), split = lin / (p.nm * p.nn);
   g_band(lin - split * p.nm * p.nn, p.nm, p.nn, tm, tn);
-  const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * G::BN;
+  // n tile 0: the tokens, 1: their second parts (the same rows of W, from L2)
+  const int64_t c0 = (int64_t)tm * G::BM, t0 = (int64_t)tn * 64;
   const int64_t kb = split * p.span, ke = kb + p.span < p.nv ? kb + p.span : p.nv;
   const GOperand A{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, p.nv, nullptr};
-  const GOperand B{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
+  const GOperand B{p.dz + t0 * G_K, G_K, p.zstep, p.T, dz_cols(p.nv), nullptr};
   f4_t acc[G::MI][G::NJ];
   g_tile<T8, G>(smem, A, B, kb, ke, acc);
   const int lane = threadIdx.x & 63;
@@ -861,7 +897,7 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dh(const DhArgs p) {
   for (int j = 0; j < G::NJ; ++j)
 #pragma unroll
     for (int i = 0; i < G::MI; ++i)
-      dh_add(p, split, t0 + (wave % G::WGN) * G::WN + 16 * j + (lane & 15),
+      dh_add(p, 2 * split + tn, (wave % G::WGN) * G::WN + 16 * j + (lane & 15),
              c0 + (wave / G::WGN) * G::WM + 16 * i + 4 * (lane >> 4), acc[i][j]);
 }
 
@@ -926,8 +962,18 @@ __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int
   const int64_t n4 = T * (C / 4);
   const float f = fac.get();
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n4; e += (int64_t)gridDim.x * 256) {
-    float4 v = *(const float4*)(P + e * 4);
-    for (int s = 1; s < ns; ++s) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    int s = 0;
+    for (; s + 8 <= ns; s += 8) {
+      float4 u[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) u[d] = *(const float4*)(P + (int64_t)(s + d) * T * C + e * 4);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        v.x += u[d].x; v.y += u[d].y; v.z += u[d].z; v.w += u[d].w;
+      }
+    }
+    for (; s < ns; ++s) {
       const float4 u = *(const float4*)(P + (int64_t)s * T * C + e * 4);
       v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
     }
@@ -954,7 +1000,10 @@ struct DwJob {
   static constexpr bool MASKED = true;
   __device__ static int64_t lda() { return g_args<DwArgs>().ldh; }
   __device__ static int64_t ldb() { return G_K; }
-  __device__ static int64_t kstep_a() { return G_K * lda(); }
+  __device__ static int64_t kstep_a() {
+    const DwArgs p = g_args<DwArgs>();
+    return p.T <= 64 ? 0 : G_K * p.ldh;
+  }
   __device__ static int64_t kstep_b() { return G_K * G_K; }
   __device__ static int64_t unit_a() { return G_K; }
   __device__ static int64_t unit_b() { return g_args<DwArgs>().zstep; }
@@ -973,10 +1022,12 @@ struct DwJob {
     const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
     place(p, lin, c0, v0);
-    A = GOperand{p.h + c0, p.ldh, G_K * p.ldh, p.C - c0, p.T, p.live};
-    B = GOperand{p.dz + v0 / G_K * p.zstep, G_K, G_K * G_K, 256, p.T, nullptr};
+    // (up to 64 tokens: a second stage, the same tokens times the second parts)
+    const int64_t K = p.T <= 64 ? 128 : p.T;
+    A = GOperand{p.h + c0, p.ldh, kstep_a(), p.C - c0, K, p.live};
+    B = GOperand{p.dz + v0 / G_K * p.zstep, G_K, G_K * G_K, 256, K, nullptr};
     k = 0;
-    nch = (int)((p.T + G_K - 1) / G_K);
+    nch = (int)((K + G_K - 1) / G_K);
   }
   __device__ __forceinline__ void side(int, char*) const {}
   __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
@@ -1091,11 +1142,11 @@ struct GradWs {
     span = cdiv(cdiv(piece < V ? piece : V, dh_splits(T, C, piece)), G_K) * G_K;
     ns = (int)cdiv(piece < V ? piece : V, span);
     dz = w.take<uint16_t>((size_t)(dz_rows(T) * piece));
-    P = w.take<float>((size_t)(T * C) * ns);
+    P = w.take<float>((size_t)(T * C) * ns * (T <= 64 ? 2 : 1));
     rowb = w.take<float>((size_t)T);
     ratio = w.take<float>((size_t)T);
     gmax = w.take<float>(1);
-    live = w.take<uint64_t>((size_t)cdiv(T, 64));
+    live = w.take<uint64_t>((size_t)live_words(T));
     bytes = w.off;
     ok = w.ok();
   }
@@ -1208,9 +1259,10 @@ static int head_grad(const GradCall& c, const State& st, const GradWs& w, hipStr
     }
     if (c.dh) {
       const int mh = (int)cdiv(C, GH::BM);
-      const DhArgs q{Wv, w.dz, c.ldw, zstep, T, nv, C, w.span, mh, nt, (int)cdiv(nv, w.span), w.P,
+      const int nn = T <= 64 ? 2 : nt;
+      const DhArgs q{Wv, w.dz, c.ldw, zstep, T, nv, C, w.span, mh, nn, (int)cdiv(nv, w.span), w.P,
                      v > 0};
-      const int64_t tiles = (int64_t)mh * nt * q.ns;
+      const int64_t tiles = (int64_t)mh * nn * q.ns;
       if constexpr (std::is_same<GH, Big>::value)
         k_head_dh_p<T8><<<persistent(tiles), G_THREADS, 0, s>>>(q);
       else
@@ -1226,8 +1278,8 @@ static int head_grad(const GradCall& c, const State& st, const GradWs& w, hipStr
   }
   if (c.dh) {
     const int64_t nb = cdiv(T * (C / 4), 256);
-    k_dh_out<T8><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, s>>>(w.P, w.ns, T, C, fac, c.dh,
-                                                                   c.ldd);
+    k_dh_out<T8><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, s>>>(
+        w.P, w.ns * (T <= 64 ? 2 : 1), T, C, fac, c.dh, c.ldd);
     CRBQ_LAUNCH_CHECK();
   }
   return CRBQ_OK;

@@ -5,9 +5,9 @@ Tolerances.  z is a sum of C exact products in fp32: its error is taken as a
 random walk of C roundings, dz0 = 4 sqrt(C) 2^-24 max sum_c |s h W|.  A
 loss is a few exponentials and logarithms of such z (relative 2^-22 each)
 away: |error| <= 2 dz0 + 2^-21 (1 + max |z| + |loss|).  A gradient adds one rounding
-of every dz (u = 2^-8 bf16, 2^-11 fp16), fp32 sums, one rounding of the
-result and, in fp16, the spacing of subnormal numbers:
-  |error| <= (u + 2 dz0 + 2^-20 (1 + max |z|)) sum (q + p) |factor| + u |result| + tiny.
+of every dz (d = u = 2^-8 bf16, 2^-11 fp16; up to 64 tokens dz has two parts, d = u^2),
+fp32 sums, one rounding of the result and, in fp16, the spacing of subnormal numbers:
+  |error| <= (d + 2 dz0 + 2^-20 (1 + max |z|)) sum (q + p) |factor| + u |result| + tiny.
 """
 import math
 
@@ -45,7 +45,8 @@ def grad_refs(h, W, dz, both, dz0, z, s, dtype):
     """dz [T, V] (with the loss gradient's coefficient), both = q + p times
     its size: (dh, tolerance, dW, tolerance)."""
     hd, wd, u = h.double().cpu(), W.double().cpu(), U[dtype]
-    e = u + 2 * dz0 + 2.0 ** -20 * (1 + float(z.abs().max()))
+    d = u * u if h.shape[0] <= 64 else u
+    e = d + 2 * dz0 + 2.0 ** -20 * (1 + float(z.abs().max()))
     dh, dW = s * dz @ wd, s * dz.t() @ hd
     th = abs(s) * e * (both @ wd.abs()) + u * dh.abs() + TINY[dtype]
     tw = abs(s) * e * (both.t() @ hd.abs()) + u * dW.abs() + TINY[dtype]
