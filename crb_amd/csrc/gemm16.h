@@ -333,6 +333,15 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
 // for; issued earlier within that half they stood in each other's way.)
 // The stages of consecutive tiles follow on each other without a gap, so a tile's
 // first loads run under the last stages and the epilogue of the one before.
+//
+// A workgroup takes the tiles lin, lin + gridDim, ... of a Job:
+//   tiles(), stages(lin) >= 1         how many, and the 64-k stages of one
+//   lda(), kstep_a(), unit_a(), ..b   row strides; elements from one 64 k, one unit to the next
+//   tile(lin, A, B, k, nch)           a tile's operands, first k (a multiple of 64) and stages
+//   side(lin, priv)                   loads what finish needs into the wavefront's own G_PRIV
+//                                     bytes of LDS (g_load_lds*), a tile's products ahead
+//   finish(lin, priv, acc)            the epilogue
+//   MASKED                            A (and a K-strided B) have live rows
 // ---------------------------------------------------------------------------
 constexpr int G_UNIT = 8192, G_STAGE = 8 * G_UNIT, G_RING = 2 * G_STAGE;
 constexpr int G_THREADS = 512;
@@ -463,29 +472,24 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   const int nwg = gridDim.x, first = g_xcd(blockIdx.x, nwg);
   if (first >= tiles) return;                          // no tile at all
 
-  // The stages in load order: stage lc of a tile of ln; then the next tile, whose
-  // operands are at hand.  A tile has at least 4 stages (the last ones behind
-  // A's last k, so zeros, if need be), so that it is enough to look at one tile ahead, at
-  // the end of each.
-  GCursor<LA> ca, na;
-  GCursor<LB> cb, nb;
-  const uint64_t *cl = nullptr, *nl = nullptr;
-  int lc = 0, ln = 0, nn = 0;
-  auto peek = [&](int lin) __attribute__((always_inline)) {      // the next tile: na, nb, nl, nn
-    GOperand A, B;
-    int64_t k;
-    na.k = nb.k = 0;
-    nn = 1 << 30;
-    nl = nullptr;
-    na.rows = nb.rows = 1;
-    na.p = nb.p = nullptr;
-    if (lin < tiles) {
-      job.tile(lin, A, B, k, nn);
-      nn = g_uni(nn < 4 ? 4 : nn);
-      na.open(A, k);
-      nb.open(B, k);
-      if (!AKC && A.live) nl = g_uni(A.live + k / G_K);
+  // The stages in load order: stage lc of the ln of tile ll.
+  GCursor<LA> ca;
+  GCursor<LB> cb;
+  const uint64_t* cl = nullptr;
+  int ll = first, lc = 0, ln = 0;
+  auto open = [&]() __attribute__((always_inline)) {
+    ca.k = cb.k = 0;
+    ln = 1 << 30;                                      // behind the last tile: no data, no end
+    if (ll < tiles) {
+      GOperand A, B;
+      int64_t k;
+      job.tile(ll, A, B, k, ln);
+      ln = g_uni(ln);
+      ca.open(A, k);
+      cb.open(B, k);
+      if (!AKC && A.live) cl = g_uni(A.live + k / G_K);
     }
+    lc = 0;
   };
   struct Stage {
     i4_t ra, rb;
@@ -500,11 +504,8 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
     ca.advance(ka);
     cb.advance(kb);
     if (++lc == ln) {
-      ca = na;
-      cb = nb;
-      cl = nl;
-      ln = nn;
-      lc = 0;
+      ll += nwg;
+      open();
     }
     return s;
   };
@@ -534,13 +535,7 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
   constexpr std::integral_constant<int, 2> _2{};
   constexpr std::integral_constant<int, 3> _3{};
 
-  peek(first);
-  ca = na;
-  cb = nb;
-  cl = nl;
-  ln = nn;
-  int nch = nn;                                        // stages of the tile at work
-  peek(first + nwg);
+  open();
   // stage 0, what stage 1 needs early, then B's units 0 and 1 of stage 2 over stage 0's
   Stage s1, s2;
   {
@@ -619,6 +614,7 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc.v[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
     job.side(lin, priv);
+    const int nch = g_uni(job.stages(lin));
     int c = 0;
     for (; c + 2 <= nch; c += 2) {
       stage(par, b0, b1);
@@ -630,9 +626,7 @@ __device__ __forceinline__ void g_run(char* smem, const Job& job) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) b0[q] = b1[q];
     }
-    nch = ln;                                          // the cursor is in the next tile
     job.finish(lin, priv, acc);
-    peek(lin + 2 * nwg);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // priv is free for the next side()
   }
   g_wait_vm<0>();

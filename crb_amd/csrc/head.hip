@@ -253,6 +253,7 @@ struct FwdJob {
     v0 = (int64_t)tm * 256;
     t0 = (int64_t)tn * 256;
   }
+  __device__ static int stages(int) { return (int)((g_args<FwdArgs>().C + G_K - 1) / G_K); }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
     const FwdArgs p = g_args<FwdArgs>();
@@ -262,7 +263,7 @@ struct FwdJob {
     A = GOperand{p.W + v0 * p.ldw, p.ldw, G_K, p.V - v0, p.C, nullptr};
     B = GOperand{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
     k = 0;
-    nch = (int)((p.C + G_K - 1) / G_K);
+    nch = stages(lin);
   }
   // the labels (or the tile's 8 mask words) of the wavefront's 2 x 32 rows
   __device__ __forceinline__ void side(int lin, char* priv) const {
@@ -770,6 +771,7 @@ struct DzJob {
     v0 = (int64_t)tm * 256;
     t0 = (int64_t)tn * 256;
   }
+  __device__ static int stages(int) { return (int)((g_args<DzArgs>().C + G_K - 1) / G_K); }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
     const DzArgs p = g_args<DzArgs>();
@@ -778,7 +780,7 @@ struct DzJob {
     A = GOperand{p.W + v0 * p.ldw, p.ldw, G_K, p.nv - v0, p.C, nullptr};
     B = GOperand{p.h + t0 * p.ldh, p.ldh, G_K, p.T - t0, p.C, nullptr};
     k = 0;
-    nch = (int)((p.C + G_K - 1) / G_K);
+    nch = stages(lin);
   }
   // a, rowb and label of the wavefront's 2 x 32 rows (64 words of each)
   __device__ __forceinline__ void side(int lin, char* priv) const {
@@ -920,6 +922,11 @@ struct DhJob {
     c0 = (int64_t)tm * 256;
     t0 = (int64_t)tn * 256;
   }
+  __device__ static int stages(int lin) {
+    const DhArgs p = g_args<DhArgs>();
+    const int64_t k = lin / (p.nm * p.nn) * p.span, n = p.nv - k < p.span ? p.nv - k : p.span;
+    return (int)((n + G_K - 1) / G_K);                 // n > 0 for every split of a launch
+  }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
     const DhArgs p = g_args<DhArgs>();
@@ -927,10 +934,9 @@ struct DhJob {
     int split;
     place(p, lin, c0, t0, split);
     k = split * p.span;
-    const int64_t end = p.nv < k + p.span ? p.nv : k + p.span;   // > k for every split of a launch
-    A = GOperand{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, end, nullptr};
+    A = GOperand{p.W + c0, p.ldw, G_K * p.ldw, p.C - c0, p.nv, nullptr};
     B = GOperand{p.dz + t0 * G_K, G_K, p.zstep, p.T - t0, dz_cols(p.nv), nullptr};
-    nch = (int)((end - k + G_K - 1) / G_K);
+    nch = stages(lin);
   }
   __device__ __forceinline__ void side(int, char*) const {}
   __device__ __forceinline__ void finish(int lin, char*, GAcc& acc) const {
@@ -1017,17 +1023,21 @@ struct DwJob {
     c0 = (int64_t)tm * 256;
     v0 = (int64_t)tn * 256;
   }
+  // up to 64 tokens: a second stage, the same tokens times the second parts
+  __device__ static int64_t K() {
+    const int64_t T = g_args<DwArgs>().T;
+    return T <= 64 ? 128 : T;
+  }
+  __device__ static int stages(int) { return (int)((K() + G_K - 1) / G_K); }
   __device__ __forceinline__ void tile(int lin, GOperand& A, GOperand& B, int64_t& k,
                                        int& nch) const {
     const DwArgs p = g_args<DwArgs>();
     int64_t c0, v0;
     place(p, lin, c0, v0);
-    // (up to 64 tokens: a second stage, the same tokens times the second parts)
-    const int64_t K = p.T <= 64 ? 128 : p.T;
-    A = GOperand{p.h + c0, p.ldh, kstep_a(), p.C - c0, K, p.live};
-    B = GOperand{p.dz + v0 / G_K * p.zstep, G_K, G_K * G_K, 256, K, nullptr};
+    A = GOperand{p.h + c0, p.ldh, kstep_a(), p.C - c0, K(), p.live};
+    B = GOperand{p.dz + v0 / G_K * p.zstep, G_K, G_K * G_K, 256, K(), nullptr};
     k = 0;
-    nch = (int)((K + G_K - 1) / G_K);
+    nch = stages(lin);
   }
   __device__ __forceinline__ void side(int, char*) const {}
   __device__ __forceinline__ void finish(int lin, char* priv, GAcc& acc) const {
