@@ -177,7 +177,7 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
   }
-  m = gmax4(p.scale == 0.f && m != -INFINITY ? 0.f : m * scale2);
+  m = gmax4(m * scale2);
   const float mb = m == -INFINITY ? 0.f : m;           // nothing left: 2^-inf = 0
   float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -1168,7 +1168,7 @@ static bool bad_matrix(const void* p, int64_t ld, int64_t C) {
 static int check_head(const void* h, int64_t ldh, const void* W, int64_t ldw, int dtype,
                       int64_t T, int64_t V, int64_t C) {
   if (dtype != CRBQ_F16 && dtype != CRBQ_BF16) return CRBQ_ERR_ARG;
-  if (T < 1 || V < 1 || C < 8 || (C & 7) || V >= ((int64_t)1 << 31) - 256 ||
+  if (T < 1 || V < 1 || C < 8 || (C & 7) || V >= ((int64_t)1 << 28) ||
       T >= ((int64_t)1 << 22))
     return CRBQ_ERR_ARG;
   if (bad_matrix(h, ldh, C) || bad_matrix(W, ldw, C)) return CRBQ_ERR_ARG;
@@ -1304,7 +1304,10 @@ static int head_grad_t(const GradCall& c, const State& st, const GradWs& w, hipS
   }
 }
 
+// (a scale of 0 would make the -inf of what is left out a NaN)
+static bool bad_scale(float s) { return !(fabsf(s) > 0.f) || !(fabsf(s) < INFINITY); }
 static bool bad_state(const void* p) { return !p || (((uintptr_t)p) & 7); }
+static bool bad_ws(const void* p) { return (((uintptr_t)p) & 15) != 0; }
 static bool bad_reduction(int r) { return r != CRBQ_NONE && r != CRBQ_MEAN && r != CRBQ_SUM; }
 
 }  // namespace crbq
@@ -1327,7 +1330,9 @@ extern "C" int crbq_head_xent(const void* h, int64_t ldh, const void* W, int64_t
                               int64_t ignore_index, float scale, int reduction, float* loss,
                               float* state, void* ws, size_t ws_bytes, void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!labels || !loss || bad_state(state) || bad_reduction(reduction)) return CRBQ_ERR_ARG;
+  if (!labels || !loss || bad_state(state) || bad_reduction(reduction) || bad_scale(scale) ||
+      bad_ws(ws))
+    return CRBQ_ERR_ARG;
   bool ok;
   const FwdWs w(ws, ws_bytes, T, V, 0, ok);
   if (!ok) return CRBQ_ERR_WORKSPACE;
@@ -1348,7 +1353,8 @@ extern "C" int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, in
                                    void* dW, int64_t ldo, void* ws, size_t ws_bytes,
                                    void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!labels || bad_state(state) || !g || (!dh && !dW) || bad_reduction(reduction))
+  if (!labels || bad_state(state) || !g || (!dh && !dW) || bad_reduction(reduction) || bad_scale(scale) ||
+      bad_ws(ws))
     return CRBQ_ERR_ARG;
   if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
   bool ok;
@@ -1369,7 +1375,8 @@ extern "C" int crbq_head_distill(const void* h, int64_t ldh, const void* W, int6
                                  size_t ws_bytes, void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
   if (!top_val || !top_idx || !loss || bad_state(state) || bad_reduction(reduction) || k < 1 ||
-      k > CRBQ_HEAD_MAX_K || ldv < k || ldi < k || !(temperature > 0.f))
+      k > CRBQ_HEAD_MAX_K || ldv < k || ldi < k || !(temperature > 0.f) ||
+      bad_scale(scale * (1.f / temperature)) || bad_ws(ws))
     return CRBQ_ERR_ARG;
   if (val_dtype != CRBQ_F32 && val_dtype != CRBQ_F16 && val_dtype != CRBQ_BF16)
     return CRBQ_ERR_ARG;
@@ -1405,7 +1412,8 @@ extern "C" int crbq_head_distill_grad(const void* h, int64_t ldh, const void* W,
                                       void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
   if (bad_state(state) || !g || (!dh && !dW) || k < 1 || k > CRBQ_HEAD_MAX_K ||
-      !(temperature > 0.f) || bad_reduction(reduction))
+      !(temperature > 0.f) || bad_reduction(reduction) ||
+      bad_scale(scale * (1.f / temperature)) || bad_ws(ws))
     return CRBQ_ERR_ARG;
   if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
   bool ok;

@@ -610,6 +610,9 @@ class _HeadCall:
         self.h, self.W, self.C = h, W, C         # C: the channels that are not padding
         self.labels, self.k = labels, k
         self.scale, self.temperature, self.red = scale, temperature, red
+        if not 0 < abs(scale / temperature) < float("inf"):
+            raise _lib.CrbqError(f"the logits' scale {scale} / {temperature} has to be finite and "
+                                 "not 0")
         self.lib = _lib.ready(h.device)
         self.dt = _lib.DTYPES[h.dtype]
 

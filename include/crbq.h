@@ -357,7 +357,7 @@ int crbq_linear_packed(const uint8_t* codes, int64_t ldc, const void* lut, const
  * No counterpart in the reference, whose perplexity forms all logits and
  * calls a cross entropy (eval_ppl_utils.py:626-636).  Hidden states h [T][C]
  * and the head's weight W [V][C], both fp16 or both bf16 (16-byte aligned,
- * row strides multiples of 8 below 2^22, C a multiple of 8, T below 2^22); logits
+ * row strides multiples of 8 below 2^22, C a multiple of 8, T below 2^22, V below 2^28); logits
  * z = scale * h W^T are computed piece by piece in fp32 and never kept.
  *
  * crbq_head_xent: loss_t = log sum_v exp z[t][v] - z[t][labels[t]].
@@ -383,7 +383,9 @@ int crbq_linear_packed(const uint8_t* codes, int64_t ldc, const void* lut, const
  *   (dW [V][ldo]) in the inputs' dtype; either may be NULL.  The logits are
  *   computed again; sums are fp32, in a fixed order.  A left-out row of h
  *   is not read into dW.
- * crbq_head_workspace_size(T, V, C, k, grad): bytes of ws for either. */
+ * scale (and scale / temperature) is finite and not 0.  Outputs overlap no input.
+ * crbq_head_workspace_size(T, V, C, k, grad): bytes of ws (16-byte aligned)
+ * for either. */
 enum crbq_reduction { CRBQ_NONE = 0, CRBQ_MEAN = 1, CRBQ_SUM = 2 };
 #define CRBQ_HEAD_MAX_K 256
 size_t crbq_head_state_floats(int64_t T, int64_t k);

@@ -251,6 +251,41 @@ def test_distill_odd_lists():
         assert not h2.grad[1:3].any()
 
 
+def test_distill_teacher_that_does_not_add_up():
+    """A log-sum-exp below that of the listed logits: probabilities above 1 in
+    sum, no tail; the gradient is still the loss's."""
+    from crb_amd.head import linear_distill
+    T, V, C, k = 70, 300, 64, 6
+    h, W, _ = make(T, V, C, torch.bfloat16, 21)
+    val, idx = teacher(T, V, k, 6)
+    lse = torch.logsumexp(val, 1) - 0.25
+    z, dz0, loss, dz, both = ref_distill(h, W, val, idx, lse, 1.0, 1.0, torch.ones(T).double())
+    h.requires_grad_(), W.requires_grad_()
+    rows = linear_distill(h, W, (val, idx, lse), reduction="none")
+    more = 2.0 ** -20 * (2 * float(z.abs().max()) + math.log(V) + 16)
+    close(rows.detach(), loss, 2 * (loss_tol(z, dz0, loss) + more), "rows")
+    got = torch.autograd.grad(rows, (h, W), torch.ones(T, device=DEV))
+    dh, th, dW, tw = grad_refs(h.detach(), W.detach(), dz, both, dz0, z, 1.0, torch.bfloat16)
+    close(got[0], dh, th, "dh")
+    close(got[1], dW, tw, "dW")
+
+
+@pytest.mark.parametrize("T", [1, 64, 65, 200])
+def test_tile_edges_of_tokens(T):
+    """Token counts around the tiles' edges, hidden states of one stage."""
+    from crb_amd.head import linear_cross_entropy
+    V, C = 513, 64
+    h, W, y = make(T, V, C, torch.float16, T)
+    z, dz0, loss, dz, both = ref_xent(h, W, y, 1.0, -100, torch.ones(T).double())
+    h.requires_grad_(), W.requires_grad_()
+    out = linear_cross_entropy(h, W, y, reduction="sum")
+    close(out.detach(), loss.sum(), loss_tol(z, dz0, loss).sum(), "sum")
+    got = torch.autograd.grad(out, (h, W))
+    dh, th, dW, tw = grad_refs(h.detach(), W.detach(), dz, both, dz0, z, 1.0, torch.float16)
+    close(got[0], dh, th, "dh")
+    close(got[1], dW, tw, "dW")
+
+
 def test_distill_nothing_listed():
     from crb_amd.head import linear_distill
     h, W, _ = make(3, 40, 16, torch.bfloat16)
@@ -544,6 +579,8 @@ def test_refusals():
         lambda: head.linear_cross_entropy(h.cpu(), W.cpu(), y.cpu()),
         lambda: head.linear_cross_entropy(h, W, y.cpu()),
         lambda: head.linear_cross_entropy(h[:0], W, y[:0]),
+        lambda: head.linear_cross_entropy(h, W, y, scale=0.0),
+        lambda: head.linear_cross_entropy(h, W, y, scale=float("nan")),
         lambda: head.linear_distill(h, W, (val, idx.long(), None)),
         lambda: head.linear_distill(h, W, (val[:, :2], idx, None)),
         lambda: head.linear_distill(h, W, (val[:2], idx[:2], None)),

@@ -53,7 +53,8 @@ def top(**kw):
 ODD = ctypes.c_void_p(0x7f0000100002)
 MATRIX = [dict(h=None), dict(W=None), dict(h=ODD), dict(W=ODD), dict(ldh=63), dict(ldh=56),
           dict(ldw=68), dict(ldw=1 << 22), dict(dtype=0), dict(dtype=3), dict(T=0), dict(V=0),
-          dict(C=0), dict(C=60), dict(C=4), dict(T=1 << 31), dict(V=1 << 31)]
+          dict(C=0), dict(C=60), dict(C=4), dict(T=1 << 22), dict(V=1 << 28),
+          dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(ws=ODD, nws=1 << 40)]
 
 
 @pytest.mark.parametrize("call", [xent, xent_grad, distill, distill_grad])
