@@ -365,40 +365,38 @@ struct State {
   }
 };
 
-// Joins a row's partial sums and finishes its loss; WPR wavefronts a row (a
-// whole workgroup where rows are few: one wavefront alone takes 26 us for the 4008
-// pairs of one row of 128256 tokens).  A row that is left out (ignored label,
-// empty list) has loss 0 and live 0.
-template <bool XENT, int WPR>
+// Joins a row's partial sums and finishes its loss, a workgroup a row (with one
+// wavefront a row, 26 us instead of 7 for one row of 128256 tokens, 4008 pairs; no faster
+// at 4094 rows either).  Bound by the start of the launch and the pairs' way from
+// memory: 2047 rows of 128256 tokens, 16 MB, in 8 us.  A row that is left out (ignored
+// label, empty list) has loss 0 and live 0.
+template <bool XENT>
 __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ part, int64_t npart,
-                                                   int64_t T, int64_t V, int k,
+                                                   int64_t V, int k,
                                                    const int64_t* __restrict__ labels,
                                                    int64_t ignore, State st, float zscale,
                                                    float* rows, uint8_t* live) {
   __shared__ float2 red[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t t = blockIdx.x;
   if (blockIdx.x == 0 && threadIdx.x == 0) st.inv[0] = 1.f;
-  if (t >= T) return;
   float m = -INFINITY, s = 0.f;
   const float2* pt = part + t * npart;
-  int64_t i = WPR == 4 ? threadIdx.x : lane;
-  for (; i + 3 * 64 * WPR < npart; i += 4 * 64 * WPR) {
+  int64_t i = threadIdx.x;
+  for (; i + 3 * 256 < npart; i += 4 * 256) {
     float2 q[4];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) q[d] = pt[i + d * 64 * WPR];
+    for (int d = 0; d < 4; ++d) q[d] = pt[i + d * 256];
 #pragma unroll
     for (int d = 0; d < 4; ++d) ms_join(m, s, q[d].x, q[d].y);
   }
-  for (; i < npart; i += 64 * WPR) ms_join(m, s, pt[i].x, pt[i].y);
+  for (; i < npart; i += 256) ms_join(m, s, pt[i].x, pt[i].y);
 #pragma unroll
   for (int d = 32; d; d >>= 1) ms_join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
-  if (WPR == 4) {
-    if (lane == 0) red[wave] = make_float2(m, s);
-    __syncthreads();
-    if (wave) return;
-    for (int w = 1; w < 4; ++w) ms_join(m, s, red[w].x, red[w].y);
-  }
+  if (lane == 0) red[wave] = make_float2(m, s);
+  __syncthreads();
+  if (wave) return;
+  for (int w = 1; w < 4; ++w) ms_join(m, s, red[w].x, red[w].y);
   const float a = LN2 * (m + log2f(s));                // -inf where every token is listed
   float loss, lse, tail;                               // tail: the factor of exp(z - a)
   bool on;
@@ -1092,11 +1090,14 @@ static int64_t n_part(int64_t T, int64_t V) {
   return cdiv(V, 256) * wgm[token_tile(T)];
 }
 
-// Vocabulary of a backward piece: dz of a piece in about 128 MB (it is read
-// back by two products: within the 256 MB of the last-level cache), at
-// least 8192 tokens of the vocabulary.
+// Vocabulary of a backward piece: dz of a piece in about 256 MB, at least 8192
+// tokens of the vocabulary.  Larger pieces end fewer rounds of tiles half empty and
+// add to dh's sums less often: gradients of 2047 x 50272 x 4096 in 2230, 2015
+// and 2010 us with pieces of 128, 256 and 512 MB, of 4094 x 50272 x 768 in 1050, 980 and
+// 930, of 4094 x 128256 x 4096 in 9850, 9750 and 9630.  256 MB is taken, for the
+// memory it leaves; that the last-level cache holds a piece does not show.
 static int64_t piece_of(int64_t T, int64_t V) {
-  int64_t p = ((int64_t)64 << 20) / T / 256 * 256;
+  int64_t p = ((int64_t)128 << 20) / T / 256 * 256;
   if (p < 8192) p = 8192;
   const int64_t all = cdiv(V, 256) * 256;
   return p < all ? p : all;
@@ -1207,13 +1208,8 @@ static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int6
   CRBQ_LAUNCH_CHECK();
   float* rows = reduction ? w.rows : loss;
   uint8_t* live = reduction ? w.live : nullptr;
-  // 4 wavefronts a row up to 4 rows a CU
-  if (T <= 1024)
-    k_head_join<XENT, 4><<<(unsigned)T, 256, 0, s>>>(w.part, n_part(T, V), T, V, ls.k, ls.labels,
-                                                     ignore, st, dz_scale<T8>(), rows, live);
-  else
-    k_head_join<XENT, 1><<<(unsigned)cdiv(T, 4), 256, 0, s>>>(
-        w.part, n_part(T, V), T, V, ls.k, ls.labels, ignore, st, dz_scale<T8>(), rows, live);
+  k_head_join<XENT><<<(unsigned)T, 256, 0, s>>>(w.part, n_part(T, V), V, ls.k, ls.labels, ignore, st,
+                                                dz_scale<T8>(), rows, live);
   CRBQ_LAUNCH_CHECK();
   if (reduction) {
     k_head_reduce<<<1, 1024, 0, s>>>(w.rows, w.live, T, reduction == CRBQ_MEAN, loss, st);

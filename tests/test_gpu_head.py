@@ -216,6 +216,42 @@ def test_distill(T, V, C, k, dtype):
         close(W2.grad, dW, tw, "dW")
 
 
+def test_distill_many_pieces():
+    """Lists over more than one piece of the backward pass."""
+    from crb_amd.head import linear_distill
+    T, V, C, k, dtype = 8200, 20001, 64, 12, torch.float16
+    h, W, _ = make(T, V, C, dtype, 3)
+    g = torch.Generator().manual_seed(7)
+    idx = (torch.arange(k) * (V // k) + torch.randint(0, V // k, (T, k), generator=g)).to(DEV)
+    idx = torch.where(torch.arange(T, device=DEV)[:, None] % 2 == 0, idx, idx.flip(1))
+    val = torch.randn(T, k, generator=g).to(DEV)
+    lse = torch.logsumexp(val, 1) + 0.5
+    h.requires_grad_(), W.requires_grad_()
+    loss = linear_distill(h, W, (val, idx.int(), lse), reduction="sum")
+    dh, dW = torch.autograd.grad(loss, (h, W))
+    with torch.no_grad():
+        hd, wd = h.double(), W.double()
+        z = hd @ wd.t()
+        dz0 = 4 * math.sqrt(C) * 2.0 ** -24 * float((hd.abs() @ wd.abs().t()).max())
+        big = float(z.abs().max())
+        logq = torch.log_softmax(z, 1)
+        p = (val.double() - lse.double()[:, None]).exp()
+        pt = 1 - p.sum(1)
+        lt = torch.logsumexp(logq.scatter(1, idx, -math.inf), 1)
+        want = ((p * (p.log() - logq.gather(1, idx))).sum(1) + pt * (pt.log() - lt)).sum()
+        target = (pt[:, None] * (logq - lt[:, None]).exp()).scatter(1, idx, p)
+        q = logq.exp()
+        del z, logq
+        e = U[dtype] + 2 * dz0 + 2.0 ** -20 * (1 + big)
+        # a row: z's error, and p's and 1 - sum p's (2^-22 each, times |log q|)
+        row = 2 * dz0 + 2.0 ** -20 * (2 * big + math.log(V) + 16)
+        assert abs(float(loss.double() - want)) <= T * row + 2.0 ** -18 * float(want)
+        for got, r, m in ((dh, (q - target) @ wd, (q + target) @ wd.abs()),
+                          (dW, (q - target).t() @ hd, (q + target).t() @ hd.abs())):
+            tol = e * m + U[dtype] * r.abs() + TINY[dtype]
+            assert float(((got.double() - r).abs() - tol).max()) <= 0
+
+
 def test_distill_odd_lists():
     """Empty slots, a row that lists nothing, a token listed twice, a teacher
     that gives a listed token no probability, one with all of it."""
