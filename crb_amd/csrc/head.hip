@@ -25,13 +25,31 @@
 // (fp32) and the listed tokens' own z; a second kernel joins the tiles.
 // Backward: per piece of the vocabulary, the product again with an epilogue
 // that writes the piece's dz (16 bits, the operand of the two products that
-// follow), then dh += dz W (fp32 sums) and dW = dz^T h.  dz is rounded to the inputs'
-// type as the gradients themselves are: its error (at most 2^-8 or 2^-11 of it, independent
-// from element to element) is that of the final rounding again.  Up to 64
-// tokens, where few elements of dz may make up a gradient and the products
-// wait for memory anyway, a second 16-bit part holds what the rounding left
-// (relative 2^-16).  dz is scaled by a power of two (fp16) and by the
+// follow), then dh += dz W (fp32 sums) and dW = dz^T h.  dz is
+// rounded to the inputs' type as the gradients themselves are: its error (at most 2^-8 or
+// 2^-11 of it, independent from element to element) is that of the final rounding
+// again.  Up to 64 tokens, where few elements of dz may make up a gradient and
+// the products wait for memory anyway, a second 16-bit part holds what the rounding
+// left (relative 2^-16).  dz is scaled by a power of two (fp16) and by the
 // largest row coefficient so that it stays in range.
+//
+// The logits are computed twice, 4/3 of the operations that a step on kept logits
+// has: keeping them (525 MB for 2047 x 128256 in 16 bits, 1 GB in 32) would save a product of
+// 1.5 ms there, at the price of that memory from the forward pass to the
+// backward pass and of 16-bit logits in the gradient.
+//
+// Measured (one MI355X, bf16 unless said otherwise; TF: 2 T V C / time):
+//   product, T x V x C       forward      dz           dh           dW
+//   2047 x 128256 x 4096     1545 us      1640         1590         1770
+//                            (1390 TF)    (1310)       (1350)       (1215)
+//   2047 x 50272 x 4096      752 (fp16, 128 listed; 1120 TF)
+//   2047 x 50272 x 768       159          112          90           117
+//   333 x 32007 x 1000       32           35           36           35
+//   17 x 50272 x 2048        32           (206 MB of W at 6.3 TB/s, part of it cached)
+//   1 x 128256 x 4096        167 - 300    167 - 209    188          288
+// The range of one token: W (1 GB) just read, or just pushed out of the caches by dW.
+// The products of many tokens: MFMAs busy 77, 71, 78 and 64 % of the time at
+// 1.6 to 1.85 GHz, no LDS bank conflicts in the forward product and dh.
 #include "gemm16.h"
 
 namespace crbq {
@@ -39,8 +57,6 @@ namespace crbq {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int PAD_IDX = 0x7fffffff;     // an empty slot of a row's list
-
-__device__ __forceinline__ float g_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
 template <typename T8> struct Half;
 template <> struct Half<h8_t> { typedef _Float16 t; };
@@ -189,7 +205,8 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   if (ok && lane < 16) *out = make_float2(m, sum);
 }
 
-// few tokens: one tile a workgroup, the weight's loads deep in flight
+// Few tokens (up to 64): one tile of 256 tokens of the vocabulary a workgroup, 4 stages of
+// the weight in LDS, 3 of them in flight: bound by reading W.
 template <typename T8, typename G, bool XENT>
 __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[G::LDS];
@@ -233,7 +250,9 @@ __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
   });
 }
 
-// many tokens: persistent workgroups
+// Many tokens: persistent workgroups on 256 x 256 tiles (gemm16.h).  Bound by the MFMAs at
+// the clock that their power leaves; the epilogue, 5 to 6 us of a tile's 100 at C = 4096
+// and a quarter of the time at C = 768, runs while the next tile's first loads arrive.
 template <bool XENT>
 struct FwdJob {
   static constexpr bool MASKED = false;
@@ -247,7 +266,8 @@ struct FwdJob {
     const FwdArgs p = g_args<FwdArgs>();
     return p.nm * p.nn;
   }
-  __device__ __forceinline__ static void place(const FwdArgs& p, int lin, int64_t& v0, int64_t& t0, int& tm) {
+  __device__ __forceinline__ static void place(const FwdArgs& p, int lin, int64_t& v0,
+                                               int64_t& t0, int& tm) {
     int tn;
     g_band(lin, p.nm, p.nn, tm, tn);
     v0 = (int64_t)tm * 256;
@@ -447,7 +467,7 @@ __global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ pa
 }
 
 // Sum or mean of the rows' losses, in a fixed order, and the live rows' bits,
-// by one workgroup.
+// by one workgroup: the latency of a launch and of two trips to memory, 4 to 5 us.
 __global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ rows,
                                                       const uint8_t* __restrict__ live, int64_t T,
                                                       int mean, float* loss, State st) {
@@ -484,9 +504,11 @@ __global__ __launch_bounds__(1024) void k_head_reduce(const float* __restrict__ 
 
 // The teacher's list of each row: tokens ascending, probabilities, the
 // bits of the forward product (the row's words are cleared first).  One
-// wavefront a row.  Tokens outside
-// [0, V) are empty slots; of one listed twice the list holds one entry with
-// the sum of its probabilities.
+// wavefront a row.  Tokens outside [0, V) are empty slots; of one listed twice
+// the list holds one entry with the sum of its probabilities.  Repeats and ranks by
+// comparing all pairs, 4 a read of LDS: k^2 / 256 reads a lane, no more than the clearing of
+// the words takes: 2047 rows of 128 (50272 tokens) in 36 us, 250 of 20 in 7,
+// 17 of 64 in 11 (the latency of its dependent steps).
 constexpr int LIST_MAX = 256;
 template <typename TV>
 __global__ __launch_bounds__(64) void k_list(const TV* __restrict__ val, int64_t ldv,
@@ -650,9 +672,9 @@ struct Factor {
   __device__ float get() const { return f0[0] * f1[0] * mul; }
 };
 
-// dz of a piece of the vocabulary: dz[t][v - vbeg] = rowb exp(z - a), zeros
-// in the columns past the vocabulary (and where rowb is 0, whatever z is).  A
-// label's own dz is -rowb (cross entropy); the listed tokens' of a
+// dz of a piece of the vocabulary, the forward's product with another epilogue:
+// dz[t][v - vbeg] = rowb exp(z - a), zeros in the columns past the vocabulary (and
+// where rowb is 0, whatever z is).  A label's own dz is -rowb (cross entropy); the listed tokens' of a
 // distillation follow (k_dz_listed).
 struct DzArgs {
   const uint16_t *h, *W;
@@ -668,8 +690,8 @@ struct DzArgs {
 
 // A piece's dz in memory: blocks of 64 columns, each dz_rows(T) rows of 128
 // bytes, so that a unit of either product that reads it is 8 KB in one
-// piece (row by row, dW's loads went 64 KB from row to row: 0.53 of the time
-// with busy MFMAs against 0.72 of dh's).  The columns of whole tiles are
+// piece (row by row, dW's loads went 64 KB from row to row: MFMAs busy 53 % of the
+// time instead of 64).  The columns of whole tiles are
 // written, zeros behind nv; the rows behind T are not, and dh's tiles, which
 // read them, do not keep what comes of them.  Up to 64 tokens, rows 64 on hold the
 // second parts.
@@ -763,7 +785,8 @@ struct DzJob {
     const DzArgs p = g_args<DzArgs>();
     return p.nm * p.nn;
   }
-  __device__ __forceinline__ static void place(const DzArgs& p, int lin, int64_t& v0, int64_t& t0) {
+  __device__ __forceinline__ static void place(const DzArgs& p, int lin, int64_t& v0,
+                                               int64_t& t0) {
     int tm, tn;
     g_band(lin, p.nm, p.nn, tm, tn);
     v0 = (int64_t)tm * 256;
@@ -837,7 +860,8 @@ __global__ __launch_bounds__(G_THREADS) void k_head_dz_p(const DzArgs) {
   g_run<T8, G_KC, G_KC>(smem, DzJob<T8>());
 }
 
-// the listed tokens' dz within [vbeg, vbeg + nv) (distillation)
+// The listed tokens' dz within [vbeg, vbeg + nv) (distillation), a thread each: 5 to 7 us,
+// in place of a search for listed tokens in the epilogue of the product.
 template <typename T8>
 __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
                                                    const float* __restrict__ ratio, int64_t vbeg,
@@ -856,7 +880,8 @@ __global__ __launch_bounds__(256) void k_dz_listed(State st, int64_t T, int k,
 }
 
 // dh partial sums (fp32): P[split][t][c] (+)= sum of dz[t][v] W[v][c] over the
-// split's v (span of them, a multiple of 64)
+// split's v (span of them, a multiple of 64).  No atomics: a split's sums are its own,
+// and the pieces of the vocabulary follow each other, so the result is the same each time.
 struct DhArgs {
   const uint16_t *W, *dz;
   int64_t ldw, zstep, T, nv, C, span;
@@ -913,7 +938,8 @@ struct DhJob {
     const DhArgs p = g_args<DhArgs>();
     return p.nm * p.nn * p.ns;
   }
-  __device__ __forceinline__ static void place(const DhArgs& p, int lin, int64_t& c0, int64_t& t0, int& split) {
+  __device__ __forceinline__ static void place(const DhArgs& p, int lin, int64_t& c0,
+                                               int64_t& t0, int& split) {
     int tm, tn;
     split = lin / (p.nm * p.nn);
     g_band(lin - split * p.nm * p.nn, p.nm, p.nn, tm, tn);
@@ -958,7 +984,8 @@ __global__ __launch_bounds__(G_THREADS) void k_head_dh_p(const DhArgs) {
   g_run<T8, G_KS, G_KC_BLOCKED>(smem, DhJob());
 }
 
-// dh = factor * (P[0] + P[1] + ...), rounded once; 4 channels a thread
+// dh = factor * (P[0] + P[1] + ...), rounded once; 4 channels a thread.  Bound by reading
+// P: 2047 x 4096 in 22 us with 2 splits, 333 x 1000 in 8.
 template <typename T8>
 __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int ns, int64_t T,
                                                 int64_t C, Factor fac, uint16_t* dh,
@@ -988,7 +1015,9 @@ __global__ __launch_bounds__(256) void k_dh_out(const float* __restrict__ P, int
   }
 }
 
-// dW[v][c] = factor * sum_t dz[t][v] h[t][c] of a piece's rows v
+// dW[v][c] = factor * sum_t dz[t][v] h[t][c] of a piece's rows v.  From about 500 tokens on
+// bound by the MFMAs, fed by transpose reads of both operands; with few tokens by
+// writing dW: one token, 1 GB in 288 us (3.65 TB/s; a workgroup a CU waits for its own stores).
 struct DwArgs {
   const uint16_t *h, *dz;
   int64_t ldh, zstep, T, nv, C;
@@ -1083,7 +1112,10 @@ struct Big {               // the persistent 256 x 256 tiles
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// tokens per tile: 0 = 16, 1 = 64, 2 = 256
+// Tokens per tile: 0 = 16, 1 = 64, 2 = 256.  Forward over V = 128256, C = 4096: 16 tokens in
+// 189 us with tiles of 16 and of 64, 17 in 211 and 188; 64 in 192 us with tiles of
+// 64, 240 with 256; 65 in 225 and 238, 160 in 317 and 247.  The gradients of 16 tokens (50272
+// x 768, 32007 x 1000) take 76 and 66 us with tiles of 16, 81 and 70 with 64.
 static int token_tile(int64_t T) { return T <= 16 ? 0 : T <= 64 ? 1 : 2; }
 static int64_t n_part(int64_t T, int64_t V) {
   static const int wgm[3] = {ZS::WGM, ZM::WGM, Big::WGM};
@@ -1208,8 +1240,8 @@ static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int6
   CRBQ_LAUNCH_CHECK();
   float* rows = reduction ? w.rows : loss;
   uint8_t* live = reduction ? w.live : nullptr;
-  k_head_join<XENT><<<(unsigned)T, 256, 0, s>>>(w.part, n_part(T, V), V, ls.k, ls.labels, ignore, st,
-                                                dz_scale<T8>(), rows, live);
+  k_head_join<XENT><<<(unsigned)T, 256, 0, s>>>(w.part, n_part(T, V), V, ls.k, ls.labels, ignore,
+                                                st, dz_scale<T8>(), rows, live);
   CRBQ_LAUNCH_CHECK();
   if (reduction) {
     k_head_reduce<<<1, 1024, 0, s>>>(w.rows, w.live, T, reduction == CRBQ_MEAN, loss, st);
@@ -1349,8 +1381,8 @@ extern "C" int crbq_head_xent_grad(const void* h, int64_t ldh, const void* W, in
                                    void* dW, int64_t ldo, void* ws, size_t ws_bytes,
                                    void* stream) {
   if (int e = check_head(h, ldh, W, ldw, dtype, T, V, C)) return e;
-  if (!labels || bad_state(state) || !g || (!dh && !dW) || bad_reduction(reduction) || bad_scale(scale) ||
-      bad_ws(ws))
+  if (!labels || bad_state(state) || !g || (!dh && !dW) || bad_reduction(reduction) ||
+      bad_scale(scale) || bad_ws(ws))
     return CRBQ_ERR_ARG;
   if ((dh && bad_matrix(dh, ldd, C)) || (dW && bad_matrix(dW, ldo, C))) return CRBQ_ERR_ARG;
   bool ok;

@@ -2,19 +2,20 @@
 // index) and the row's log-sum-exp: what a teacher leaves behind for
 // distillation instead of its logits.
 //
-// One workgroup a row (1024 threads, or fewer).  One pass over the row takes each
-// thread's largest logit and its sum of exponentials against that (rescaled
-// the few times the largest one rises): 8.5 vector instructions' time an
-// element, below the time its bytes take.  The k-th largest of
-// the threads' maxima is a lower bound of the row's k-th largest logit that only about
-// k elements reach (with k of 1024 threads hit, -1024 log(1 - k / 1024)
-// elements: 137 for k = 128).  Each thread keeps the largest logit of each of
-// its 16-byte groups (every 16th of them where it has more than 16) and reads
-// those groups again that reach the bound: about k of them, where all groups of all threads
-// whose maximum reaches it cost as much as the row over again (2047 rows of 128256: 85
-// us of 200).  What they hold above the bound is ranked by counting.  Rows whose ties leave more candidates than the list holds (a
-// constant row, a row masked to one value) and rows with a NaN are selected
-// exactly, by digits of the key.
+// One workgroup a row.  One pass over the row takes each thread's largest logit
+// and its sum of exponentials against that (rescaled the few times the largest
+// one rises): 8.5 vector instructions' time an element, below the time its bytes
+// take.  The k-th largest of the threads' maxima is a lower bound of the row's k-th
+// largest logit that only about k elements reach (with k of 1024 threads hit, -1024
+// log(1 - k / 1024) elements: 137 for k = 128).  Each thread keeps the largest logit of
+// each of its 16-byte groups (every 16th of them where it has more than 16) and
+// reads those groups again that reach the bound: about k of them, where all groups of
+// all threads whose maximum reaches it cost as much as the row over again (2047 rows of
+// 128256: 85 us of 200).  What they hold above the bound is ranked by counting.  Rows whose
+// ties leave more candidates than the list holds (a constant row, a row masked to one
+// value) and rows with a NaN are selected exactly, by digits of the key.
+// Measured, 16 bits: 2047 x 128256, k = 128, in 123 us (4.3 TB/s), 2047 x 50272 in 66;
+// 301 x 32007 in fp32, 22; one row of 50272, 12 us: the latency of its steps.
 // Logits are compared as whole numbers in the order of the values (-0 as
 // +0, NaN above everything); the values written are the logits themselves.
 #include "common.h"
@@ -269,7 +270,8 @@ __global__ __launch_bounds__(NT) void k_top_logits(const void* logits, int64_t V
         const int first = __shfl(dig, __ffsll((unsigned long long)act) - 1);
         const uint64_t same = __ballot(dig == first);
         if (dig != first) atomicAdd(&hist[dig], 1);
-        else if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(&hist[dig], __popcll(same));
+        else if (lane == __ffsll((unsigned long long)same) - 1)
+          atomicAdd(&hist[dig], __popcll(same));
       });
       __syncthreads();
       if (tid == 0) {
