@@ -14,8 +14,8 @@
 // 128256: 85 us of 200).  What they hold above the bound is ranked by counting.  Rows whose
 // ties leave more candidates than the list holds (a constant row, a row masked to one
 // value) and rows with a NaN are selected exactly, by digits of the key.
-// Measured, 16 bits: 2047 x 128256, k = 128, in 123 us (4.3 TB/s), 2047 x 50272 in 66;
-// 301 x 32007 in fp32, 22; one row of 50272, 12 us: the latency of its steps.
+// Measured, 16 bits: 2047 x 128256, k = 128, in 123 us (4.3 TB/s), 2047 x 50272 in 63;
+// 301 x 32007 in fp32, 19; one row of 50272, 12 us: the latency of its steps.
 // Logits are compared as whole numbers in the order of the values (-0 as
 // +0, NaN above everything); the values written are the logits themselves.
 #include "common.h"
@@ -325,19 +325,19 @@ __global__ __launch_bounds__(NT) void k_top_logits(const void* logits, int64_t V
   }
 }
 
-// Up to a row a CU: workgroups of 1024, for the row's latency.  More rows:
-// small workgroups, since after its pass over the row a workgroup mostly
-// waits, so that what counts is the rows at work on a CU (2, 4 or 8): 4096 rows of
-// 8000, 256 threads 33 us, 512 70, 1024 120.  256 maxima bound the k-th logit well
-// for k up to 128 (177 candidates), and a thread's groups are read again one
-// by one while it has few: 2047 rows of 128256, 256 threads 152 us, 512 123; of
-// 50272, 66 and 73.
+// Threads a row.  After its pass over the row a workgroup mostly waits, so that with many
+// rows what counts is the rows at work on a CU (2, 4 or 8), with few the row's own
+// latency, and for k above 128 a bound from 256 maxima is loose.  Measured with k = 100, us
+// with 256, 512 and 1024 threads: 256 rows of 32007 in 16 bits 16.9, 13.9, 14.2; of
+// 128256 40.8, 26.5, 22.6; 301 rows of 32007 in 32 bits 23.5, 19.3, 27.2; 2047 rows of 8000
+// 28.6, 36.5, 67; of 32007 45, 50, 84; of 50272 61, 58, 96; of 128256 133, 118, 151.
 template <typename E>
 static void top_logits(const void* logits, int64_t T, int64_t V, int64_t ld, int k, float it,
                        void* val, int32_t* idx, float* lse, hipStream_t s) {
-  if (T <= 256)
+  const int64_t bytes = V * (int64_t)sizeof(E);
+  if (T <= 256 && bytes > 160 * 1024)
     k_top_logits<E, 1024><<<(unsigned)T, 1024, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
-  else if (k > 128 || V > 65536)
+  else if (T <= 512 || k > 128 || bytes > 96 * 1024)
     k_top_logits<E, 512><<<(unsigned)T, 512, 0, s>>>(logits, V, ld, k, it, val, idx, lse);
   else
     k_top_logits<E, 256><<<(unsigned)T, 256, 0, s>>>(logits, V, ld, k, it, val, idx, lse);

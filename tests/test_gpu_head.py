@@ -588,6 +588,18 @@ def test_top_logits_ties_and_specials(dtype):
         check_top(x.to(DEV), k)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T,V,k", [(3, 90001, 200), (520, 1500, 128), (515, 50273, 20)])
+def test_top_logits_rows_and_lengths(T, V, k, dtype):
+    """Few long rows, many short and many long ones; ties, masked rows and NaN among them."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(T, V, generator=g).to(dtype)
+    x[0] = 1.0
+    x[1, : V - 3] = -math.inf
+    x[2, V // 2] = math.nan
+    check_top(x.to(DEV), k)
+
+
 def test_top_logits_rows_of_any_stride():
     base = torch.randn(6, 30001, generator=torch.Generator().manual_seed(2)).half().to(DEV)
     for a in range(1, 9):
