@@ -205,7 +205,7 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   if (ok && lane < 16) *out = make_float2(m, sum);
 }
 
-// Few tokens (up to 64): one tile of 256 tokens of the vocabulary a workgroup, 4 stages of
+// Few tokens or few tiles: one tile of 256 tokens of the vocabulary a workgroup, 4 stages of
 // the weight in LDS, 3 of them in flight: bound by reading W.
 template <typename T8, typename G, bool XENT>
 __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
@@ -770,7 +770,7 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
       uint2 rest;
       *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8, true>(
           acc[i][j], scale2, a2, b, p.nv - v, o >= 0 && o < 4 ? (int)o : -1, &rest);
-      *(uint2*)dz_at(p.dz, p.zstep, 64 + t, v) = rest;
+      if (p.T <= 64) *(uint2*)dz_at(p.dz, p.zstep, 64 + t, v) = rest;
     }
   }
 }
@@ -1047,7 +1047,8 @@ struct DwJob {
     const DwArgs p = g_args<DwArgs>();
     return p.nm * p.nn;
   }
-  __device__ __forceinline__ static void place(const DwArgs& p, int lin, int64_t& c0, int64_t& v0) {
+  __device__ __forceinline__ static void place(const DwArgs& p, int lin, int64_t& c0,
+                                               int64_t& v0) {
     int tm, tn;
     g_band(lin, p.nm, p.nn, tm, tn);
     c0 = (int64_t)tm * 256;
@@ -1115,14 +1116,19 @@ struct Big {               // the persistent 256 x 256 tiles
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tokens per tile: 0 = 16, 1 = 64, 2 = 256.  Forward over V = 128256, C = 4096: 16 tokens in
-// 189 us with tiles of 16 and of 64, 17 in 211 and 188; 64 in 192 us with tiles of
-// 64, 240 with 256; 65 in 225 and 238, 160 in 317 and 247.  The gradients of 16 tokens (50272
-// x 768, 32007 x 1000) take 76 and 66 us with tiles of 16, 81 and 70 with 64.
-static int token_tile(int64_t T) { return T <= 16 ? 0 : T <= 64 ? 1 : 2; }
+// Tokens per tile of the logits: 0 = 16, 1 = 64, 2 = 256.  Forward over V = 128256, C =
+// 4096: 16 tokens in 189 us with tiles of 16 and of 64, 17 in 211 and 188; 64 in 192 us
+// with tiles of 64, 240 with 256; 65 in 225 and 238, 160 in 317 and 247.  The gradients
+// of 16 tokens (50272 x 768, 32007 x 1000) take 76 and 66 us with tiles of 16, 81 and 70
+// with 64.  Tiles of 64 also while there is at most one of them a CU: forward of 2047 x 2000 x
+// 4096 in 56 us instead of 91, gradients 154 instead of 189; 250 x 16000 x 768, 25 and
+// 30, 63 and 74 (a CU that has one tile takes 0.6 of the time of one of 256).
+static int token_tile(int64_t T, int64_t V) {
+  return T <= 16 ? 0 : T <= 64 || cdiv(T, 64) * cdiv(V, 256) <= 256 ? 1 : 2;
+}
 static int64_t n_part(int64_t T, int64_t V) {
   static const int wgm[3] = {ZS::WGM, ZM::WGM, Big::WGM};
-  return cdiv(V, 256) * wgm[token_tile(T)];
+  return cdiv(V, 256) * wgm[token_tile(T, V)];
 }
 
 // Vocabulary of a backward piece: dz of a piece in about 256 MB, at least 8192
@@ -1141,8 +1147,7 @@ static int64_t piece_of(int64_t T, int64_t V) {
 // workgroups times the 64-k stages of a part (1.2 us each, 6 more a tile), and
 // the fp32 partial sums, written and read back at about 4 TB/s.
 static int dh_splits(int64_t T, int64_t C, int64_t piece) {
-  static const int bn[3] = {16, 64, 256};
-  const int64_t tiles = cdiv(C, 256) * cdiv(T, bn[token_tile(T)]), stages = cdiv(piece, G_K);
+  const int64_t tiles = cdiv(C, 256) * cdiv(T, T <= 16 ? 16 : T <= 64 ? 64 : 256), stages = cdiv(piece, G_K);
   int64_t best = 1;
   double least = 0.;
   for (int64_t s = 1; s <= 256 && s * 4 <= stages; ++s) {
@@ -1235,7 +1240,7 @@ static int head_fwd(const void* h, int64_t ldh, const void* W, int64_t ldw, int6
                     float* loss, const State& st, const FwdWs& w, hipStream_t s) {
   const FwdArgs p{(const uint16_t*)h, (const uint16_t*)W, ldh, ldw, T, V, C, scale, ls, 0, 0,
                   w.part, n_part(T, V), st.zt};
-  switch (token_tile(T)) {
+  switch (token_tile(T, V)) {
     case 0: launch_fwd<T8, ZS, XENT>(p, s); break;
     case 1: launch_fwd<T8, ZM, XENT>(p, s); break;
     default: launch_fwd<T8, Big, XENT>(p, s);
@@ -1300,7 +1305,7 @@ static int head_grad(const GradCall& c, const State& st, const GradWs& w, hipStr
     }
     if (c.dh) {
       const int mh = (int)cdiv(C, GH::BM);
-      const int nn = T <= 64 ? 2 : nt;
+      const int nn = T <= 64 ? 2 : (int)cdiv(T, 256);
       const DhArgs q{Wv, w.dz, c.ldw, zstep, T, nv, C, w.span, mh, nn, (int)cdiv(nv, w.span), w.P,
                      v > 0};
       const int64_t tiles = (int64_t)mh * nn * q.ns;
@@ -1328,9 +1333,10 @@ static int head_grad(const GradCall& c, const State& st, const GradWs& w, hipStr
 
 template <typename T8>
 static int head_grad_t(const GradCall& c, const State& st, const GradWs& w, hipStream_t s) {
-  switch (token_tile(c.T)) {
+  switch (token_tile(c.T, w.piece)) {
     case 0: return head_grad<T8, ZS, HS>(c, st, w, s);
-    case 1: return head_grad<T8, ZM, HM>(c, st, w, s);
+    case 1: return c.T <= 64 ? head_grad<T8, ZM, HM>(c, st, w, s)
+                             : head_grad<T8, ZM, Big>(c, st, w, s);
     default: return head_grad<T8, Big, Big>(c, st, w, s);
   }
 }

@@ -252,6 +252,46 @@ def test_distill_many_pieces():
             assert float(((got.double() - r).abs() - tol).max()) <= 0
 
 
+# more tiles of 64 tokens than CUs
+MANY = [(300, 14001, 72), (65, 35001, 200), (513, 8001, 136), (1030, 4099, 328)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("T,V,C", MANY)
+def test_xent_many_tiles(T, V, C, dtype):
+    test_xent(T, V, C, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("T,V,C", MANY)
+def test_distill_many_tiles(T, V, C, dtype):
+    test_distill(T, V, C, T % 64 + 1, dtype)
+
+
+def test_many_tiles_rows():
+    """Gradients of their own for many rows, some of them 0, NaN hidden states where
+    nothing is learned, a strided weight."""
+    from crb_amd.head import linear_cross_entropy
+    T, V, C, dtype = 300, 14001, 72, torch.bfloat16
+    h, W, y = make(T, V, C, dtype, 23)
+    y[7::9] = -100
+    g = torch.randn(T, generator=torch.Generator().manual_seed(2))
+    g[:128:2] = 0.0
+    z, dz0, loss, dz, both = ref_xent(h, W, y, 1.0, -100, g.double())
+    wide = torch.full((V, C + 16), math.nan, device=DEV, dtype=dtype)
+    wide[:, 8:8 + C] = W
+    dead = h.clone()
+    dead[7::9] = math.nan
+    dead.requires_grad_(), wide.requires_grad_()
+    rows = linear_cross_entropy(dead, wide[:, 8:8 + C], y, reduction="none")
+    close(rows.detach(), loss, loss_tol(z, dz0, loss), "rows")
+    got = torch.autograd.grad(rows, (dead, wide), g.to(DEV))
+    dh, th, dW, tw = grad_refs(h, W, dz, both, dz0, z, 1.0, dtype)
+    close(got[0], dh, th, "dh")
+    close(got[1][:, 8:8 + C], dW, tw, "dW")
+    assert not got[0][7::9].any() and not got[0][:128:2].any()
+
+
 def test_distill_odd_lists():
     """Empty slots, a row that lists nothing, a token listed twice, a teacher
     that gives a listed token no probability, one with all of it."""
