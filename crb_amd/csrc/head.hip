@@ -38,15 +38,15 @@
 // 1.5 ms there, at the price of that memory from the forward pass to the
 // backward pass and of 16-bit logits in the gradient.
 //
-// Measured (one MI355X, bf16 unless said otherwise; TF: 2 T V C / time):
-//   product, T x V x C       forward      dz           dh           dW
-//   2047 x 128256 x 4096     1545 us      1640         1590         1770
-//                            (1390 TF)    (1310)       (1350)       (1215)
-//   2047 x 50272 x 4096      752 (fp16, 128 listed; 1120 TF)
-//   2047 x 50272 x 768       159          112          90           117
-//   333 x 32007 x 1000       32           35           36           35
-//   17 x 50272 x 2048        32           (206 MB of W at 6.3 TB/s, part of it cached)
-//   1 x 128256 x 4096        167 - 300    167 - 209    188          288
+// Measured (one MI355X, bf16 unless said otherwise; us, in brackets the TF of 2 T V C):
+//   product, T x V x C                 forward       dz            dh            dW
+//   2047 x 128256 x 4096               1550 (1390)   1670 (1290)   1530 (1400)   1815 (1185)
+//   2047 x 50272 x 4096 fp16, 128 listed  760 (1110)   738 (1140)    645 (1310)    766 (1100)
+//   2047 x 50272 x 768                 160           194           132           177
+//   333 x 32007 x 1000                 32            36            37            36
+//   250 x 50272 x 768, 20 listed       30            30            34            39
+//   17 x 50272 x 2048 fp16, 64 listed  32            (206 MB of W at 6.3 TB/s, part of it cached)
+//   1 x 128256 x 4096                  167 - 300     167 - 209     188           288
 // The range of one token: W (1 GB) just read, or just pushed out of the caches by dW.
 // The products of many tokens: MFMAs busy 77, 71, 78 and 64 % of the time at
 // 1.6 to 1.85 GHz, no LDS bank conflicts in the forward product and dh.
@@ -128,15 +128,15 @@ struct FwdArgs {
 // from v0 + off(i) on: listed tokens and what lies behind the vocabulary
 // become -inf (the listed ones' z is written), then the maximum and the sum
 // of exponentials.  lab: the label's place behind v0; words: each i's 16 mask
-// bits; before(q): the slot of the first token of words[q].
+// bits; slots(s): s[q] = the slot of the first token of words[q].
 // In units of log 2: exp z = 2^(acc * scale2), so an exponential is one
 // multiply-add and one v_exp; the listed tokens and the end are looked for
 // only where a wavefront has any.  Bound by the v_exp (16 cycles a wavefront)
 // and the 2 to 3 vector operations beside each.
-template <int MI, int NJ, bool XENT, int j, typename Off, typename Before>
+template <int MI, int NJ, bool XENT, int j, typename Off, typename Slots>
 __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t v0, Off off,
                                            int lab, const uint32_t (&words)[(MI + 1) / 2],
-                                           Before before, f4_t (&acc)[MI][NJ], float2* out) {
+                                           const Slots& slots, f4_t (&acc)[MI][NJ], float2* out) {
   const int lane = g_lane(), g4 = (lane >> 4) * 4;
   const bool ok = t < p.T;
   bool any;
@@ -151,10 +151,7 @@ __device__ __forceinline__ void fwd_column(const FwdArgs& p, int64_t t, int64_t 
   const float fin = p.scale < 0.f ? INFINITY : -INFINITY;        // scale * fin = -inf
   if (__any(any)) {
     int slot[(MI + 1) / 2] = {};
-    if (!XENT) {
-#pragma unroll
-      for (int q = 0; q < (MI + 1) / 2; ++q) slot[q] = before(q);
-    }
+    if (!XENT) slots(slot);
     g_each<MI>([&](auto ii) __attribute__((always_inline)) {
       constexpr int i = decltype(ii)::value;
       const int o = off(i) + g4;
@@ -241,11 +238,13 @@ __global__ __launch_bounds__(G::THREADS) void k_head_fwd(const FwdArgs p) {
         for (int e = 0; e < G::WM / 32; ++e)
           if (q == wr * (G::WM / 32) + e) words[e] = all[q];
     }
-    auto before = [&](int q) __attribute__((always_inline)) {
-      return ok ? p.ls.base[t * p.ls.ntile + tm] + bits_before(all, wr * (G::WM / 32) + q) : 0;
+    auto slots = [&](int (&slot)[G::WM / 32]) __attribute__((always_inline)) {
+      const int base = ok ? p.ls.base[t * p.ls.ntile + tm] : 0;
+#pragma unroll
+      for (int q = 0; q < G::WM / 32; ++q) slot[q] = base + bits_before(all, wr * (G::WM / 32) + q);
     };
     fwd_column<G::MI, G::NJ, XENT, j>(
-        p, t, vw, [](int i) { return 16 * i; }, lab, words, before, acc,
+        p, t, vw, [](int i) { return 16 * i; }, lab, words, slots, acc,
         p.part + t * p.npart + (int64_t)tm * G::WGM + wr);
   });
 }
@@ -333,15 +332,23 @@ struct FwdJob {
 #pragma unroll
         for (int q = 0; q < 4; ++q) words[q] = w[2 * q];
       }
-      auto before = [&](int q) __attribute__((always_inline)) {
-        const uint32_t* w = (const uint32_t*)(priv + 1024 * (j >> 1)) + row * 8;
+      // (the words between are the other wavefront's: all four read at once)
+      auto slots = [&](int (&slot)[4]) __attribute__((always_inline)) {
+        const uint32_t* w = (const uint32_t*)(priv + 1024 * (j >> 1)) + row * 8 + (wr ^ 1);
         int c = ((const int*)(priv + 2048 + 256 * (j >> 1)))[row];
-        for (int e = 0; e < 2 * q + wr; ++e) c += __popc(w[e]);
-        return c;
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = w[2 * q];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int between = __popc(o[q]);
+          slot[q] = c + (wr ? between : 0);
+          c += between + __popc(words[q]);
+        }
       };
       fwd_column<8, 4, XENT, j>(
           p, t, v0, [&](int i) { return 64 * (i >> 1) + 32 * wr + 16 * (i & 1); }, lab, words,
-          before, acc.v, p.part + t * p.npart + (int64_t)tm * 2 + wr);
+          slots, acc.v, p.part + t * p.npart + (int64_t)tm * 2 + wr);
     });
   }
 };
