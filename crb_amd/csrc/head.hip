@@ -48,8 +48,8 @@
 //   17 x 50272 x 2048 fp16, 64 listed  32            (206 MB of W at 6.3 TB/s, part of it cached)
 //   1 x 128256 x 4096                  167 - 300     167 - 209     188           288
 // The range of one token: W (1 GB) just read, or just pushed out of the caches by dW.
-// The products of many tokens: MFMAs busy 77, 71, 78 and 64 % of the time at
-// 1.6 to 1.85 GHz, no LDS bank conflicts in the forward product and dh.
+// The products of many tokens at 4096 channels: MFMAs busy 76, 72, 80 and 64 % of the
+// time at 1.6 to 1.85 GHz; at 768, 55, 45, 71 and 61 %.
 #include "gemm16.h"
 
 namespace crbq {
