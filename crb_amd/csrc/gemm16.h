@@ -325,7 +325,7 @@ __device__ __forceinline__ void g_tile(char* smem, const GOperand& A, const GOpe
 // 1, units 2 and 3 in quarter 3).  After each half stage, a barrier: the units
 // read in it are free, and the loads of the half before the last have
 // arrived.  So every half issues 4 loads of each wavefront, evenly spaced, and
-// each has between 2 and 3 halves (2048 to 3072 cycles of MFMAs) to arrive:
+// each has between 2 and 3 halves (of 1024 cycles of MFMAs) to arrive:
 //   first half of stage c:   A(c + 2) unit 0, A(c + 1) unit 3, B(c + 2) units 2, 3
 //   second half:             A(c + 2) units 1, 2,              B(c + 3) units 0, 1
 // With one barrier a stage and each stage loaded as a whole in the half

@@ -650,6 +650,61 @@ def test_top_logits_rows_of_any_stride():
 
 
 # ---------------------------------------------------------------------------
+# more than 2^31 elements
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [5, 70])
+def test_weight_beyond_32_bits(T):
+    from crb_amd.head import linear_cross_entropy
+    V, C, dtype = 140001, 16384, torch.bfloat16
+    g = torch.Generator(device=DEV).manual_seed(T)
+    W = torch.empty(V, C, device=DEV, dtype=dtype).normal_(0.0, 1.5 / math.sqrt(C), generator=g)
+    h = torch.randn(T, C, device=DEV, generator=g).to(dtype)
+    y = torch.randint(0, V, (T,), device=DEV, generator=g)
+    y[0], y[1], y[2] = V - 1, V - 2, 0
+    W[V - 1] = (0.05 * h[0].float()).to(dtype)                     # rows that are learned or wrong
+    W[V - 3] = (0.06 * h[1].float()).to(dtype)
+    h.requires_grad_(), W.requires_grad_()
+    loss = linear_cross_entropy(h, W, y, reduction="sum")
+    dh, dW = torch.autograd.grad(loss, (h, W))
+    with torch.no_grad():
+        hd, step = h.double(), 20000
+        parts = range(0, V, step)
+        z = torch.cat([hd @ W[v:v + step].double().t() for v in parts], 1)
+        mag = max(float((hd.abs() @ W[v:v + step].double().abs().t()).max()) for v in parts)
+        dz0 = 4 * math.sqrt(C) * 2.0 ** -24 * mag
+        logq = torch.log_softmax(z, 1)
+        rows = -logq.gather(1, y[:, None])[:, 0]
+        assert abs(float(loss.double() - rows.sum())) <= float(loss_tol(z, dz0, rows).sum())
+        q, one = logq.exp(), torch.zeros_like(logq).scatter_(1, y[:, None], 1.0)
+        u = U[dtype]
+        e = (u * u if T <= 64 else u) + 2 * dz0 + 2.0 ** -20 * (1 + float(z.abs().max()))
+        want, size = torch.zeros_like(hd), torch.zeros_like(hd)
+        for v in parts:
+            w, d, m = W[v:v + step].double(), (q - one)[:, v:v + step], (q + one)[:, v:v + step]
+            want += d @ w
+            size += m @ w.abs()
+            r = d.t() @ hd
+            tol = e * (m.t() @ hd.abs()) + u * r.abs()
+            assert float(((dW[v:v + step].double() - r).abs() - tol).max()) <= 0, v
+        assert float(((dh.double() - want).abs() - e * size - u * want.abs()).max()) <= 0
+
+
+def test_top_logits_beyond_32_bits():
+    T, V, k = 20000, 120001, 40
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.empty(T, V, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    from crb_amd.head import TopLogits, top_logits
+    top = top_logits(x, k)
+    for t in (0, 17000, 17897, T - 1):                             # 2^31 lies in row 17895
+        val, idx = torch.sort(x[t].double(), descending=True, stable=True)
+        lse = float(torch.logsumexp(x[t].double(), 0))
+        assert torch.equal(top.idx[t].long(), idx[:k]), t
+        assert torch.equal(top.val[t].double(), val[:k]), t
+        assert abs(float(top.lse[t]) - lse) <= 2.0 ** -21 + 4 * math.sqrt(V) * 2.0 ** -24 + 2.0 ** -23 * lse
+    assert isinstance(top, TopLogits)
+
+
+# ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
 def test_refusals():
