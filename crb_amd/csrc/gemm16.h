@@ -654,14 +654,21 @@ __device__ __forceinline__ void g_load_lds_words(const void* dst, const void* p,
 // 16 rows (n) of a wavefront's 16-bit output of a 256 x 256 tile (128 elements each, m
 // as above) through its own LDS: in as each lane's 4 consecutive
 // elements of one row, out as 16-byte stores, 64 bytes of a row side by
-// side.  put(row, m, 8 elements) stores.
-template <typename F>
-__device__ __forceinline__ void g_rows_out(char* priv, const uint2 (&v)[8], F&& put) {
+// side.  put(row, m, 8 elements) stores.  g_rows_at(priv, n, m) is where element
+// m of row n lies meanwhile: patch() may change some there.
+__device__ __forceinline__ uint16_t* g_rows_at(char* priv, int n, int m) {
+  const int i = 2 * (m >> 6) + ((m >> 4) & 1), g = (m >> 2) & 3;
+  return (uint16_t*)(priv + n * 256 + (((2 * i + (g >> 1)) ^ n) << 4) + (g & 1) * 8) + (m & 3);
+}
+template <typename P, typename F>
+__device__ __forceinline__ void g_rows_out(char* priv, const uint2 (&v)[8], P&& patch, F&& put) {
   const int lane = g_lane(), n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     *(uint2*)(priv + n * 256 + (((2 * i + (g >> 1)) ^ n) << 4) + (g & 1) * 8) = v[i];
+  asm volatile("" ::: "memory");                      // (other types at the same place)
+  patch();
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
   for (int q = 0; q < 4; ++q) {

@@ -41,8 +41,8 @@
 // Measured (one MI355X, bf16 unless said otherwise; us, in brackets the TF of 2 T V C):
 //   product, T x V x C                 forward       dz            dh            dW
 //   2047 x 128256 x 4096               1550 (1390)   1670 (1290)   1530 (1400)   1815 (1185)
-//   2047 x 50272 x 4096 fp16, 128 listed  760 (1110)   738 (1140)    645 (1310)    766 (1100)
-//   2047 x 50272 x 768                 160           194           132           177
+//   2047 x 50272 x 4096 fp16, 128 listed  760 (1110)   749 (1125)    645 (1310)    766 (1100)
+//   2047 x 50272 x 768                 160           182           132           177
 //   333 x 32007 x 1000                 32            36            37            36
 //   250 x 50272 x 768, 20 listed       30            30            34            39
 //   17 x 50272 x 2048 fp16, 64 listed  32            (206 MB of W at 6.3 TB/s, part of it cached)
@@ -684,8 +684,10 @@ struct Factor {
 
 // dz of a piece of the vocabulary, the forward's product with another epilogue:
 // dz[t][v - vbeg] = rowb exp(z - a), zeros in the columns past the vocabulary (and
-// where rowb is 0, whatever z is).  A label's own dz is -rowb (cross entropy); the listed tokens' of a
-// distillation follow (k_dz_listed).
+// where rowb is 0, whatever z is).  A label's own dz is -rowb (cross entropy; in the
+// persistent kernel put in place on the rows' way out: looked for at each 4 elements, 195 us
+// instead of 182 at 2047 x 50272 x 768); the listed tokens' of a distillation follow
+// (k_dz_listed).
 struct DzArgs {
   const uint16_t *h, *W;
   int64_t ldh, ldw, T, nv, C;
@@ -713,11 +715,10 @@ __device__ __forceinline__ uint16_t* dz_at(uint16_t* dz, int64_t zstep, int64_t 
   return dz + v / G_K * zstep + t * G_K + v % G_K;
 }
 
-// 4 consecutive tokens of a row, `left` of them within the vocabulary, the
-// label lab tokens on from the first; rest: what the rounding leaves (TWO)
+// dz of 4 consecutive tokens of a row; rest: what the rounding leaves (TWO)
 template <typename T8, bool TWO = false>
 __device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2, float b,
-                                         int64_t left, int lab, uint2* rest = nullptr) {
+                                         uint2* rest = nullptr) {
   typedef typename Half<T8>::t H;
   uint16_t o[4], l[4];
 #pragma unroll
@@ -726,28 +727,21 @@ __device__ __forceinline__ uint2 dz_pack(const f4_t& acc, float scale2, float a2
     o[r] = to16<T8>(x);
     if (TWO) l[r] = to16<T8>(x - (float)__builtin_bit_cast(H, o[r]));
   }
-  if ((unsigned)lab < 4u) {
-    const uint16_t y = to16<T8>(-b);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r == lab) {
-        o[r] = y;
-        if (TWO) l[r] = to16<T8>(-b - (float)__builtin_bit_cast(H, y));
-      }
-  }
-  if (left < 4) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r >= left) {
-        o[r] = 0;
-        if (TWO) l[r] = 0;
-      }
-  }
   if (TWO)
     *rest = b == 0.f ? make_uint2(0u, 0u)
                      : make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
   const uint2 u = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
   return b == 0.f ? make_uint2(0u, 0u) : u;
+}
+// element r of 4 becomes x
+__device__ __forceinline__ void set16(uint2& u, int r, uint32_t x) {
+  uint32_t& w = r < 2 ? u.x : u.y;
+  w = r & 1 ? (w & 0xffffu) | x << 16 : (w & 0xffff0000u) | x;
+}
+// the first `left` of 4 elements
+__device__ __forceinline__ uint2 first16(const uint2& u, int64_t left) {
+  return make_uint2(left >= 2 ? u.x : left == 1 ? u.x & 0xffffu : 0u,
+                    left >= 4 ? u.y : left == 3 ? u.y & 0xffffu : 0u);
 }
 
 template <typename T8, typename G>
@@ -774,10 +768,14 @@ __global__ __launch_bounds__(G::THREADS) void k_head_dz(const DzArgs p) {
     for (int i = 0; i < G::MI; ++i) {
       const int64_t v = vw + 16 * i + 4 * (lane >> 4);           // below dz_cols
       const int64_t o = y - v;
-      uint2 rest;
-      *(uint2*)dz_at(p.dz, p.zstep, t, v) = dz_pack<T8, true>(
-          acc[i][j], scale2, a2, b, p.nv - v, o >= 0 && o < 4 ? (int)o : -1, &rest);
-      if (p.T <= 64) *(uint2*)dz_at(p.dz, p.zstep, 64 + t, v) = rest;
+      uint2 rest, u = dz_pack<T8, true>(acc[i][j], scale2, a2, b, &rest);
+      if (o >= 0 && o < 4) {
+        const uint16_t x = to16<T8>(0.f - b);
+        set16(u, (int)o, x);
+        set16(rest, (int)o, to16<T8>(0.f - b - (float)__builtin_bit_cast(typename Half<T8>::t, x)));
+      }
+      *(uint2*)dz_at(p.dz, p.zstep, t, v) = first16(u, p.nv - v);
+      if (p.T <= 64) *(uint2*)dz_at(p.dz, p.zstep, 64 + t, v) = first16(rest, p.nv - v);
     }
   }
 }
@@ -845,7 +843,9 @@ struct DzJob {
       at[j] = ((const float*)q)[row] * LOG2E;
       b[j] = ((const float*)q)[64 + row];
       const int64_t y = p.labels ? ((const int64_t*)(q + 512))[row] - vt : -1;
-      lab[j] = y >= 0 && y < 256 ? (int)y : -4;
+      // (a row's label is written by the first of its 4 lanes)
+      const bool mine = y >= 0 && y < 256 && v0 + y < p.nv && (int)(y >> 5 & 1) == (wave >> 2);
+      lab[j] = mine && lane < 16 ? (int)y : -1;
     }
     const bool whole = v0 + 256 <= p.nv;
     g_each<4>([&](auto jj) __attribute__((always_inline)) {
@@ -853,13 +853,19 @@ struct DzJob {
       uint2 u[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        u[i] = dz_pack<T8>(acc.v[i][j], scale2, at[j], b[j],
-                           whole ? 4 : p.nv - (v0 + g_m(i, wave, lane)),
-                           lab[j] - g_m(i, wave, lane));
-      g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
-        const int64_t t = t0 + g_n(j, wave, 0) + r;
-        if (t < p.T) *(uint4*)dz_at(p.dz, p.zstep, t, v0 + m) = x;
-      });
+        u[i] = dz_pack<T8>(acc.v[i][j], scale2, at[j], b[j]);
+      if (!whole)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = first16(u[i], p.nv - (v0 + g_m(i, wave, lane)));
+      g_rows_out(
+          priv, u,
+          [&]() __attribute__((always_inline)) {
+            if (lab[j] >= 0) *g_rows_at(priv, lane, lab[j]) = to16<T8>(0.f - b[j]);
+          },
+          [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
+            const int64_t t = t0 + g_n(j, wave, 0) + r;
+            if (t < p.T) *(uint4*)dz_at(p.dz, p.zstep, t, v0 + m) = x;
+          });
     });
   }
 };
@@ -1093,7 +1099,7 @@ struct DwJob {
         u[i] = make_uint2(to16<T8>(f * a[0]) | (uint32_t)to16<T8>(f * a[1]) << 16,
                           to16<T8>(f * a[2]) | (uint32_t)to16<T8>(f * a[3]) << 16);
       }
-      g_rows_out(priv, u, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
+      g_rows_out(priv, u, [] {}, [&](int r, int m, const uint4& x) __attribute__((always_inline)) {
         const int64_t v = v0 + g_n(j, wave, 0) + r;
         if (v < p.nv && c0 + m < p.C)                            // C: a multiple of 8
           *(uint4*)(p.dW + v * p.ldo + c0 + m) = x;
@@ -1154,7 +1160,8 @@ static int64_t piece_of(int64_t T, int64_t V) {
 // workgroups times the 64-k stages of a part (1.2 us each, 6 more a tile), and
 // the fp32 partial sums, written and read back at about 4 TB/s.
 static int dh_splits(int64_t T, int64_t C, int64_t piece) {
-  const int64_t tiles = cdiv(C, 256) * cdiv(T, T <= 16 ? 16 : T <= 64 ? 64 : 256), stages = cdiv(piece, G_K);
+  const int64_t tiles = cdiv(C, 256) * cdiv(T, T <= 16 ? 16 : T <= 64 ? 64 : 256);
+  const int64_t stages = cdiv(piece, G_K);
   int64_t best = 1;
   double least = 0.;
   for (int64_t s = 1; s <= 256 && s * 4 <= stages; ++s) {
